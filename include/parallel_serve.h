@@ -399,6 +399,97 @@ int ps_prefill_attention(const void* q, const void* k_pool0, const void* v_pool0
                          int max_pages, int page_size, float scale, int dtype, int32_t* status,
                          ps_stream_t stream);
 
+/* ------------------------------------------------------------------------- *
+ * Head norms + rotary positions in one pass (an addition of this library).
+ * For token j (model m(j), position p = pos[j]) and every q and k head:
+ *   y = x / sqrt(mean(x^2) + eps) * w[m(j)]      (where w is given)
+ *   y = y with its first rotary_dim channels rotated by rope_cos / rope_sin[p]
+ * q, k: 128 contiguous channels per head, heads contiguous, token strides in
+ * elements (multiples of 8: views of one qkv row work); q_w / k_w [2][128]
+ * (nullable); rope tables [rope_len][rotary_dim / 2] fp32 (nullable: no
+ * rotation); rotary_dim a multiple of 16. Pairs are (i, i + rotary_dim / 2), or
+ * (2i, 2i + 1) when interleaved. fp32 arithmetic, one rounding at the end. A row
+ * may be written in place (q_out == q, k_out == k). q may be NULL with q_out. A
+ * position outside [0, rope_len) (negative, without tables) sets
+ * PS_ERR_BAD_INDEX and leaves the token's rows unwritten.
+ * ------------------------------------------------------------------------- */
+int ps_qk_norm_rope(const void* q, long long q_stride, const void* k, long long k_stride,
+                    void* q_out, long long qo_stride, void* k_out, long long ko_stride,
+                    const void* q_w, const void* k_w, float eps, const float* rope_cos,
+                    const float* rope_sin, int rope_len, int rotary_dim, int interleaved,
+                    const int32_t* pos, const int32_t* counts, int split_point, int M,
+                    int n_heads, int n_kv_heads, int dtype, int32_t* status, ps_stream_t stream);
+
+/* ------------------------------------------------------------------------- *
+ * 4-bit KV cache (an addition of this library; the reference keeps no cache).
+ * The 128 channels of one (position, KV head) are 4 groups of 32; a group holds
+ *   zero z = T(min), scale s = T((max - z) / 15) in the 16-bit model type T,
+ *   codes c = clamp(rint((x - z) / s), 0, 15), standing for s * c + z.
+ * Pools, per model and for K and V: codes uint8 [rows, n_kv_heads, len, 64] and
+ * meta T [rows, n_kv_heads, len, 4, 2] = (s, z); rows = slots with len = L_cap,
+ * or pages with len = page_size (power of two in [8, 4096]) and a block table
+ * int32 [table_rows, max_pages]. A row's 16 words of 8 codes (low nibble =
+ * lowest channel) are stored transposed: word w of group g is word 4 * w + g.
+ * Values beyond T saturate; a group with a NaN or an infinity reads back as NaN.
+ * A model without sequences has rows = 0 and NULL pointers.
+ * ------------------------------------------------------------------------- */
+typedef struct ps_kv4_pool {
+  void* k_codes;
+  void* k_meta;
+  void* v_codes;
+  void* v_meta;
+  int rows; /* slots or pages */
+} ps_kv4_pool_t;
+
+typedef struct ps_kv4_cache {
+  ps_kv4_pool_t pool[2];      /* per model */
+  const int32_t* block_table; /* NULL: contiguous slots */
+  int n_kv_heads;
+  int L_cap;                             /* contiguous */
+  int page_size, max_pages, table_rows;  /* paged */
+} ps_kv4_cache_t;
+
+/* Write token j's k and v at position pos[j] of its cache row: rows[j] (a slot
+ * of its model's pool, or a block-table row), or when rows == NULL slot
+ * j - (m ? c0 : 0), or block-table row j. q, norms and rotation as in
+ * ps_qk_norm_rope (q -> q_out in the same pass; all optional); k is normed and
+ * rotated in fp32 and quantised from there, v quantised as it is. Two tokens of
+ * one call must not share a position of a sequence. An index outside its range
+ * sets PS_ERR_BAD_INDEX and leaves that token unwritten (cache and q_out). */
+int ps_kv4_append(const void* q, long long q_stride, const void* k, long long k_stride,
+                  const void* v, long long v_stride, void* q_out, long long qo_stride,
+                  const ps_kv4_cache_t* cache, const void* q_w, const void* k_w, float eps,
+                  const float* rope_cos, const float* rope_sin, int rope_len, int rotary_dim,
+                  int interleaved, const int32_t* pos, const int32_t* rows,
+                  const int32_t* counts, int split_point, int M, int n_heads, int dtype,
+                  int32_t* status, ps_stream_t stream);
+
+/* Read cached rows back as 16-bit values, packed: sequence i (seqs[i] = {model,
+ * slot or block-table row, first position}) fills rows [cu[i], cu[i + 1]) of
+ * k_out and v_out [total, n_kv_heads, 128]. cu is nondecreasing; rows outside
+ * [cu[0], cu[n_seqs]) stay as they were, a row whose index is out of range sets
+ * PS_ERR_BAD_INDEX and stays too. */
+int ps_kv4_gather(const ps_kv4_cache_t* cache, const int32_t* seqs, const int32_t* cu, int n_seqs,
+                  int total, void* k_out, void* v_out, int dtype, int32_t* status,
+                  ps_stream_t stream);
+
+/* Decode attention over the 4-bit cache, grouped heads (n_heads a multiple of
+ * n_kv_heads; query head h reads KV head h / (n_heads / n_kv_heads)):
+ * out[j, h] = softmax(q[j, h] . K[0..pos[j]] * scale) V[0..pos[j]]. q
+ * [M, n_heads, 128] with a token stride, out [M, n_heads * 128]; rows as in
+ * ps_kv4_append; max_len bounds pos[j] + 1. A token whose position, row or page
+ * is out of range sets PS_ERR_BAD_INDEX and its output stays unwritten.
+ * The workspace starts with 4096 bytes of counters: zero them once before the
+ * first use, calls leave them zero, so calls of any shapes may follow one
+ * another on it. Calls that may overlap need workspaces of their own. */
+size_t ps_kv4_decode_attention_workspace_bytes(int M, int n_heads, int n_kv_heads, int max_len);
+
+int ps_kv4_decode_attention(const void* q, long long q_stride, const ps_kv4_cache_t* cache,
+                            void* out, const int32_t* pos, const int32_t* rows,
+                            const int32_t* counts, int split_point, int M, int n_heads,
+                            int max_len, float scale, int dtype, void* workspace,
+                            size_t workspace_bytes, int32_t* status, ps_stream_t stream);
+
 /* Segment self-attention with the reference's no-KV semantics
  * (kernel/src/two_model_block_routed.py:100-120, experiments/two_model_block.py:61-65):
  * every token of model m attends (non-causally) to all tokens of model m's

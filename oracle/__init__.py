@@ -21,3 +21,4 @@ reference serves) on small random models and checks ``decode_step`` and
 reference's Marlin-24 kernel lives in a vLLM fork that is absent).
 """
 from .ref_ops import *  # noqa: F401,F403
+from .kv4_ref import *  # noqa: F401,F403

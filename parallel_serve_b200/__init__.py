@@ -12,6 +12,8 @@ Public API (mirrors the reference's operator modules):
   TwoModelDecoder                                (KV-cache decode loop, CUDA graphs,
                                                   contiguous or paged KV)
   deltazip_linear                                (Route-A base + int4 2:4 delta)
+  KV4Pool, ops.kv4_append / kv4_gather / kv4_decode_attention (a KV cache held in 4 bits),
+  ops.qk_norm_rope               (additions of this library)
   pack_hf_llama, load_two_llama                  (experiments/real_weights_correctness.py:27-51)
   torch.ops.parallel_serve.*                     (the entry points as PyTorch custom operators)
 """
@@ -23,6 +25,7 @@ from .routed_linear_n2 import reference_routed_linear, routed_linear_n2
 from .two_model_block import TransformerBlock, TwoModelBlockBMM, TwoModelBlockFused
 from .two_model_block_routed import TwoModelBlockRouted
 from .deltazip import DeltaZipLinear, deltazip_linear
+from .kv4 import KV4Pool
 from .decoder import DecoderConfig, TwoModelDecoder
 from .loader import decoder_config_from_hf, load_two_llama, pack_hf_llama
 from . import torch_ops  # noqa: F401  (registers torch.ops.parallel_serve.*)
@@ -32,4 +35,5 @@ __all__ = [
     "TransformerBlock", "TwoModelBlockFused", "TwoModelBlockBMM", "TwoModelBlockRouted",
     "deltazip_linear", "DeltaZipLinear", "DecoderConfig", "TwoModelDecoder",
     "pack_hf_llama", "load_two_llama", "decoder_config_from_hf",
+    "KV4Pool",
 ]

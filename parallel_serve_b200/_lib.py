@@ -37,6 +37,7 @@ _p = ctypes.c_void_p
 _i = ctypes.c_int
 _f = ctypes.c_float
 _sz = ctypes.c_size_t
+_ll = ctypes.c_longlong
 
 
 class GemmEpilogue(ctypes.Structure):
@@ -50,6 +51,18 @@ class GemmEpilogue(ctypes.Structure):
         ("page_size", _i), ("kv_rows", _p), ("table_rows", _i), ("max_model_rows", _i),
         ("w_packed", _p), ("max_ctas", _i),
     ]
+
+
+class KV4PoolDesc(ctypes.Structure):
+    """ps_kv4_pool_t (one model's 4-bit K and V pools)."""
+    _fields_ = [("k_codes", _p), ("k_meta", _p), ("v_codes", _p), ("v_meta", _p), ("rows", _i)]
+
+
+class KV4CacheDesc(ctypes.Structure):
+    """ps_kv4_cache_t (both models' pools and their paging)."""
+    _fields_ = [("pool", KV4PoolDesc * 2), ("block_table", _p), ("n_kv_heads", _i),
+                ("L_cap", _i), ("page_size", _i), ("max_pages", _i), ("table_rows", _i)]
+
 
 PS_JOB_GEMM, PS_JOB_ALLREDUCE = 0, 1
 
@@ -93,6 +106,14 @@ SIGNATURES: dict[str, tuple] = {
     "ps_segment_attention": (_i, [_p, _p, _i, _i, _i, _p, _f, _i, _p, _p]),
     "ps_prefill_attention": (_i, [_p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _p, _i,
                                   _i, _i, _f, _i, _p, _p]),
+    "ps_qk_norm_rope": (_i, [_p, _ll, _p, _ll, _p, _ll, _p, _ll, _p, _p, _f, _p, _p, _i, _i, _i,
+                             _p, _p, _i, _i, _i, _i, _i, _p, _p]),
+    "ps_kv4_append": (_i, [_p, _ll, _p, _ll, _p, _ll, _p, _ll, ctypes.POINTER(KV4CacheDesc), _p,
+                           _p, _f, _p, _p, _i, _i, _i, _p, _p, _p, _i, _i, _i, _i, _p, _p]),
+    "ps_kv4_gather": (_i, [ctypes.POINTER(KV4CacheDesc), _p, _p, _i, _i, _p, _p, _i, _p, _p]),
+    "ps_kv4_decode_attention_workspace_bytes": (_sz, [_i, _i, _i, _i]),
+    "ps_kv4_decode_attention": (_i, [_p, _ll, ctypes.POINTER(KV4CacheDesc), _p, _p, _p, _p, _i,
+                                     _i, _i, _i, _f, _i, _p, _sz, _p, _p]),
     "ps_deltazip_packed_bytes": (_sz, [_i, _i]),
     "ps_deltazip_workspace_bytes": (_sz, [_i, _i, _i]),
     "ps_deltazip_linear": (_i, [_p, _p, _p, _p, _i, _i, _i, _i, _p, _i, _p, _sz, _p, _p]),

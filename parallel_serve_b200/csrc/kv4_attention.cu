@@ -1,0 +1,717 @@
+// Decode attention over the 4-bit KV cache (format: kv4.cuh), grouped heads,
+// contiguous or paged, both models in one launch.
+//
+// For one (token, KV head) the G query heads share the cached rows, so a row is
+// read once for up to 8 heads and both products run on mma.sync.m16n8k16 (fp16
+// inputs, fp32 sums), the 8 heads being the narrow N dimension:
+//   S[pos, head] = K[pos, ch] q[ch, head]         M = 16 positions
+//   O[ch, head]  = V^T[ch, pos] P[pos, head]      M = 16 channels
+// tcgen05 has nothing to offer here: its M is at least 64 rows of an operand in
+// shared memory, and the codes have to pass through registers to become 16-bit.
+//
+// Codes are never converted. A nibble masked in place inside a 16-bit lane is
+// the fp16 subnormal c * 2^-24 (bits 0..3) or c * 2^-20 (bits 4..7), exactly, so
+// 8 codes cost one shift and four ANDs; the factor 16 between the two is taken
+// by q (low-nibble channels times 16) and, for V, by the output channel. Scale
+// and zero stay outside the products, in fp32:
+//   S = sum_g s_g * (sum_{ch in g} q c) + z_g * (sum_{ch in g} q)
+//   O = sum_pos (P s_g) c  (P s_g / ref rounded to fp16: one rounding, 2^-12)
+//       + sum_pos P z_g    (fp32)
+// with ref a running power of two >= every s seen, rescaled like the softmax's
+// running maximum, so bf16 scales of any exponent fit. q is scaled per head by a
+// power of two into fp16's range (exact down to 2^-24 of the head's largest).
+//
+// S comes out of the instruction with positions in lanes and heads in registers,
+// P has to go in with heads in lanes: movmatrix transposes 8 x 8 tiles in
+// registers, so P never touches shared memory.
+//
+// Work: the (token, KV head, block of 8 heads, tile of 128 positions) space is
+// cut into equal contiguous ranges over one wave of CTAs from the device's own
+// lengths (a captured graph follows them). A producer warp streams tiles through
+// an mbarrier ring by bulk copies, 4 compute warps take 32 positions of each. The
+// last CTA to finish a piece of an item merges the pieces in order, so results
+// do not depend on timing.
+#include <cuda_runtime.h>
+
+#include "kv4.cuh"
+#include "ps_host.h"
+
+namespace ps {
+namespace kv4 {
+
+constexpr int kHB = 8;                       // query heads of one item
+constexpr int kWarps = 4;                    // compute warps
+constexpr int kWarpPos = 32;                 // positions of a tile per compute warp
+constexpr int kTile = kWarps * kWarpPos;     // 128
+constexpr int kStages = 2;
+constexpr int kCtasPerSm = 3;
+constexpr int kAttnThreads = (kWarps + 1) * 32;
+constexpr int kTileCodes = kTile * kCodeBytes;
+constexpr int kTileMeta = kTile * kMetaBytes;
+constexpr int kStageBytes = 2 * (kTileCodes + kTileMeta);  // K codes, K meta, V codes, V meta
+constexpr int kMaxEntries = 1024;            // prefix-sum entries of the token lengths
+constexpr int kMergeBytes = kWarps * kHB * (kD + 2) * 4;
+constexpr size_t kCounterBytes = 4096;       // arrival counters, zero at rest: one per CTA
+constexpr int kAttnSmem = kStages * kStageBytes + kMergeBytes + 256 + (kMaxEntries + 1) * 4 + 128;
+
+struct AttnArgs {
+  const void* q;  // [M, n_heads, 128], token stride q_stride
+  void* out;      // [M, n_heads * 128]
+  long long q_stride;
+  Pool pool[2];
+  const int32_t* pos;
+  const int32_t* rows;  // slot or block-table row of token j (nullable)
+  const int32_t* counts;
+  const int32_t* block_table;
+  float* ws_o;   // [2 per CTA][8][128]
+  float* ws_ml;  // [2 per CTA][8][2]
+  int32_t* counter;
+  int32_t* status;
+  int split_point, M, n_heads, n_kv, group, hblocks, max_len;
+  int L_cap, page_size, page_shift, max_pages, table_rows;
+  int per_entry;  // tokens per prefix-sum entry
+  float scale_log2;
+};
+
+PS_DEV void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                     uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+PS_DEV uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
+PS_DEV uint32_t half2_bits(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Cached positions of token j, 0 when its position or home is out of range.
+PS_DEV int token_len(const AttnArgs& a, int j, int c0) {
+  const int p = a.pos[j];
+  const int m = j >= c0 ? 1 : 0;
+  const int home = a.rows ? a.rows[j] : (a.block_table ? j : j - (m ? c0 : 0));
+  const int cap = a.block_table ? a.max_pages * a.page_size : a.L_cap;
+  const int pool_rows = m ? a.pool[1].rows : a.pool[0].rows;
+  const bool ok = p >= 0 && p < a.max_len && p < cap && home >= 0 && pool_rows > 0 &&
+                  home < (a.block_table ? a.table_rows : pool_rows);
+  return ok ? p + 1 : 0;
+}
+
+PS_DEV int tiles_of(int len) { return (len + kTile - 1) / kTile; }
+
+// One piece of a CTA's range: tiles [t0, t1) of item (token j, KV head kvh,
+// head block hb).
+struct Piece {
+  int j, len, kvh, hb, t0, t1, slot, nsplit;
+  long long first_cta, item_start, end;
+};
+
+PS_DEV Piece piece_at(const AttnArgs& a, const int32_t* P, int entries, int c0, long long S,
+                      long long g, long long g1, int b) {
+  const int HB = a.n_kv * a.hblocks;
+  int lo = 0, hi = entries - 1;  // last entry that starts at or before g
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if ((long long)P[mid] * HB <= g) lo = mid; else hi = mid - 1;
+  }
+  long long at = (long long)P[lo] * HB;
+  int j = lo * a.per_entry, len = token_len(a, j, c0);
+  while ((long long)tiles_of(len) * HB + at <= g && j + 1 < a.M) {  // within the entry
+    at += (long long)tiles_of(len) * HB;
+    len = token_len(a, ++j, c0);
+  }
+  Piece p;
+  p.j = j;
+  p.len = len;
+  const int nt = max(1, tiles_of(len));
+  const int it = (int)((g - at) / nt);
+  p.kvh = it / a.hblocks;
+  p.hb = it % a.hblocks;
+  p.t0 = (int)((g - at) % nt);
+  p.item_start = at + (long long)it * nt;
+  const long long iend = p.item_start + nt;
+  p.end = g1 < iend ? g1 : iend;
+  p.t1 = p.t0 + (int)(p.end - g);
+  p.first_cta = p.item_start / S;
+  p.nsplit = (int)((iend - 1) / S - p.first_cta) + 1;
+  p.slot = g == (long long)b * S ? 0 : 1;
+  return p;
+}
+
+// Merged softmax state of up to 8 heads x 128 channels, one thread a channel.
+template <typename T>
+__global__ void __launch_bounds__(kAttnThreads, kCtasPerSm)
+    kv4_decode_attention_kernel(const AttnArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem =
+      reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127));
+  float* so = reinterpret_cast<float*>(smem + kStages * kStageBytes);  // [warp][head][128]
+  float* sml = so + kWarps * kHB * kD;                                 // [warp][head][2]
+  uint64_t* full = reinterpret_cast<uint64_t*>(sml + kWarps * kHB * 2);
+  uint64_t* empty = full + kStages;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(empty + kStages);
+  volatile int* last_flag = abort_flag + 1;
+  volatile int* stage_bad = last_flag + 1;                         // [kStages]
+  int* wsum = const_cast<int*>(stage_bad) + kStages;               // [8]
+  int32_t* P = reinterpret_cast<int32_t*>(smem + kStages * kStageBytes + kMergeBytes + 256);
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int b = blockIdx.x;
+  pdl_wait();
+  pdl_launch_dependents();
+  const int c0 = a.counts ? a.counts[0] : a.split_point;
+
+  // Tiles per entry of tokens, then their prefix sums.
+  const int entries = (a.M + a.per_entry - 1) / a.per_entry;
+  for (int e = tid; e < entries; e += kAttnThreads) {
+    int n = 0;
+    for (int j = e * a.per_entry; j < min(a.M, (e + 1) * a.per_entry); ++j) {
+      const int len = token_len(a, j, c0);
+      if (len == 0 && b == 0) set_status(a.status, PS_ERR_BAD_INDEX);
+      n += tiles_of(len);
+    }
+    P[e + 1] = n;
+  }
+  if (tid == 0) {
+    P[0] = 0;
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(full + i, 1);
+      mbar_init(empty + i, kWarps);
+    }
+    abort_flag[0] = 0;
+    fence_mbar_init();
+  }
+  __syncthreads();
+  {
+    const int per = (entries + kAttnThreads - 1) / kAttnThreads;
+    const int e0 = min(entries, tid * per), e1 = min(entries, e0 + per);
+    int run = 0;
+    for (int e = e0; e < e1; ++e) run += P[e + 1];
+    int incl = run;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    if (lane == 31) wsum[warp] = incl;
+    __syncthreads();
+    int acc = incl - run;
+    for (int w = 0; w < warp; ++w) acc += wsum[w];
+    __syncthreads();
+    for (int e = e0; e < e1; ++e) {
+      acc += P[e + 1];
+      P[e + 1] = acc;
+    }
+  }
+  __syncthreads();
+  const long long W = (long long)P[entries] * a.n_kv * a.hblocks;
+  const long long S = (W + gridDim.x - 1) / gridDim.x;
+  const long long g0 = (long long)b * S;
+  const long long g1 = g0 + S < W ? g0 + S : W;
+  if (g0 >= g1) return;
+
+  if (warp == kWarps) {
+    // -------------------------------------------------------------- producer
+    const uint64_t pol = l2_policy_evict_first();
+    int gs = 0;
+    bool dead = false;
+    for (long long g = g0; g < g1 && !dead;) {
+      const Piece pc = piece_at(a, P, entries, c0, S, g, g1, b);
+      const int m = pc.j >= c0 ? 1 : 0;
+      const Pool pool = m ? a.pool[1] : a.pool[0];
+      const int home = a.rows ? a.rows[pc.j] : (a.block_table ? pc.j : pc.j - (m ? c0 : 0));
+      for (int t = pc.t0; t < pc.t1; ++t, ++gs) {
+        const int st = gs % kStages;
+        if (!mbar_wait(empty + st, ((gs / kStages) & 1) ^ 1, a.status)) abort_flag[0] = 1;
+        dead = __any_sync(0xffffffffu, abort_flag[0] != 0);
+        if (dead) break;
+        const int pos0 = t * kTile;
+        const int npos = min(kTile, pc.len - pos0);
+        uint8_t* buf = smem + st * kStageBytes;
+        if (!a.block_table) {
+          if (lane == 0) {
+            stage_bad[st] = 0;
+            mbar_arrive_expect_tx(full + st, (uint32_t)npos * 2 * (kCodeBytes + kMetaBytes));
+          }
+          __syncwarp();
+          const size_t row = ((size_t)home * a.n_kv + pc.kvh) * a.L_cap + pos0;
+          if (lane == 0)
+            bulk_load(buf, pool.k_codes + row * kCodeBytes, npos * kCodeBytes, full + st, pol);
+          if (lane == 1)
+            bulk_load(buf + kTileCodes, pool.k_meta + row * kMetaBytes, npos * kMetaBytes,
+                      full + st, pol);
+          if (lane == 2)
+            bulk_load(buf + kTileCodes + kTileMeta, pool.v_codes + row * kCodeBytes,
+                      npos * kCodeBytes, full + st, pol);
+          if (lane == 3)
+            bulk_load(buf + 2 * kTileCodes + kTileMeta, pool.v_meta + row * kMetaBytes,
+                      npos * kMetaBytes, full + st, pol);
+        } else {
+          // one run per page (128 % page_size == 0 or page_size % 128 == 0, so
+          // runs start at multiples of page_size or fill the tile): lane l
+          // takes run l (at most 16 of them)
+          const int run = min(a.page_size, kTile);
+          const int nrun = (npos + run - 1) / run;
+          int page = 0;
+          bool bad = false;
+          if (lane < nrun) {
+            const int pi = (pos0 + lane * run) >> a.page_shift;
+            page = a.block_table[(size_t)home * a.max_pages + pi];
+            bad = page < 0 || page >= pool.rows;
+            if (bad) page = 0;  // read a page that exists; the piece's output is dropped
+          }
+          const bool any_bad = __any_sync(0xffffffffu, bad);
+          if (lane == 0) {
+            if (any_bad) set_status(a.status, PS_ERR_BAD_INDEX);
+            stage_bad[st] = any_bad ? 1 : 0;
+            mbar_arrive_expect_tx(full + st, (uint32_t)npos * 2 * (kCodeBytes + kMetaBytes));
+          }
+          __syncwarp();
+          if (lane < nrun) {
+            const int o = lane * run;
+            const int n = min(run, npos - o);
+            const size_t row = ((size_t)page * a.n_kv + pc.kvh) * a.page_size +
+                               ((pos0 + o) & (a.page_size - 1));
+            bulk_load(buf + o * kCodeBytes, pool.k_codes + row * kCodeBytes, n * kCodeBytes,
+                      full + st, pol);
+            bulk_load(buf + kTileCodes + o * kMetaBytes, pool.k_meta + row * kMetaBytes,
+                      n * kMetaBytes, full + st, pol);
+            bulk_load(buf + kTileCodes + kTileMeta + o * kCodeBytes,
+                      pool.v_codes + row * kCodeBytes, n * kCodeBytes, full + st, pol);
+            bulk_load(buf + 2 * kTileCodes + kTileMeta + o * kMetaBytes,
+                      pool.v_meta + row * kMetaBytes, n * kMetaBytes, full + st, pol);
+          }
+        }
+      }
+      __syncwarp();
+      g = pc.end;
+    }
+    if (dead && lane == 0) {  // let every issued copy land before the CTA exits
+      for (int st = 0; st < kStages && st < gs; ++st) {
+        const int last = st + kStages * ((gs - 1 - st) / kStages);
+        mbar_wait(full + st, (last / kStages) & 1, a.status);
+      }
+    }
+    return;
+  }
+
+  // ---------------------------------------------------------------- compute
+  const int gr = lane >> 2, t4 = lane & 3;
+  // Row gr of a 16-position tile is position sig(gr) of its 8: pairs (2i, 2i+1)
+  // keep their places up to order, and rows 0, 2, 4, 6 alternate between even
+  // and odd positions, which halves the bank conflicts of the V reads.
+  const int sig = gr ^ ((gr >> 1) & 1);
+  const int sig0 = (2 * t4) ^ (t4 & 1), sig1 = (2 * t4 + 1) ^ (t4 & 1);
+  const uint32_t vsel = (gr & 1) ? 0x7632u : 0x5410u;
+  int gs = 0;
+  bool dead = false;
+  for (long long g = g0; g < g1;) {
+    const Piece pc = piece_at(a, P, entries, c0, S, g, g1, b);
+    const int nh = min(kHB, a.group - pc.hb * kHB);
+    const int head0 = pc.kvh * a.group + pc.hb * kHB;
+    const T* qrow = reinterpret_cast<const T*>(a.q) + (size_t)pc.j * a.q_stride;
+
+    // q as B fragments: lane (gr, t4) holds head gr, channels 32 g + 8 t4 + i.
+    uint32_t qb[4][4];     // [group][(i=0,4) (1,5) (2,6) (3,7)]
+    float qs[4][2];        // sum of q over the group, for heads 2 t4, 2 t4 + 1
+    float qf[2];           // what S is multiplied by for those heads
+    {
+      uint4 raw[4];
+      const bool live = gr < nh;
+#pragma unroll
+      for (int gi = 0; gi < 4; ++gi)
+        raw[gi] = live ? *reinterpret_cast<const uint4*>(qrow + (size_t)(head0 + gr) * kD +
+                                                         gi * kGroup + 8 * t4)
+                       : make_uint4(0, 0, 0, 0);
+      float mx = 0.f, sum[4];
+#pragma unroll
+      for (int gi = 0; gi < 4; ++gi) {
+        const uint32_t u[4] = {raw[gi].x, raw[gi].y, raw[gi].z, raw[gi].w};
+        sum[gi] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float x, y;
+          unpack2<T>(u[i], x, y);
+          mx = fmaxf(mx, fmaxf(fabsf(x), fabsf(y)));
+          sum[gi] += x + y;
+        }
+      }
+#pragma unroll
+      for (int o = 1; o <= 2; o <<= 1) {
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+#pragma unroll
+        for (int gi = 0; gi < 4; ++gi) sum[gi] += __shfl_xor_sync(0xffffffffu, sum[gi], o);
+      }
+      int e = (int)(__float_as_uint(mx) >> 23) - 127;  // max |q| in [2^e, 2^(e+1))
+      e = max(-100, min(100, e));
+      const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+#pragma unroll
+      for (int gi = 0; gi < 4; ++gi) {
+        const uint32_t u[4] = {raw[gi].x, raw[gi].y, raw[gi].z, raw[gi].w};
+        float f[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) unpack2<T>(u[i], f[2 * i], f[2 * i + 1]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float k = (i & 1) ? down : 16.f * down;  // low nibbles: channels i even
+          qb[gi][i] = half2_bits(f[i] * k, f[i + 4] * k);
+        }
+      }
+      const float up = __uint_as_float((uint32_t)(127 + e) << 23) * 1048576.f * a.scale_log2;
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int src = (2 * t4 + x) * 4;  // a lane of head 2 t4 + x
+        qf[x] = __shfl_sync(0xffffffffu, up, src);
+#pragma unroll
+        for (int gi = 0; gi < 4; ++gi)
+          qs[gi][x] = __shfl_sync(0xffffffffu, sum[gi], src) * a.scale_log2;
+      }
+    }
+
+    float o[8][4];   // [2 g + half][channel pair x head]: see the store below
+    float zs[4][2];  // sum over positions of P z_g (this lane's rows)
+    float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
+    float ref = __uint_as_float(27u << 23);  // 2^-100
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) o[i][k] = 0.f;
+#pragma unroll
+    for (int gi = 0; gi < 4; ++gi) zs[gi][0] = zs[gi][1] = 0.f;
+    bool bad = false;
+
+    for (int t = pc.t0; t < pc.t1 && !dead; ++t, ++gs) {
+      const int st = gs % kStages;
+      const bool got = !abort_flag[0] && mbar_wait(full + st, (gs / kStages) & 1, a.status);
+      if (!__all_sync(0xffffffffu, got)) {
+        abort_flag[0] = 1;
+        dead = true;
+        break;
+      }
+      bad |= stage_bad[st] != 0;
+      const int left = pc.len - t * kTile - warp * kWarpPos;  // live positions of this warp
+      if (left > 0) {
+        const uint8_t* kc = smem + st * kStageBytes + warp * kWarpPos * kCodeBytes;
+        const uint8_t* km = smem + st * kStageBytes + kTileCodes + warp * kWarpPos * kMetaBytes;
+        const uint8_t* vc = kc + kTileCodes + kTileMeta;
+        const uint8_t* vm = km + kTileCodes + kTileMeta;
+        float s[2][4];
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
+          const int r0 = mt * 16 + sig, r1 = r0 + 8;
+          const uint4 w0 = *reinterpret_cast<const uint4*>(kc + r0 * kCodeBytes + t4 * 16);
+          const uint4 w1 = *reinterpret_cast<const uint4*>(kc + r1 * kCodeBytes + t4 * 16);
+          const uint4 e0 = *reinterpret_cast<const uint4*>(km + r0 * kMetaBytes);
+          const uint4 e1 = *reinterpret_cast<const uint4*>(km + r1 * kMetaBytes);
+          const uint32_t a0[4] = {w0.x, w0.y, w0.z, w0.w}, a1[4] = {w1.x, w1.y, w1.z, w1.w};
+          const uint32_t p0[4] = {e0.x, e0.y, e0.z, e0.w}, p1[4] = {e1.x, e1.y, e1.z, e1.w};
+          float qk[4] = {0.f, 0.f, 0.f, 0.f}, qz[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int gi = 0; gi < 4; ++gi) {
+            float c[4] = {0.f, 0.f, 0.f, 0.f};
+            const uint32_t h0 = a0[gi] >> 8, h1 = a1[gi] >> 8;
+            mma16816(c, a0[gi] & 0x000f000fu, a1[gi] & 0x000f000fu, a0[gi] & 0x00f000f0u,
+                     a1[gi] & 0x00f000f0u, qb[gi][0], qb[gi][1]);
+            mma16816(c, h0 & 0x000f000fu, h1 & 0x000f000fu, h0 & 0x00f000f0u, h1 & 0x00f000f0u,
+                     qb[gi][2], qb[gi][3]);
+            float s0, z0, s1, z1;
+            unpack2<T>(p0[gi], s0, z0);
+            unpack2<T>(p1[gi], s1, z1);
+            qk[0] += s0 * c[0], qk[1] += s0 * c[1], qk[2] += s1 * c[2], qk[3] += s1 * c[3];
+            qz[0] += z0 * qs[gi][0], qz[1] += z0 * qs[gi][1];
+            qz[2] += z1 * qs[gi][0], qz[3] += z1 * qs[gi][1];
+          }
+          s[mt][0] = r0 < left ? qk[0] * qf[0] + qz[0] : -INFINITY;
+          s[mt][1] = r0 < left ? qk[1] * qf[1] + qz[1] : -INFINITY;
+          s[mt][2] = r1 < left ? qk[2] * qf[0] + qz[2] : -INFINITY;
+          s[mt][3] = r1 < left ? qk[3] * qf[1] + qz[3] : -INFINITY;
+        }
+        // V's meta of this lane's rows; rows past the end count as s = z = 0
+        float vs[2][2][4], vz[2][2][4];
+        float smax = 0.f;
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const int r = mt * 16 + k * 8 + sig;
+            const uint4 e = *reinterpret_cast<const uint4*>(vm + r * kMetaBytes);
+            const uint32_t p[4] = {e.x, e.y, e.z, e.w};
+#pragma unroll
+            for (int gi = 0; gi < 4; ++gi) {
+              unpack2<T>(r < left ? p[gi] : 0u, vs[mt][k][gi], vz[mt][k][gi]);
+              smax = fmaxf(smax, vs[mt][k][gi]);
+            }
+          }
+        float mx[2] = {fmaxf(fmaxf(s[0][0], s[0][2]), fmaxf(s[1][0], s[1][2])),
+                       fmaxf(fmaxf(s[0][1], s[0][3]), fmaxf(s[1][1], s[1][3]))};
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int off = 4; off <= 16; off <<= 1)
+            mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], off));
+        // the next power of two above the largest scale of the warp's rows
+        const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(smax)) & 0x7f800000u;
+        const float ref_new = fmaxf(ref, __uint_as_float(min(top + 0x00800000u, 0x7f000000u)));
+        const float m_new[2] = {fmaxf(m_run[0], mx[0]), fmaxf(m_run[1], mx[1])};
+        float al[2];
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          al[x] = m_new[x] == -INFINITY ? 1.f : exp2f(m_run[x] - m_new[x]);
+        const float shrink = ref / ref_new;
+        if (__any_sync(0xffffffffu, al[0] != 1.f || al[1] != 1.f || shrink != 1.f)) {
+          const float f0 = al[0] * shrink, f1 = al[1] * shrink;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) o[i][0] *= f0, o[i][1] *= f1, o[i][2] *= f0, o[i][3] *= f1;
+#pragma unroll
+          for (int gi = 0; gi < 4; ++gi) zs[gi][0] *= al[0], zs[gi][1] *= al[1];
+          l_run[0] *= al[0];
+          l_run[1] *= al[1];
+        }
+        m_run[0] = m_new[0];
+        m_run[1] = m_new[1];
+        ref = ref_new;
+        const float inv = 1.f / ref;  // a power of two: exact
+        const float mu[2] = {m_new[0] == -INFINITY ? 0.f : m_new[0],
+                             m_new[1] == -INFINITY ? 0.f : m_new[1]};
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
+          float p[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) p[k] = exp2f(s[mt][k] - mu[k & 1]);
+          l_run[0] += p[0] + p[2];
+          l_run[1] += p[1] + p[3];
+          // V codes of positions (2 t4, 2 t4 + 1) and (2 t4 + 8, 2 t4 + 9) in row order
+          uint32_t v[4][4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int r = mt * 16 + (k >> 1) * 8 + ((k & 1) ? sig1 : sig0);
+            const uint4 w = *reinterpret_cast<const uint4*>(vc + r * kCodeBytes + (gr >> 1) * 16);
+            v[k][0] = w.x, v[k][1] = w.y, v[k][2] = w.z, v[k][3] = w.w;
+          }
+#pragma unroll
+          for (int gi = 0; gi < 4; ++gi) {
+            zs[gi][0] += p[0] * vz[mt][0][gi] + p[2] * vz[mt][1][gi];
+            zs[gi][1] += p[1] * vz[mt][0][gi] + p[3] * vz[mt][1][gi];
+            const float w0 = vs[mt][0][gi] * inv, w1 = vs[mt][1][gi] * inv;
+            const uint32_t b0 = transpose8x8(half2_bits(p[0] * w0, p[1] * w0));
+            const uint32_t b1 = transpose8x8(half2_bits(p[2] * w1, p[3] * w1));
+            // halfword gr of the group: channels 4 gr + 0..3 of both positions
+            const uint32_t x = __byte_perm(v[0][gi], v[1][gi], vsel);
+            const uint32_t y = __byte_perm(v[2][gi], v[3][gi], vsel);
+            const uint32_t xh = x >> 8, yh = y >> 8;
+            mma16816(o[2 * gi], x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu,
+                     y & 0x00f000f0u, b0, b1);
+            mma16816(o[2 * gi + 1], xh & 0x000f000fu, xh & 0x00f000f0u, yh & 0x000f000fu,
+                     yh & 0x00f000f0u, b0, b1);
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(empty + st);
+    }
+
+    // ---- merge the four warps. o[2 gi + x][0..1]: channel 32 gi + 4 gr + 2 x,
+    // heads 2 t4, 2 t4 + 1; [2..3]: the next channel (a high nibble).
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int off = 4; off <= 16; off <<= 1) {
+        l_run[x] += __shfl_xor_sync(0xffffffffu, l_run[x], off);
+#pragma unroll
+        for (int gi = 0; gi < 4; ++gi)
+          zs[gi][x] += __shfl_xor_sync(0xffffffffu, zs[gi][x], off);
+      }
+    const float lo24 = ref * 16777216.f, hi20 = ref * 1048576.f;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int head = 2 * t4 + x;
+      if (gr == 0) {
+        sml[(warp * kHB + head) * 2] = m_run[x];
+        sml[(warp * kHB + head) * 2 + 1] = l_run[x];
+      }
+#pragma unroll
+      for (int gi = 0; gi < 4; ++gi) {
+        const float z = zs[gi][x];
+        float4 f;
+        f.x = o[2 * gi][x] * lo24 + z;
+        f.y = o[2 * gi][2 + x] * hi20 + z;
+        f.z = o[2 * gi + 1][x] * lo24 + z;
+        f.w = o[2 * gi + 1][2 + x] * hi20 + z;
+        *reinterpret_cast<float4*>(so + (warp * kHB + head) * kD + gi * kGroup + 4 * gr) = f;
+      }
+    }
+    dead = named_bar_or(1, kWarps * 32, dead);
+    bad |= dead;
+    const int ch = tid;
+    T* out = reinterpret_cast<T*>(a.out) + ((size_t)pc.j * a.n_heads + head0) * kD + ch;
+    const size_t slot = (size_t)b * 2 + pc.slot;
+    for (int h = 0; h < nh; ++h) {
+      float M = -INFINITY, L = 0.f, O = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) M = fmaxf(M, sml[(w * kHB + h) * 2]);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float mw = sml[(w * kHB + h) * 2];
+        const float f = mw == -INFINITY ? 0.f : exp2f(mw - M);
+        L += sml[(w * kHB + h) * 2 + 1] * f;
+        O += so[(w * kHB + h) * kD + ch] * f;
+      }
+      if (pc.nsplit == 1) {
+        if (!bad) out[h * kD] = from_f32<T>(O / L);
+      } else {
+        __stcg(a.ws_o + (slot * kHB + h) * kD + ch, O);
+        if (ch == 0) {
+          __stcg(a.ws_ml + (slot * kHB + h) * 2, M);
+          __stcg(a.ws_ml + (slot * kHB + h) * 2 + 1, bad ? -1.f : L);  // l < 0: a bad piece
+        }
+      }
+    }
+    named_bar_sync(1, kWarps * 32);
+    if (pc.nsplit > 1) {
+      // ranges are contiguous, so at most one item continues past each CTA's
+      // end: its first CTA's number identifies it
+      int32_t* counter = a.counter + pc.first_cta;
+      if (tid == 0) {
+        fence_acq_rel_gpu();
+        const int old = atom_add_acq_rel_gpu(counter, 1);
+        const int last = old + 1 == pc.nsplit ? 1 : 0;
+        if (last) *counter = 0;
+        last_flag[0] = last;
+      }
+      named_bar_sync(1, kWarps * 32);
+      if (last_flag[0]) {
+        // pieces in CTA order; CTA c's piece of this item is its first unless
+        // the item starts inside c's range
+        for (int h = 0; h < nh; ++h) {
+          float M = -INFINITY, L = 0.f, O = 0.f;
+          bool any_bad = false;
+          for (int c = 0; c < pc.nsplit; ++c) {
+            const long long cb = pc.first_cta + c;
+            const size_t sl = (size_t)cb * 2 + (pc.item_start <= cb * S ? 0 : 1);
+            const float mc = __ldcg(a.ws_ml + (sl * kHB + h) * 2);
+            const float lc = __ldcg(a.ws_ml + (sl * kHB + h) * 2 + 1);
+            const float oc = __ldcg(a.ws_o + (sl * kHB + h) * kD + ch);
+            any_bad |= lc < 0.f;
+            const float mn = fmaxf(M, mc);
+            const float fa = M == -INFINITY ? 0.f : exp2f(M - mn);
+            const float fb = mc == -INFINITY ? 0.f : exp2f(mc - mn);
+            L = L * fa + lc * fb;
+            O = O * fa + oc * fb;
+            M = mn;
+          }
+          if (!any_bad) out[h * kD] = from_f32<T>(O / L);
+        }
+      }
+    }
+    named_bar_sync(1, kWarps * 32);  // so / sml / last_flag are reused
+    g = pc.end;
+  }
+}
+
+struct AttnPlan {
+  int grid, per_entry;
+  size_t ml_bytes, o_bytes;
+  size_t bytes() const { return kCounterBytes + ml_bytes + o_bytes; }
+};
+
+// One wave of CTAs, fewer when the longest lengths give fewer tiles.
+static AttnPlan plan_attention(int M, int n_kv, int hblocks, int max_len, int device) {
+  AttnPlan p;
+  const long long tiles = (long long)M * n_kv * hblocks * cdiv(max_len, kTile);
+  long long wave = (long long)kCtasPerSm * sm_count(device);
+  if (wave > (long long)(kCounterBytes / 4)) wave = kCounterBytes / 4;
+  p.grid = (int)(tiles < wave ? tiles : wave);
+  p.per_entry = cdiv(M, kMaxEntries);
+  p.ml_bytes = ((size_t)p.grid * 2 * kHB * 2 * 4 + 255) / 256 * 256;
+  p.o_bytes = (size_t)p.grid * 2 * kHB * kD * 4;
+  return p;
+}
+
+}  // namespace kv4
+}  // namespace ps
+
+using namespace ps;
+
+extern "C" size_t ps_kv4_decode_attention_workspace_bytes(int M, int n_heads, int n_kv_heads,
+                                                          int max_len) {
+  if (M <= 0 || n_kv_heads <= 0 || n_heads <= 0 || n_heads % n_kv_heads || max_len <= 0) return 0;
+  const kv4::AttnPlan p = kv4::plan_attention(
+      M, n_kv_heads, cdiv(n_heads / n_kv_heads, kv4::kHB), max_len, current_device());
+  return p.bytes();
+}
+
+extern "C" int ps_kv4_decode_attention(const void* q, long long q_stride,
+                                       const ps_kv4_cache_t* cache, void* out, const int32_t* pos,
+                                       const int32_t* rows, const int32_t* counts,
+                                       int split_point, int M, int n_heads, int max_len,
+                                       float scale, int dtype, void* workspace,
+                                       size_t workspace_bytes, int32_t* status,
+                                       ps_stream_t stream) {
+  PS_CHECK_ARG(kv4::valid_cache(cache));
+  const int n_kv = cache->n_kv_heads;
+  PS_CHECK_ARG(M >= 0 && n_heads > 0 && n_heads % n_kv == 0 && max_len > 0);
+  PS_CHECK_ARG(max_len <= (cache->block_table ? cache->max_pages * cache->page_size : cache->L_cap));
+  PS_CHECK_ARG(dtype == PS_DTYPE_F16 || dtype == PS_DTYPE_BF16);
+  if (!counts) PS_CHECK_ARG(split_point >= 0 && split_point <= M);
+  if (M == 0) return PS_OK;
+  PS_CHECK_ARG(q && out && pos && aligned16(q) && q_stride >= (long long)n_heads * kv4::kD &&
+               q_stride % 8 == 0);
+  PS_CHECK_ARG(!cache->block_table || rows || cache->table_rows >= M);
+  const int hblocks = cdiv(n_heads / n_kv, kv4::kHB);
+  // the prefix sums of tiles are 32-bit
+  if ((long long)M * cdiv(max_len, kv4::kTile) > (1ll << 30)) return PS_ERR_UNSUPPORTED;
+  const int device = current_device();
+  if (!is_sm100(device)) return PS_ERR_UNSUPPORTED;
+  const kv4::AttnPlan p = kv4::plan_attention(M, n_kv, hblocks, max_len, device);
+  if (!workspace || workspace_bytes < p.bytes()) return PS_ERR_WORKSPACE;
+  PS_CHECK_ARG(aligned16(workspace));
+  kv4::AttnArgs a{};
+  a.q = q;
+  a.out = out;
+  a.q_stride = q_stride;
+  a.pool[0] = kv4::to_pool(&cache->pool[0]);
+  a.pool[1] = kv4::to_pool(&cache->pool[1]);
+  a.pos = pos;
+  a.rows = rows;
+  a.counts = counts;
+  a.block_table = cache->block_table;
+  char* ws = reinterpret_cast<char*>(workspace);
+  a.counter = reinterpret_cast<int32_t*>(ws);
+  a.ws_ml = reinterpret_cast<float*>(ws + kv4::kCounterBytes);
+  a.ws_o = reinterpret_cast<float*>(ws + kv4::kCounterBytes + p.ml_bytes);
+  a.status = status;
+  a.split_point = split_point;
+  a.M = M;
+  a.n_heads = n_heads;
+  a.n_kv = n_kv;
+  a.group = n_heads / n_kv;
+  a.hblocks = hblocks;
+  a.max_len = max_len;
+  a.L_cap = cache->L_cap;
+  a.page_size = cache->page_size;
+  a.page_shift = 0;
+  while (cache->block_table && (1 << a.page_shift) < cache->page_size) ++a.page_shift;
+  a.max_pages = cache->max_pages;
+  a.table_rows = cache->table_rows;
+  a.per_entry = p.per_entry;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (dtype == PS_DTYPE_BF16) {
+    PS_CUDA_RET(allow_dynamic_smem(kv4::kv4_decode_attention_kernel<__nv_bfloat16>, kv4::kAttnSmem));
+    PS_CUDA_RET(launch(kv4::kv4_decode_attention_kernel<__nv_bfloat16>, dim3(p.grid),
+                       dim3(kv4::kAttnThreads), kv4::kAttnSmem, st, a));
+  } else {
+    PS_CUDA_RET(allow_dynamic_smem(kv4::kv4_decode_attention_kernel<__half>, kv4::kAttnSmem));
+    PS_CUDA_RET(launch(kv4::kv4_decode_attention_kernel<__half>, dim3(p.grid),
+                       dim3(kv4::kAttnThreads), kv4::kAttnSmem, st, a));
+  }
+  return PS_OK;
+}

@@ -379,3 +379,342 @@ def positions_routed(seq_len: torch.Tensor, perm: torch.Tensor | None, out: torc
     check(lib.ps_positions_routed(ptr(seq_len), ptr(perm), ptr(out), out.numel(),
                                   _lib.stream_handle(seq_len.device)), "ps_positions_routed")
     return out
+
+
+# ---------------------------------------------------------------- 4-bit KV cache, head norms
+
+_HD = 128
+
+
+def _heads(t: torch.Tensor, name: str) -> tuple[int, int, int]:
+    """(tokens, heads, token stride) of ``[tokens, heads, 128]`` or ``[tokens,
+    heads * 128]`` whose heads lie one after another (views of a qkv row do)."""
+    if not t.is_cuda:
+        raise ValueError("parallel-serve ops take CUDA tensors")
+    if t.dim() == 3:
+        n, h, d = t.shape
+        ok = d == _HD and t.stride(2) == 1 and (h == 1 or t.stride(1) == _HD)
+    elif t.dim() == 2:
+        n, d = t.shape
+        h = d // _HD
+        ok = d % _HD == 0 and t.stride(1) == 1
+    else:
+        ok = False
+    if not ok or h == 0:
+        raise ValueError(f"{name} must be [tokens, heads, 128] (or [tokens, heads * 128]) with "
+                         "contiguous heads")
+    stride = t.stride(0) if n > 1 else h * _HD
+    if stride < h * _HD or stride % 8:
+        raise ValueError(f"{name}: token stride {stride} must be a multiple of 8 and hold every head")
+    return n, h, stride
+
+
+def _int32(t: torch.Tensor | None, name: str, n: int, device: torch.device) -> int | None:
+    """Pointer of a contiguous int32 vector of at least n entries (None stays None)."""
+    if t is None:
+        return None
+    if t.dtype != torch.int32 or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor on {device}")
+    if t.numel() < n:
+        raise ValueError(f"{name} needs {n} entries, has {t.numel()}")
+    return t.data_ptr()
+
+
+def _same(device: torch.device, dtype: torch.dtype | None, **ts) -> None:
+    for name, t in ts.items():
+        if t is None:
+            continue
+        if t.device != device:
+            raise ValueError(f"{name} is on {t.device}, expected {device}")
+        if dtype is not None and t.dtype != dtype:
+            raise TypeError(f"{name} is {t.dtype}, expected {dtype}")
+
+
+def _head_weight(w: torch.Tensor | None, name: str, device, dtype) -> int | None:
+    if w is None:
+        return None
+    _same(device, dtype, **{name: w})
+    if w.shape != (2, _HD) or not w.is_contiguous():
+        raise ValueError(f"{name} must be contiguous [2, 128] (one row per model)")
+    return w.data_ptr()
+
+
+def _rope_args(cos, sin, device) -> tuple:
+    """(cos, sin pointers, positions, rotary_dim) of the rotation tables."""
+    if (cos is None) != (sin is None):
+        raise ValueError("rope_cos and rope_sin come together")
+    if cos is None:
+        return None, None, 0, 0
+    _same(device, torch.float32, rope_cos=cos, rope_sin=sin)
+    if cos.dim() != 2 or cos.shape != sin.shape or not (cos.is_contiguous() and sin.is_contiguous()):
+        raise ValueError("rope tables must be contiguous [positions, rotary_dim / 2]")
+    rotary = 2 * cos.shape[1]
+    if rotary % 16 or not 0 < rotary <= _HD or cos.shape[0] == 0:
+        raise ValueError("rotary_dim must be a multiple of 16 up to 128, with at least one position")
+    return cos.data_ptr(), sin.data_ptr(), cos.shape[0], rotary
+
+
+def _split(split_point: int | None, M: int) -> int:
+    if split_point is None:
+        return M
+    if not 0 <= split_point <= M:
+        raise ValueError(f"split_point must be in [0, {M}]")
+    return split_point
+
+
+class _device_of:
+    """Makes the tensors' device current for the launch when it is not."""
+    __slots__ = ("idx", "prev")
+
+    def __init__(self, device: torch.device):
+        self.idx = device.index
+
+    def __enter__(self):
+        self.prev = torch.cuda.current_device()
+        if self.prev != self.idx:
+            torch.cuda.set_device(self.idx)
+
+    def __exit__(self, *exc):
+        if self.prev != self.idx:
+            torch.cuda.set_device(self.prev)
+
+
+def _kv4_cache(pools, block_table: torch.Tensor | None, device, dtype) -> _lib.KV4CacheDesc:
+    """Validate both models' 4-bit pools (``KV4Pool`` or None) and the block table."""
+    c = _lib.KV4CacheDesc()
+    if len(pools) != 2:
+        raise ValueError("pools are (model 0's, model 1's), either may be None")
+    n_kv = length = 0
+    for m, p in enumerate(pools):
+        if p is None or p[0].shape[0] == 0:
+            continue
+        kc, km, vc, vm = p
+        sh = kc.shape
+        if len(sh) != 4 or sh[3] != 64 or vc.shape != sh or km.shape != (*sh[:3], 4, 2) or \
+                vm.shape != km.shape:
+            raise ValueError("a 4-bit pool is codes [rows, n_kv_heads, length, 64] and meta "
+                             "[rows, n_kv_heads, length, 4, 2], for K and for V")
+        if kc.dtype != torch.uint8 or vc.dtype != torch.uint8 or km.dtype != dtype or \
+                vm.dtype != dtype:
+            raise TypeError(f"a 4-bit pool holds uint8 codes and {dtype} meta here")
+        for t in p:
+            if t.device != device or not t.is_contiguous():
+                raise ValueError(f"4-bit pools must be contiguous tensors on {device}")
+        if n_kv and (n_kv, length) != (sh[1], sh[2]):
+            raise ValueError("both models' pools must have the same heads and length")
+        n_kv, length = sh[1], sh[2]
+        d = c.pool[m]
+        d.k_codes, d.k_meta, d.v_codes, d.v_meta = (kc.data_ptr(), km.data_ptr(), vc.data_ptr(),
+                                                    vm.data_ptr())
+        d.rows = sh[0]
+    if not n_kv or not length:
+        raise ValueError("at least one model needs a 4-bit pool")
+    c.n_kv_heads = n_kv
+    if block_table is None:
+        c.L_cap = length
+    else:
+        if block_table.dim() != 2:
+            raise ValueError("block_table must be int32 [rows, max_pages]")
+        c.block_table = _int32(block_table, "block_table", 1, device)
+        c.table_rows, c.max_pages = block_table.shape
+        c.page_size = length
+        if length < 8 or length > 4096 or length & (length - 1):
+            raise ValueError("page_size must be a power of two in [8, 4096]")
+    return c
+
+
+def _home_arg(rows, block_table, M: int, device) -> int | None:
+    """Pointer of the tokens' cache rows; without them a table needs a row per token."""
+    if rows is None and block_table is not None and block_table.shape[0] < M:
+        raise ValueError("block_table needs a row per token when rows is not given")
+    return _int32(rows, "rows", M, device)
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, pos: torch.Tensor, *,
+                 q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None,
+                 eps: float = 1e-6, rope_cos: torch.Tensor | None = None,
+                 rope_sin: torch.Tensor | None = None, interleaved: bool = False,
+                 split_point: int | None = None, counts: torch.Tensor | None = None,
+                 q_out: torch.Tensor | None = None,
+                 k_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """RMSNorm of every q and k head and the position rotation, in one pass.
+
+    ``q`` [tokens, n_heads, 128] and ``k`` [tokens, n_kv_heads, 128] may be views
+    of one qkv row. ``q_weight`` / ``k_weight`` [2, 128] (one row per model;
+    None: that norm is left out); ``rope_cos`` / ``rope_sin`` [positions,
+    rotary_dim / 2] fp32 (``rope_tables``; None: no rotation) turn the first
+    rotary_dim channels, as pairs (i, i + rotary_dim / 2), or (2i, 2i + 1) when
+    ``interleaved``. Tokens are in routed order: the first ``split_point`` (or
+    counts[0], read on the device; default: all) belong to model 0.
+    ``q_out`` / ``k_out`` may be the inputs themselves.
+    """
+    M, nh, qs = _heads(q, "q")
+    Mk, nkv, ks = _heads(k, "k")
+    dev, dt = q.device, q.dtype
+    code = _lib.dtype_code(dt)
+    if Mk != M:
+        raise ValueError("q and k must have the same tokens")
+    _same(dev, dt, k=k, q_out=q_out, k_out=k_out)
+    _same(dev, None, counts=counts)
+    q_out = torch.empty(q.shape, dtype=dt, device=dev) if q_out is None else q_out
+    k_out = torch.empty(k.shape, dtype=dt, device=dev) if k_out is None else k_out
+    Mq, nho, qos = _heads(q_out, "q_out")
+    Mo, nko, kos = _heads(k_out, "k_out")
+    if (Mq, nho, Mo, nko) != (M, nh, M, nkv):
+        raise ValueError("q_out / k_out must have the shapes of q / k")
+    rc, rs, rope_len, rotary = _rope_args(rope_cos, rope_sin, dev)
+    with _device_of(dev):
+        check(lib.ps_qk_norm_rope(q.data_ptr(), qs, k.data_ptr(), ks, q_out.data_ptr(), qos,
+                                  k_out.data_ptr(), kos, _head_weight(q_weight, "q_weight", dev, dt),
+                                  _head_weight(k_weight, "k_weight", dev, dt), float(eps), rc, rs,
+                                  rope_len, rotary, 1 if interleaved else 0,
+                                  _int32(pos, "pos", M, dev), _counts_arg(counts),
+                                  _split(split_point, M), M, nh, nkv, code,
+                                  ptr(_lib.status_tensor(dev)), _lib.stream_handle(dev)),
+              "ps_qk_norm_rope")
+    return q_out, k_out
+
+
+def kv4_append(k: torch.Tensor, v: torch.Tensor, pools: tuple, pos: torch.Tensor, *,
+               q: torch.Tensor | None = None, q_weight: torch.Tensor | None = None,
+               k_weight: torch.Tensor | None = None, eps: float = 1e-6,
+               rope_cos: torch.Tensor | None = None, rope_sin: torch.Tensor | None = None,
+               interleaved: bool = False, rows: torch.Tensor | None = None,
+               block_table: torch.Tensor | None = None, split_point: int | None = None,
+               counts: torch.Tensor | None = None,
+               q_out: torch.Tensor | None = None) -> torch.Tensor | None:
+    """Quantise the tokens' k and v into the 4-bit cache at positions ``pos``.
+
+    ``pools`` = (model 0's ``KV4Pool``, model 1's), either None. Token j goes to
+    its model's slot ``rows[j]`` (default: its rank within its model), or with
+    ``block_table`` [rows, max_pages] to the pages of table row ``rows[j]``
+    (default: j). Norms and rotation as in ``qk_norm_rope`` (all optional) happen
+    in the same pass: k is quantised from their fp32 result, ``q`` (optional)
+    returns in 16 bits. Two tokens of a call must not share a position of a
+    sequence. Returns q_out, or None without ``q``.
+    """
+    M, nkv, ks = _heads(k, "k")
+    Mv, nv, vs = _heads(v, "v")
+    dev, dt = k.device, k.dtype
+    code = _lib.dtype_code(dt)
+    if (Mv, nv) != (M, nkv):
+        raise ValueError("k and v must have the same shape")
+    _same(dev, dt, v=v, q=q, q_out=q_out)
+    _same(dev, None, counts=counts)
+    cache = _kv4_cache(pools, block_table, dev, dt)
+    if cache.n_kv_heads != nkv:
+        raise ValueError(f"k has {nkv} heads, the pools {cache.n_kv_heads}")
+    nh = qs = qos = 0
+    if q is not None:
+        Mq, nh, qs = _heads(q, "q")
+        q_out = torch.empty(q.shape, dtype=dt, device=dev) if q_out is None else q_out
+        Mo, nho, qos = _heads(q_out, "q_out")
+        if Mq != M or (Mo, nho) != (M, nh):
+            raise ValueError("q and q_out must have one row per token of k")
+    elif q_out is not None:
+        raise ValueError("q_out needs q")
+    rc, rs, rope_len, rotary = _rope_args(rope_cos, rope_sin, dev)
+    with _device_of(dev):
+        check(lib.ps_kv4_append(ptr(q), qs, k.data_ptr(), ks, v.data_ptr(), vs, ptr(q_out), qos,
+                                ctypes.byref(cache), _head_weight(q_weight, "q_weight", dev, dt),
+                                _head_weight(k_weight, "k_weight", dev, dt), float(eps), rc, rs,
+                                rope_len, rotary, 1 if interleaved else 0,
+                                _int32(pos, "pos", M, dev), _home_arg(rows, block_table, M, dev),
+                                _counts_arg(counts), _split(split_point, M), M, nh, code,
+                                ptr(_lib.status_tensor(dev)), _lib.stream_handle(dev)),
+              "ps_kv4_append")
+    return q_out
+
+
+def kv4_gather(pools: tuple, seqs: torch.Tensor, cu: torch.Tensor, total: int, *,
+               block_table: torch.Tensor | None = None,
+               out: tuple[torch.Tensor, torch.Tensor] | None = None
+               ) -> tuple[torch.Tensor, torch.Tensor]:
+    """Read cached rows back in 16 bits, packed: (k, v) [total, n_kv_heads, 128].
+
+    Sequence i (``seqs`` int32 [n, 3]: model, slot or block-table row, first
+    position) fills rows ``cu[i]`` to ``cu[i + 1]`` (``cu`` int32 [n + 1] on the
+    device). Rows behind the last sequence are left as ``out`` had them.
+    """
+    live = [p for p in pools if p is not None and p[0].shape[0]]
+    if not live:
+        raise ValueError("at least one model needs a 4-bit pool")
+    dev, dt = live[0][0].device, live[0][1].dtype
+    if dev.type != "cuda":
+        raise ValueError("parallel-serve ops take CUDA tensors")
+    code = _lib.dtype_code(dt)
+    cache = _kv4_cache(pools, block_table, dev, dt)
+    if seqs.dim() != 2 or seqs.shape[1] != 3:
+        raise ValueError("seqs must be int32 [n, 3] (model, slot or block-table row, first position)")
+    n = seqs.shape[0]
+    if total < 0:
+        raise ValueError("total must be >= 0")
+    if out is None:
+        out = tuple(torch.empty(total, cache.n_kv_heads, _HD, dtype=dt, device=dev)
+                    for _ in range(2))
+    for t in out:
+        _same(dev, dt, out=t)
+        if t.shape != (total, cache.n_kv_heads, _HD) or not t.is_contiguous():
+            raise ValueError("out must be two contiguous [total, n_kv_heads, 128] tensors")
+    with _device_of(dev):
+        check(lib.ps_kv4_gather(ctypes.byref(cache), _int32(seqs, "seqs", 3 * n, dev),
+                                _int32(cu, "cu", n + 1, dev), n, total, out[0].data_ptr(),
+                                out[1].data_ptr(), code, ptr(_lib.status_tensor(dev)),
+                                _lib.stream_handle(dev)), "ps_kv4_gather")
+    return out[0], out[1]
+
+
+def _counter_workspace(device: torch.device, nbytes: int, tag: str, counter_bytes: int) -> torch.Tensor:
+    """Workspace whose first ``counter_bytes`` are zero at rest. Under graph capture
+    a workspace of the graph's own (two captured graphs may run at the same
+    time), else the stream's."""
+    if torch.cuda.is_current_stream_capturing():
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        ws[:counter_bytes].zero_()
+        return ws
+    return _lib.workspace(device, nbytes, tag)
+
+
+def kv4_decode_attention(q: torch.Tensor, pools: tuple, pos: torch.Tensor, *, max_len: int,
+                         rows: torch.Tensor | None = None,
+                         block_table: torch.Tensor | None = None,
+                         split_point: int | None = None, counts: torch.Tensor | None = None,
+                         out: torch.Tensor | None = None, scale: float | None = None,
+                         workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Decode attention over the 4-bit cache: token j sees positions 0..pos[j] of
+    its sequence; query head h reads KV head h // (n_heads / n_kv_heads).
+
+    ``q`` [M, n_heads, 128] (or [M, n_heads * 128]); ``rows``, ``block_table``,
+    ``split_point`` and ``counts`` as in ``kv4_append``; ``max_len`` bounds
+    pos[j] + 1. Returns [M, n_heads * 128].
+    """
+    M, nh, qs = _heads(q, "q")
+    dev, dt = q.device, q.dtype
+    code = _lib.dtype_code(dt)
+    _same(dev, None, counts=counts, workspace=workspace)
+    _same(dev, dt, out=out)
+    cache = _kv4_cache(pools, block_table, dev, dt)
+    nkv = cache.n_kv_heads
+    if nh % nkv:
+        raise ValueError(f"{nh} query heads do not divide over {nkv} KV heads")
+    cap = cache.L_cap if block_table is None else cache.max_pages * cache.page_size
+    if not 0 < max_len <= cap:
+        raise ValueError(f"max_len must be in [1, {cap}]")
+    if out is None:
+        out = torch.empty(M, nh * _HD, dtype=dt, device=dev)
+    elif out.shape != (M, nh * _HD) or not out.is_contiguous():
+        raise ValueError("out must be contiguous [M, n_heads * 128]")
+    scale = 1.0 / math.sqrt(_HD) if scale is None else scale
+    with _device_of(dev):
+        if workspace is None:
+            nbytes = lib.ps_kv4_decode_attention_workspace_bytes(M, nh, nkv, max_len)
+            workspace = _counter_workspace(dev, nbytes, "kv4_attn", 4096)
+        check(lib.ps_kv4_decode_attention(q.data_ptr(), qs, ctypes.byref(cache), out.data_ptr(),
+                                          _int32(pos, "pos", M, dev),
+                                          _home_arg(rows, block_table, M, dev),
+                                          _counts_arg(counts), _split(split_point, M), M, nh,
+                                          max_len, float(scale), code, workspace.data_ptr(),
+                                          workspace.numel() * workspace.element_size(),
+                                          ptr(_lib.status_tensor(dev)), _lib.stream_handle(dev)),
+              "ps_kv4_decode_attention")
+    return out
