@@ -15,10 +15,15 @@
 // by q (low-nibble channels times 16) and, for V, by the output channel. Scale
 // and zero stay outside the products, in fp32:
 //   S = sum_g s_g * (sum_{ch in g} q c) + z_g * (sum_{ch in g} q)
-//   O = sum_pos (P s_g) c  (P s_g / ref rounded to fp16: one rounding, 2^-12)
-//       + sum_pos P z_g    (fp32)
+//   O = sum_pos (P s_g) (c - 8)  (P s_g / ref rounded to fp16)
+//       + sum_pos P (z_g + 8 s_g)  (fp32)
 // with ref a running power of two >= every s seen, rescaled like the softmax's
-// running maximum, so bf16 scales of any exponent fit. q is scaled per head by a
+// running maximum, so bf16 scales of any exponent fit. The - 8 (one more
+// instruction per product, with a constant operand) keeps the summands of O as
+// small as the values themselves: around c alone, the rounding of P s_g weighs
+// about twice as much and a long sum loses the digits that z then cancels.
+// The z term of S is a product too: the sums of q, cut into 16-bit parts that
+// together carry fp32's digits, against the stored zeros. q is scaled per head by a
 // power of two into fp16's range (exact down to 2^-24 of the head's largest).
 //
 // S comes out of the instruction with positions in lanes and heads in registers,
@@ -32,6 +37,8 @@
 // last CTA to finish a piece of an item merges the pieces in order, so results
 // do not depend on timing.
 #include <cuda_runtime.h>
+
+#include <type_traits>
 
 #include "kv4.cuh"
 #include "ps_host.h"
@@ -52,7 +59,7 @@ constexpr int kStageBytes = 2 * (kTileCodes + kTileMeta);  // K codes, K meta, V
 constexpr int kMaxEntries = 1024;            // prefix-sum entries of the token lengths
 constexpr int kMergeBytes = kWarps * kHB * (kD + 2) * 4;
 constexpr size_t kCounterBytes = 4096;       // arrival counters, zero at rest: one per CTA
-constexpr int kAttnSmem = kStages * kStageBytes + kMergeBytes + 256 + (kMaxEntries + 1) * 4 + 128;
+constexpr int kAttnSmem = kStages * kStageBytes + kMergeBytes + 256 + (kMaxEntries + 1) * 4;
 
 struct AttnArgs {
   const void* q;  // [M, n_heads, 128], token stride q_stride
@@ -73,19 +80,65 @@ struct AttnArgs {
   float scale_log2;
 };
 
+// d += a b on one 16 x 8 x 16 tile; kBf16: bf16 operands, else fp16.
+template <bool kBf16 = false>
 PS_DEV void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                      uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-      "{%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  if (kBf16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// d = a b (the zero addend costs no register).
+template <bool kBf16 = false>
+PS_DEV void mma16816_zero(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                          uint32_t b0, uint32_t b1) {
+  if (kBf16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+
+// 2^x; results below 2^-126 are 0.
+PS_DEV float exp2_ftz(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 PS_DEV uint32_t transpose8x8(uint32_t v) {
   uint32_t r;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
+}
+
+// Maxima of two pairs of 16-bit values.
+template <typename T>
+PS_DEV uint32_t max16x2(uint32_t a, uint32_t b) {
+  if (std::is_same<T, __half>::value) {
+    const __half2 m = __hmax2(*reinterpret_cast<const __half2*>(&a),
+                              *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&m);
+  }
+  const __nv_bfloat162 m = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&a),
+                                   *reinterpret_cast<const __nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&m);
 }
 
 PS_DEV uint32_t half2_bits(float lo, float hi) {
@@ -150,9 +203,9 @@ PS_DEV Piece piece_at(const AttnArgs& a, const int32_t* P, int entries, int c0, 
 template <typename T>
 __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm)
     kv4_decode_attention_kernel(const AttnArgs a) {
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem =
-      reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127));
+  // no pointer arithmetic through integers here: the compiler then knows that
+  // every access below is to shared memory (generic loads cost 20% of the time)
+  extern __shared__ __align__(128) uint8_t smem[];
   float* so = reinterpret_cast<float*>(smem + kStages * kStageBytes);  // [warp][head][128]
   float* sml = so + kWarps * kHB * kD;                                 // [warp][head][2]
   uint64_t* full = reinterpret_cast<uint64_t*>(sml + kWarps * kHB * 2);
@@ -311,6 +364,9 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm)
   const int sig = gr ^ ((gr >> 1) & 1);
   const int sig0 = (2 * t4) ^ (t4 & 1), sig1 = (2 * t4 + 1) ^ (t4 & 1);
   const uint32_t vsel = (gr & 1) ? 0x7632u : 0x5410u;
+  constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  // -8 on the scale of a low and of a high nibble, twice
+  constexpr uint32_t kMinus8Low = 0x80088008u, kMinus8High = 0x80808080u;
   int gs = 0;
   bool dead = false;
   for (long long g = g0; g < g1;) {
@@ -321,8 +377,8 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm)
 
     // q as B fragments: lane (gr, t4) holds head gr, channels 32 g + 8 t4 + i.
     uint32_t qb[4][4];     // [group][(i=0,4) (1,5) (2,6) (3,7)]
-    float qs[4][2];        // sum of q over the group, for heads 2 t4, 2 t4 + 1
-    float qf[2];           // what S is multiplied by for those heads
+    uint32_t zb[2];        // the groups' sums of q, cut into parts (see below)
+    float qf[2];           // the scale of head 2 t4, 2 t4 + 1: softmax scale x its power of two
     {
       uint4 raw[4];
       const bool live = gr < nh;
@@ -365,15 +421,25 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm)
           qb[gi][i] = half2_bits(f[i] * k, f[i + 4] * k);
         }
       }
-      const float up = __uint_as_float((uint32_t)(127 + e) << 23) * 1048576.f * a.scale_log2;
+      // B operand of the z term: rows k = 4 part + group hold the parts of the
+      // group sums, each part what the ones before leave of it in 16 bits
+      // (fp16: 11 bits each, bf16: 8; three parts make fp32's 24)
+      float r0 = (t4 & 1 ? sum[2] : sum[0]) * down, r1 = (t4 & 1 ? sum[3] : sum[1]) * down;
+      uint32_t part[4];
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int src = (2 * t4 + x) * 4;  // a lane of head 2 t4 + x
-        qf[x] = __shfl_sync(0xffffffffu, up, src);
-#pragma unroll
-        for (int gi = 0; gi < 4; ++gi)
-          qs[gi][x] = __shfl_sync(0xffffffffu, sum[gi], src) * a.scale_log2;
+      for (int i = 0; i < 4; ++i) {
+        part[i] = pack2<T>(r0, r1);
+        float x, y;
+        unpack2<T>(part[i], x, y);
+        r0 -= x;
+        r1 -= y;
       }
+      zb[0] = t4 & 2 ? part[1] : part[0];
+      zb[1] = t4 & 2 ? part[3] : part[2];
+      const float up = __uint_as_float((uint32_t)(127 + e) << 23) * a.scale_log2;
+#pragma unroll
+      for (int x = 0; x < 2; ++x)  // from a lane of head 2 t4 + x
+        qf[x] = __shfl_sync(0xffffffffu, up, (2 * t4 + x) * 4);
     }
 
     float o[8][4];   // [2 g + half][channel pair x head]: see the store below
@@ -399,10 +465,20 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm)
       bad |= stage_bad[st] != 0;
       const int left = pc.len - t * kTile - warp * kWarpPos;  // live positions of this warp
       if (left > 0) {
-        const uint8_t* kc = smem + st * kStageBytes + warp * kWarpPos * kCodeBytes;
-        const uint8_t* km = smem + st * kStageBytes + kTileCodes + warp * kWarpPos * kMetaBytes;
-        const uint8_t* vc = kc + kTileCodes + kTileMeta;
-        const uint8_t* vm = km + kTileCodes + kTileMeta;
+        uint8_t* kc = smem + st * kStageBytes + warp * kWarpPos * kCodeBytes;
+        uint8_t* km = smem + st * kStageBytes + kTileCodes + warp * kWarpPos * kMetaBytes;
+        uint8_t* vc = kc + kTileCodes + kTileMeta;
+        uint8_t* vm = km + kTileCodes + kTileMeta;
+        if (left < kWarpPos) {
+          // rows behind the last position may hold anything: their scales and
+          // zeros become 0 here, their scores -inf below
+          if (lane >= left) {
+            *reinterpret_cast<uint4*>(km + lane * kMetaBytes) = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(vm + lane * kMetaBytes) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();  // before the stage's next bulk copies
+          __syncwarp();
+        }
         float s[2][4];
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt) {
@@ -413,82 +489,91 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm)
           const uint4 e1 = *reinterpret_cast<const uint4*>(km + r1 * kMetaBytes);
           const uint32_t a0[4] = {w0.x, w0.y, w0.z, w0.w}, a1[4] = {w1.x, w1.y, w1.z, w1.w};
           const uint32_t p0[4] = {e0.x, e0.y, e0.z, e0.w}, p1[4] = {e1.x, e1.y, e1.z, e1.w};
-          float qk[4] = {0.f, 0.f, 0.f, 0.f}, qz[4] = {0.f, 0.f, 0.f, 0.f};
+          // z term: A row = the position's zeros, pair (0, 1) or (2, 3) in lane t4
+          const uint32_t z0 = __byte_perm(t4 & 1 ? e0.z : e0.x, t4 & 1 ? e0.w : e0.y, 0x7632);
+          const uint32_t z1 = __byte_perm(t4 & 1 ? e1.z : e1.x, t4 & 1 ? e1.w : e1.y, 0x7632);
+          float zt[4], qk[4] = {0.f, 0.f, 0.f, 0.f};
+          mma16816_zero<kBf16>(zt, z0, z1, z0, z1, zb[0], zb[1]);
 #pragma unroll
           for (int gi = 0; gi < 4; ++gi) {
-            float c[4] = {0.f, 0.f, 0.f, 0.f};
+            float c[4];
             const uint32_t h0 = a0[gi] >> 8, h1 = a1[gi] >> 8;
-            mma16816(c, a0[gi] & 0x000f000fu, a1[gi] & 0x000f000fu, a0[gi] & 0x00f000f0u,
-                     a1[gi] & 0x00f000f0u, qb[gi][0], qb[gi][1]);
+            mma16816_zero(c, a0[gi] & 0x000f000fu, a1[gi] & 0x000f000fu, a0[gi] & 0x00f000f0u,
+                          a1[gi] & 0x00f000f0u, qb[gi][0], qb[gi][1]);
             mma16816(c, h0 & 0x000f000fu, h1 & 0x000f000fu, h0 & 0x00f000f0u, h1 & 0x00f000f0u,
                      qb[gi][2], qb[gi][3]);
-            float s0, z0, s1, z1;
-            unpack2<T>(p0[gi], s0, z0);
-            unpack2<T>(p1[gi], s1, z1);
+            float s0, s1, unused;
+            unpack2<T>(p0[gi], s0, unused);
+            unpack2<T>(p1[gi], s1, unused);
             qk[0] += s0 * c[0], qk[1] += s0 * c[1], qk[2] += s1 * c[2], qk[3] += s1 * c[3];
-            qz[0] += z0 * qs[gi][0], qz[1] += z0 * qs[gi][1];
-            qz[2] += z1 * qs[gi][0], qz[3] += z1 * qs[gi][1];
           }
-          s[mt][0] = r0 < left ? qk[0] * qf[0] + qz[0] : -INFINITY;
-          s[mt][1] = r0 < left ? qk[1] * qf[1] + qz[1] : -INFINITY;
-          s[mt][2] = r1 < left ? qk[2] * qf[0] + qz[2] : -INFINITY;
-          s[mt][3] = r1 < left ? qk[3] * qf[1] + qz[3] : -INFINITY;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) s[mt][k] = (qk[k] * 1048576.f + zt[k]) * qf[k & 1];
+          if (left < kWarpPos) {
+            if (r0 >= left) s[mt][0] = s[mt][1] = -INFINITY;
+            if (r1 >= left) s[mt][2] = s[mt][3] = -INFINITY;
+          }
         }
-        // V's meta of this lane's rows; rows past the end count as s = z = 0
-        float vs[2][2][4], vz[2][2][4];
-        float smax = 0.f;
+        // V's meta of this lane's rows, and their largest scale (low halves)
+        uint32_t ve[2][2][4], top2 = 0;
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            const int r = mt * 16 + k * 8 + sig;
-            const uint4 e = *reinterpret_cast<const uint4*>(vm + r * kMetaBytes);
-            const uint32_t p[4] = {e.x, e.y, e.z, e.w};
+            const uint4 e =
+                *reinterpret_cast<const uint4*>(vm + (mt * 16 + k * 8 + sig) * kMetaBytes);
+            ve[mt][k][0] = e.x, ve[mt][k][1] = e.y, ve[mt][k][2] = e.z, ve[mt][k][3] = e.w;
 #pragma unroll
-            for (int gi = 0; gi < 4; ++gi) {
-              unpack2<T>(r < left ? p[gi] : 0u, vs[mt][k][gi], vz[mt][k][gi]);
-              smax = fmaxf(smax, vs[mt][k][gi]);
-            }
+            for (int gi = 0; gi < 4; ++gi) top2 = max16x2<T>(top2, ve[mt][k][gi]);
           }
+        float smax, unused;
+        unpack2<T>(top2 & 0xffffu, smax, unused);
         float mx[2] = {fmaxf(fmaxf(s[0][0], s[0][2]), fmaxf(s[1][0], s[1][2])),
                        fmaxf(fmaxf(s[0][1], s[0][3]), fmaxf(s[1][1], s[1][3]))};
+        // The references move only when a score is 2^8 above its head's, or a
+        // scale above ref: P (at most 2^8) stays within fp16 and sums keep their
+        // precision, and most tiles need no exchange between lanes at all.
+        if (__any_sync(0xffffffffu, mx[0] > m_run[0] + 8.f || mx[1] > m_run[1] + 8.f ||
+                                        smax > ref)) {
 #pragma unroll
-        for (int x = 0; x < 2; ++x)
+          for (int x = 0; x < 2; ++x)
 #pragma unroll
-          for (int off = 4; off <= 16; off <<= 1)
-            mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], off));
-        // the next power of two above the largest scale of the warp's rows
-        const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(smax)) & 0x7f800000u;
-        const float ref_new = fmaxf(ref, __uint_as_float(min(top + 0x00800000u, 0x7f000000u)));
-        const float m_new[2] = {fmaxf(m_run[0], mx[0]), fmaxf(m_run[1], mx[1])};
-        float al[2];
+            for (int off = 4; off <= 16; off <<= 1)
+              mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], off));
+          // the next power of two above the largest scale of the warp's rows
+          const uint32_t top =
+              __reduce_max_sync(0xffffffffu, __float_as_uint(smax)) & 0x7f800000u;
+          const float ref_new = fmaxf(ref, __uint_as_float(min(top + 0x00800000u, 0x7f000000u)));
+          const float shrink = ref / ref_new;
+          ref = ref_new;
+          float al[2];
 #pragma unroll
-        for (int x = 0; x < 2; ++x)
-          al[x] = m_new[x] == -INFINITY ? 1.f : exp2f(m_run[x] - m_new[x]);
-        const float shrink = ref / ref_new;
-        if (__any_sync(0xffffffffu, al[0] != 1.f || al[1] != 1.f || shrink != 1.f)) {
+          for (int x = 0; x < 2; ++x) {
+            const float mn = fmaxf(m_run[x], mx[x]);
+            al[x] = mn == -INFINITY ? 1.f : exp2_ftz(m_run[x] - mn);
+            m_run[x] = mn;
+            l_run[x] *= al[x];
+          }
           const float f0 = al[0] * shrink, f1 = al[1] * shrink;
 #pragma unroll
           for (int i = 0; i < 8; ++i) o[i][0] *= f0, o[i][1] *= f1, o[i][2] *= f0, o[i][3] *= f1;
 #pragma unroll
           for (int gi = 0; gi < 4; ++gi) zs[gi][0] *= al[0], zs[gi][1] *= al[1];
-          l_run[0] *= al[0];
-          l_run[1] *= al[1];
         }
-        m_run[0] = m_new[0];
-        m_run[1] = m_new[1];
-        ref = ref_new;
-        const float inv = 1.f / ref;  // a power of two: exact
-        const float mu[2] = {m_new[0] == -INFINITY ? 0.f : m_new[0],
-                             m_new[1] == -INFINITY ? 0.f : m_new[1]};
+        const float inv = __uint_as_float(0x7f000000u - __float_as_uint(ref));  // 1 / 2^k
+        const float mu[2] = {m_run[0] == -INFINITY ? 0.f : m_run[0],
+                             m_run[1] == -INFINITY ? 0.f : m_run[1]};
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt) {
-          float p[4];
+          float p[4], pn[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) p[k] = exp2f(s[mt][k] - mu[k & 1]);
+          for (int k = 0; k < 4; ++k) {
+            p[k] = exp2_ftz(s[mt][k] - mu[k & 1]);
+            pn[k] = p[k] * inv;
+          }
           l_run[0] += p[0] + p[2];
           l_run[1] += p[1] + p[3];
-          // V codes of positions (2 t4, 2 t4 + 1) and (2 t4 + 8, 2 t4 + 9) in row order
+          // V codes of rows 2 t4, 2 t4 + 1 and 2 t4 + 8, 2 t4 + 9
           uint32_t v[4][4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
@@ -498,15 +583,21 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm)
           }
 #pragma unroll
           for (int gi = 0; gi < 4; ++gi) {
-            zs[gi][0] += p[0] * vz[mt][0][gi] + p[2] * vz[mt][1][gi];
-            zs[gi][1] += p[1] * vz[mt][0][gi] + p[3] * vz[mt][1][gi];
-            const float w0 = vs[mt][0][gi] * inv, w1 = vs[mt][1][gi] * inv;
-            const uint32_t b0 = transpose8x8(half2_bits(p[0] * w0, p[1] * w0));
-            const uint32_t b1 = transpose8x8(half2_bits(p[2] * w1, p[3] * w1));
+            float s0, z0, s1, z1;
+            unpack2<T>(ve[mt][0][gi], s0, z0);
+            unpack2<T>(ve[mt][1][gi], s1, z1);
+            const uint32_t b0 = transpose8x8(half2_bits(pn[0] * s0, pn[1] * s0));
+            const uint32_t b1 = transpose8x8(half2_bits(pn[2] * s1, pn[3] * s1));
+            z0 += 8.f * s0;
+            z1 += 8.f * s1;
+            zs[gi][0] += p[0] * z0 + p[2] * z1;
+            zs[gi][1] += p[1] * z0 + p[3] * z1;
             // halfword gr of the group: channels 4 gr + 0..3 of both positions
             const uint32_t x = __byte_perm(v[0][gi], v[1][gi], vsel);
             const uint32_t y = __byte_perm(v[2][gi], v[3][gi], vsel);
             const uint32_t xh = x >> 8, yh = y >> 8;
+            mma16816(o[2 * gi], kMinus8Low, kMinus8High, kMinus8Low, kMinus8High, b0, b1);
+            mma16816(o[2 * gi + 1], kMinus8Low, kMinus8High, kMinus8Low, kMinus8High, b0, b1);
             mma16816(o[2 * gi], x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu,
                      y & 0x00f000f0u, b0, b1);
             mma16816(o[2 * gi + 1], xh & 0x000f000fu, xh & 0x00f000f0u, yh & 0x000f000fu,
