@@ -58,8 +58,9 @@ constexpr int kTileMeta = kTile * kMetaBytes;
 constexpr int kStageBytes = 2 * (kTileCodes + kTileMeta);  // K codes, K meta, V codes, V meta
 constexpr int kMaxEntries = 1024;            // prefix-sum entries of the token lengths
 constexpr int kMergeBytes = kWarps * kHB * (kD + 2) * 4;
+constexpr int kQBytes = kWarps * 32 * 64;    // q as matrix operand, per warp
 constexpr size_t kCounterBytes = 4096;       // arrival counters, zero at rest: one per CTA
-constexpr int kAttnSmem = kStages * kStageBytes + kMergeBytes + 256 + (kMaxEntries + 1) * 4;
+constexpr int kAttnSmem = kStages * kStageBytes + kMergeBytes + 256 + kQBytes + (kMaxEntries + 1) * 4;
 
 struct AttnArgs {
   const void* q;  // [M, n_heads, 128], token stride q_stride
@@ -85,13 +86,13 @@ template <bool kBf16 = false>
 PS_DEV void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                      uint32_t b0, uint32_t b1) {
   if (kBf16)
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
         "{%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   else
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
         "{%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -102,13 +103,13 @@ template <bool kBf16 = false>
 PS_DEV void mma16816_zero(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                           uint32_t b0, uint32_t b1) {
   if (kBf16)
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
         "{%8,%9}, {%10,%10,%10,%10};"
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
   else
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
         "{%8,%9}, {%10,%10,%10,%10};"
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
@@ -124,7 +125,7 @@ PS_DEV float exp2_ftz(float x) {
 
 PS_DEV uint32_t transpose8x8(uint32_t v) {
   uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
 
@@ -214,7 +215,9 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm)
   volatile int* last_flag = abort_flag + 1;
   volatile int* stage_bad = last_flag + 1;                         // [kStages]
   int* wsum = const_cast<int*>(stage_bad) + kStages;               // [8]
-  int32_t* P = reinterpret_cast<int32_t*>(smem + kStages * kStageBytes + kMergeBytes + 256);
+  uint4* sq = reinterpret_cast<uint4*>(smem + kStages * kStageBytes + kMergeBytes + 256);
+  int32_t* P =
+      reinterpret_cast<int32_t*>(smem + kStages * kStageBytes + kMergeBytes + 256 + kQBytes);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int b = blockIdx.x;
@@ -375,8 +378,10 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm)
     const int head0 = pc.kvh * a.group + pc.hb * kHB;
     const T* qrow = reinterpret_cast<const T*>(a.q) + (size_t)pc.j * a.q_stride;
 
-    // q as B fragments: lane (gr, t4) holds head gr, channels 32 g + 8 t4 + i.
-    uint32_t qb[4][4];     // [group][(i=0,4) (1,5) (2,6) (3,7)]
+    // q as B fragments: lane (gr, t4) holds head gr, channels 32 g + 8 t4 + i,
+    // kept in shared memory [group][lane] as (i=0,4) (1,5) (2,6) (3,7): 16
+    // registers that the accumulators need more.
+    uint4* qb = sq + warp * 128 + lane;
     uint32_t zb[2];        // the groups' sums of q, cut into parts (see below)
     float qf[2];           // the scale of head 2 t4, 2 t4 + 1: softmax scale x its power of two
     {
@@ -415,11 +420,11 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm)
         float f[8];
 #pragma unroll
         for (int i = 0; i < 4; ++i) unpack2<T>(u[i], f[2 * i], f[2 * i + 1]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float k = (i & 1) ? down : 16.f * down;  // low nibbles: channels i even
-          qb[gi][i] = half2_bits(f[i] * k, f[i + 4] * k);
-        }
+        const float low = 16.f * down;  // low nibbles: even channels
+        qb[gi * 32] = make_uint4(half2_bits(f[0] * low, f[4] * low),
+                                 half2_bits(f[1] * down, f[5] * down),
+                                 half2_bits(f[2] * low, f[6] * low),
+                                 half2_bits(f[3] * down, f[7] * down));
       }
       // B operand of the z term: rows k = 4 part + group hold the parts of the
       // group sums, each part what the ones before leave of it in 16 bits
@@ -492,20 +497,24 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm)
           // z term: A row = the position's zeros, pair (0, 1) or (2, 3) in lane t4
           const uint32_t z0 = __byte_perm(t4 & 1 ? e0.z : e0.x, t4 & 1 ? e0.w : e0.y, 0x7632);
           const uint32_t z1 = __byte_perm(t4 & 1 ? e1.z : e1.x, t4 & 1 ? e1.w : e1.y, 0x7632);
-          float zt[4], qk[4] = {0.f, 0.f, 0.f, 0.f};
+          float zt[4], c[4][4], qk[4] = {0.f, 0.f, 0.f, 0.f};
           mma16816_zero<kBf16>(zt, z0, z1, z0, z1, zb[0], zb[1]);
 #pragma unroll
           for (int gi = 0; gi < 4; ++gi) {
-            float c[4];
             const uint32_t h0 = a0[gi] >> 8, h1 = a1[gi] >> 8;
-            mma16816_zero(c, a0[gi] & 0x000f000fu, a1[gi] & 0x000f000fu, a0[gi] & 0x00f000f0u,
-                          a1[gi] & 0x00f000f0u, qb[gi][0], qb[gi][1]);
-            mma16816(c, h0 & 0x000f000fu, h1 & 0x000f000fu, h0 & 0x00f000f0u, h1 & 0x00f000f0u,
-                     qb[gi][2], qb[gi][3]);
+            const uint4 qf4 = qb[gi * 32];
+            mma16816_zero(c[gi], a0[gi] & 0x000f000fu, a1[gi] & 0x000f000fu, a0[gi] & 0x00f000f0u,
+                          a1[gi] & 0x00f000f0u, qf4.x, qf4.y);
+            mma16816(c[gi], h0 & 0x000f000fu, h1 & 0x000f000fu, h0 & 0x00f000f0u,
+                     h1 & 0x00f000f0u, qf4.z, qf4.w);
+          }
+#pragma unroll
+          for (int gi = 0; gi < 4; ++gi) {
             float s0, s1, unused;
             unpack2<T>(p0[gi], s0, unused);
             unpack2<T>(p1[gi], s1, unused);
-            qk[0] += s0 * c[0], qk[1] += s0 * c[1], qk[2] += s1 * c[2], qk[3] += s1 * c[3];
+            qk[0] += s0 * c[gi][0], qk[1] += s0 * c[gi][1];
+            qk[2] += s1 * c[gi][2], qk[3] += s1 * c[gi][3];
           }
 #pragma unroll
           for (int k = 0; k < 4; ++k) s[mt][k] = (qk[k] * 1048576.f + zt[k]) * qf[k & 1];
