@@ -490,6 +490,22 @@ int ps_kv4_decode_attention(const void* q, long long q_stride, const ps_kv4_cach
                             int max_len, float scale, int dtype, void* workspace,
                             size_t workspace_bytes, int32_t* status, ps_stream_t stream);
 
+/* Causal attention over packed prompts, grouped heads, on the tensor cores (an
+ * addition of this library). Sequence i's queries are rows [cu_q[i], cu_q[i+1])
+ * of q [Tq, n_heads, 128], its keys and values rows [cu_k[i], cu_k[i+1]) of k, v
+ * [Tk, n_kv_heads, 128]; the last query sees every key: query r of lq sees keys
+ * 0 .. r + (lk - lq), where keys that precede the queries are a history. out
+ * [Tq, n_heads, 128]; a query that sees no key gets 0, rows outside every
+ * sequence stay as they were. Token strides in elements (multiples of 8, heads
+ * contiguous); scale > 0. cu_q and cu_k are device arrays, nondecreasing; a
+ * sequence whose range leaves [0, Tq] or [0, Tk] sets PS_ERR_BAD_INDEX and is
+ * skipped. */
+int ps_prompt_attention(const void* q, long long q_stride, const void* k, long long k_stride,
+                        const void* v, long long v_stride, void* out, long long o_stride,
+                        const int32_t* cu_q, const int32_t* cu_k, int n_seqs, int Tq, int Tk,
+                        int n_heads, int n_kv_heads, float scale, int dtype, int32_t* status,
+                        ps_stream_t stream);
+
 /* Segment self-attention with the reference's no-KV semantics
  * (kernel/src/two_model_block_routed.py:100-120, experiments/two_model_block.py:61-65):
  * every token of model m attends (non-causally) to all tokens of model m's

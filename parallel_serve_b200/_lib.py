@@ -114,6 +114,8 @@ SIGNATURES: dict[str, tuple] = {
     "ps_kv4_decode_attention_workspace_bytes": (_sz, [_i, _i, _i, _i]),
     "ps_kv4_decode_attention": (_i, [_p, _ll, ctypes.POINTER(KV4CacheDesc), _p, _p, _p, _p, _i,
                                      _i, _i, _i, _f, _i, _p, _sz, _p, _p]),
+    "ps_prompt_attention": (_i, [_p, _ll, _p, _ll, _p, _ll, _p, _ll, _p, _p, _i, _i, _i, _i, _i,
+                                 _f, _i, _p, _p]),
     "ps_deltazip_packed_bytes": (_sz, [_i, _i]),
     "ps_deltazip_workspace_bytes": (_sz, [_i, _i, _i]),
     "ps_deltazip_linear": (_i, [_p, _p, _p, _p, _i, _i, _i, _i, _p, _i, _p, _sz, _p, _p]),

@@ -1,0 +1,561 @@
+// Causal attention over packed prompts on the 5th-generation tensor cores
+// (sm_100a): grouped heads, sequences of different lengths one after another,
+// keys that may begin before the queries (a prompt chunk behind its history).
+//
+//   out[i, h] = softmax_k(q[i, h] . k[k, h / G] * scale) v[k, h / G]
+//   over the keys k <= i + (keys - queries) of i's sequence
+//
+// Two matrix products of 4 * 128 flops per visible pair bound it, so the tensor
+// core must never wait. One CTA per SM works on 256 queries of one (sequence,
+// head) as two tiles of 128 that take turns: while one tile's scores are in
+// softmax, the other's products run.
+//   warps 0-3, 4-7  softmax of tile 0 / 1, one thread per query row: the row of
+//                   S (128 scores) goes TMEM -> registers in one read, its
+//                   maximum and exponentials stay there, P goes back to TMEM in
+//                   16 bits over S's own columns. P never touches shared memory.
+//   warp 8          TMA: Q, then K and V blocks of 128 keys through a 5-slot ring
+//   warp 9          MMA issue, in the order
+//                   PV0(j) S0(j+1) PV1(j) S1(j+1): products of one thread run in
+//                   order, so S(j+1) may overwrite P(j), and a completed S(j+1)
+//                   says that O is at rest. No further barriers are needed.
+// TMEM (512 columns): S0 S1 (128 fp32 columns each), O0 O1.
+//
+// The running maximum moves only when a score exceeds it by 2^8 (P and the row
+// sum share it, so the result is exact either way): rescaling O, a read and
+// write of 128 columns, is rare after the first blocks. Sums and maxima are fp32;
+// P is rounded to the 16-bit type of V, its only rounding.
+//
+// A masked key's P is 0, but 0 * NaN is not: in the blocks that need a mask (the
+// diagonal and a sequence's end) the V rows behind the end are cleared in shared
+// memory, and a row that holds a NaN or an infinity is cleared too, its key
+// remembered: the queries that see it get NaN, the others what they should.
+#include <cuda_runtime.h>
+
+#include <type_traits>
+
+#include "ps_common.cuh"
+#include "ps_host.h"
+
+namespace ps {
+namespace pra {
+
+constexpr int kD = 128;
+constexpr int kTile = 128;              // queries of a tile, keys of a block
+constexpr int kTiles = 2;               // tiles of a CTA
+constexpr int kRows = kTile * kTiles;   // queries of a CTA
+constexpr int kTileBytes = kTile * kD * 2;
+constexpr int kHalf = kTileBytes / 2;   // one 64-column TMA box (128 rows x 128 bytes)
+constexpr int kSlots = 5;
+constexpr int kThreads = 384;          // warps 10 and 11 only fill their warpgroup
+constexpr int kSmem = 1024 + kTileBytes * (kTiles + kSlots) + 256;
+constexpr int kTmemCols = 512;
+constexpr int kTmemO = 256;             // S tiles at 0, 128; O tiles at 256, 384
+constexpr float kLazyLog2 = 8.f;
+
+struct Args {
+  void* out;
+  long long o_stride;
+  const int32_t* cu_q;  // [n + 1]
+  const int32_t* cu_k;
+  int n, Tq, Tk, n_heads, group, bf16;
+  float scale_log2;
+  int32_t* status;
+};
+
+// D[tmem] (+)= A[tmem, 16-bit pairs] * B[smem desc], kind::f16.
+PS_DEV void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                        uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+#define PS_R32(r)                                                                             \
+  "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),         \
+      "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), \
+      "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),           \
+      "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),           \
+      "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+#define PS_RW16(r)                                                                            \
+  "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]),         \
+      "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), \
+      "+r"(r[14]), "+r"(r[15])
+#define PS_IN32(r)                                                                            \
+  "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),     \
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),       \
+      "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]),     \
+      "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),     \
+      "r"(r[29]), "r"(r[30]), "r"(r[31])
+
+// 32 columns of this thread's lane; complete after ld_wait on the same registers.
+PS_DEV void ld32(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,"
+      "%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : PS_R32(r)
+      : "r"(taddr));
+}
+PS_DEV void ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// Ties registers to the wait above: no use of them moves in front of it.
+PS_DEV void after_wait(uint32_t* r) {
+  asm volatile("" : PS_RW16(r)::"memory");
+  asm volatile("" : PS_RW16((r + 16))::"memory");
+}
+PS_DEV void st32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,"
+      "%24,%25,%26,%27,%28,%29,%30,%31};" ::PS_IN32(r),
+      "r"(taddr)
+      : "memory");
+}
+
+PS_DEV float exp2_ftz(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <typename T>
+PS_DEV uint32_t pack16(float lo, float hi);
+template <>
+PS_DEV uint32_t pack16<__half>(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+PS_DEV uint32_t pack16<__nv_bfloat16>(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Whether 8 16-bit values are all finite (an exponent of ones is not).
+template <typename T>
+PS_DEV bool finite8(const uint4& u) {
+  const uint32_t e = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  bool fin = true;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    fin = fin && (w[i] & e) != e && ((w[i] >> 16) & e) != e;
+  return fin;
+}
+
+// Sequence i owns CTA slots [cu_q[i] / 256 + i, cu_q[i + 1] / 256 + i + 1): at
+// least as many as it has tiles, found by a binary search, no scan of lengths.
+struct Item {
+  int q0, k0, lq, lk, row;  // first rows, lengths, first query of this CTA
+  bool live;
+};
+
+PS_DEV Item item_at(const Args& a, int slot) {
+  int lo = 0, hi = a.n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (a.cu_q[mid] / kRows + mid <= slot) lo = mid; else hi = mid - 1;
+  }
+  Item it;
+  it.q0 = a.cu_q[lo];
+  it.k0 = a.cu_k[lo];
+  const int q1 = a.cu_q[lo + 1], k1 = a.cu_k[lo + 1];
+  const bool ok = it.q0 >= 0 && q1 >= it.q0 && q1 <= a.Tq && it.k0 >= 0 && k1 >= it.k0 && k1 <= a.Tk;
+  it.lq = ok ? q1 - it.q0 : 0;
+  it.lk = ok ? k1 - it.k0 : 0;
+  const int tiles = (it.lq + kRows - 1) / kRows;
+  const int t = slot - (it.q0 / kRows + lo);
+  it.live = ok && t >= 0 && t < tiles;
+  it.row = (tiles - 1 - t) * kRows;  // most work first
+  if (!ok && threadIdx.x == 0) set_status(a.status, PS_ERR_BAD_INDEX);
+  return it;
+}
+
+// Key blocks that tile t (rows row .. of lq) sees.
+PS_DEV int blocks_of(const Item& it, int t) {
+  const int first = it.row + t * kTile;
+  if (first >= it.lq) return 0;
+  const int last = min(it.lq, first + kTile) - 1;
+  const int keys = last + 1 + it.lk - it.lq;  // visible to the last row
+  return keys > 0 ? (keys + kTile - 1) / kTile : 0;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 1)
+    prompt_attention_kernel(const __grid_constant__ CUtensorMap tq,
+                            const __grid_constant__ CUtensorMap tk,
+                            const __grid_constant__ CUtensorMap tv, const Args a) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const uint32_t pad = (1024 - (smem_u32(smem_raw) & 1023)) & 1023;
+  uint8_t* sQ = smem_raw + pad;             // [2] tiles
+  uint8_t* sKV = sQ + kTiles * kTileBytes;  // ring: K0 V0 K1 V1 ...
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sKV + kSlots * kTileBytes);
+  uint64_t* q_full = bars;             // [2]
+  uint64_t* kv_full = q_full + 2;      // [kSlots]
+  uint64_t* kv_empty = kv_full + kSlots;
+  uint64_t* s_full = kv_empty + kSlots;  // [2]
+  uint64_t* p_full = s_full + 2;         // [2]
+  uint64_t* o_done = p_full + 2;         // [2]
+  uint64_t* drain = o_done + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* poison = reinterpret_cast<int*>(tmem_slot + 2);  // first cleared key that was not finite
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(q_full + i, 1);
+      mbar_init(s_full + i, 1);
+      mbar_init(p_full + i, 4);
+      mbar_init(o_done + i, 1);
+    }
+    for (int i = 0; i < kSlots; ++i) {
+      mbar_init(kv_full + i, 1);
+      mbar_init(kv_empty + i, 1);
+    }
+    mbar_init(drain, 1);
+    abort_flag[0] = 0;
+    poison[0] = 0x7fffffff;
+    fence_mbar_init();
+  }
+  if (warp == 9) {
+    tmem_alloc(tmem_slot, kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+  pdl_launch_dependents();
+
+  const int h = blockIdx.x % a.n_heads;
+  const Item it = item_at(a, blockIdx.x / a.n_heads);
+  const int nb0 = it.live ? blocks_of(it, 0) : 0, nb1 = it.live ? blocks_of(it, 1) : 0;
+  const int nb = max(nb0, nb1);
+
+  // 384 threads x 168 registers at launch = 64512 = 128 x 40 + 256 x 232: a
+  // softmax thread holds its 128 scores in registers.
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    // ------------------------------------------------------------- producer
+    if (warp == 8 && lane == 0 && nb > 0) {
+      const uint64_t pol = l2_policy_evict_last();  // a head's K / V serve all its tiles
+      for (int t = 0; t < kTiles; ++t) {
+        if ((t ? nb1 : nb0) == 0) continue;
+        mbar_arrive_expect_tx(q_full + t, kTileBytes);
+        const int r = it.q0 + it.row + t * kTile;
+        tma_load_2d(sQ + t * kTileBytes, &tq, q_full + t, h * kD, r, pol);
+        tma_load_2d(sQ + t * kTileBytes + kHalf, &tq, q_full + t, h * kD + 64, r, pol);
+      }
+      const int kc = (h / a.group) * kD;
+      int i = 0;
+      for (; i < 2 * nb; ++i) {
+        const int st = i % kSlots;
+        if (abort_flag[0] || !mbar_wait(kv_empty + st, ((i / kSlots) & 1) ^ 1, a.status)) {
+          abort_flag[0] = 1;
+          break;
+        }
+        const CUtensorMap* tm = i & 1 ? &tv : &tk;
+        const int r = it.k0 + (i >> 1) * kTile;
+        uint8_t* dst = sKV + st * kTileBytes;
+        mbar_arrive_expect_tx(kv_full + st, kTileBytes);
+        tma_load_2d(dst, tm, kv_full + st, kc, r, pol);
+        tma_load_2d(dst + kHalf, tm, kv_full + st, kc + 64, r, pol);
+      }
+      if (abort_flag[0]) {  // let every issued copy land before the CTA exits
+        if (nb0) mbar_wait(q_full, 0, a.status);
+        if (nb1) mbar_wait(q_full + 1, 0, a.status);
+        for (int n = max(0, i - kSlots); n < i; ++n)
+          mbar_wait(kv_full + n % kSlots, (n / kSlots) & 1, a.status);
+      }
+    }
+    // ------------------------------------------------------------------ MMA
+    if (warp == 9 && lane == 0 && nb > 0) {
+      const uint32_t idesc_s = idesc_f16(a.bf16, 0, 0, kTile, kTile);  // Q, K both K-major
+      const uint32_t idesc_o = idesc_f16(a.bf16, 0, 1, kTile, kD);     // P K-major, V MN-major
+      const uint32_t q_addr = smem_u32(sQ), kv_addr = smem_u32(sKV);
+      bool ok = true;
+      auto wait = [&](uint64_t* bar, uint32_t parity) {
+        if (ok) ok = !abort_flag[0] && mbar_wait(bar, parity, a.status);
+      };
+      auto scores = [&](int t, int j) {  // S_t = Q_t K_j^T
+        const int i = 2 * j;
+        wait(kv_full + i % kSlots, (i / kSlots) & 1);
+        if (j == 0) wait(q_full + t, 0);
+        if (!ok) return;
+        tc_fence_after();
+        const uint32_t qa = q_addr + t * kTileBytes, ka = kv_addr + (i % kSlots) * kTileBytes;
+#pragma unroll
+        for (int kk = 0; kk < kD / 16; ++kk) {
+          const uint32_t o = (kk >> 2) * kHalf + (kk & 3) * 32;
+          umma_f16(tmem + t * kTile, smem_desc_sw128(qa + o, 16, 1024),
+                   smem_desc_sw128(ka + o, 16, 1024), idesc_s, kk > 0 ? 1u : 0u);
+        }
+        umma_commit(s_full + t);
+      };
+      auto values = [&](int t, int j) {  // O_t += P_t V_j
+        const int i = 2 * j + 1;
+        wait(kv_full + i % kSlots, (i / kSlots) & 1);
+        wait(p_full + t, j & 1);
+        if (!ok) return;
+        tc_fence_after();
+        const uint32_t va = kv_addr + (i % kSlots) * kTileBytes;
+#pragma unroll
+        for (int kk = 0; kk < kTile / 16; ++kk)
+          umma_f16_ts(tmem + kTmemO + t * kD, tmem + t * kTile + kk * 8,
+                      smem_desc_sw128(va + kk * 2048, kHalf, 1024), idesc_o,
+                      (j > 0 || kk > 0) ? 1u : 0u);
+      };
+      // A slot is free when the last tile that reads it has: tile 1 if it sees
+      // the block, else tile 0 (nb0 <= nb1 unless tile 1 has no rows).
+      auto release = [&](int i) {
+        if (ok) umma_commit(kv_empty + i % kSlots);
+      };
+      if (nb0) scores(0, 0);
+      if (nb1) scores(1, 0);
+      release(0);
+      for (int j = 0; ok && j < nb; ++j) {
+        if (j < nb0) {
+          values(0, j);
+          if (j + 1 < nb0) scores(0, j + 1);
+          else if (ok) umma_commit(o_done);
+        }
+        if (j < nb1) {
+          values(1, j);
+          release(2 * j + 1);
+          if (j + 1 < nb1) scores(1, j + 1);
+          else if (ok) umma_commit(o_done + 1);
+        } else {
+          release(2 * j + 1);
+        }
+        if (j + 1 < nb) release(2 * j + 2);
+      }
+      if (!ok) abort_flag[0] = 1;
+      // every MMA of this CTA completes before TMEM is released
+      umma_commit(drain);
+      mbar_wait(drain, 0, a.status);
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+    // -------------------------------------------------------------- softmax
+    const int t = warp >> 2;
+    const int r = (warp & 3) * 32 + lane;  // TMEM lane = row of the tile
+    const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t s_addr = tmem + t * kTile + lane_off;
+    const uint32_t o_addr = tmem + kTmemO + t * kD + lane_off;
+    const int first = it.row + t * kTile;
+    const int row = first + r;
+    const int my_nb = t ? nb1 : nb0;
+    const int seen = row + 1 + it.lk - it.lq;  // keys this row sees: [0, seen)
+    const int all_seen = first + 1 + it.lk - it.lq;  // seen by every row of the tile
+    float m = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int j = 0; j < my_nb; ++j) {
+      const bool got = !abort_flag[0] && mbar_wait(s_full + t, j & 1, a.status);
+      if (!__all_sync(0xffffffffu, got)) {  // the warp leaves together (collective TMEM ops)
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      uint32_t s[128];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) ld32(s_addr + 32 * c, s + 32 * c);
+      ld_wait();
+#pragma unroll
+      for (int c = 0; c < 4; ++c) after_wait(s + 32 * c);
+      const bool masked = j * kTile + kTile > all_seen;  // the diagonal, or the end
+      if (masked) {
+        const int lim = seen - j * kTile;
+#pragma unroll
+        for (int c = 0; c < 128; ++c)
+          if (c >= lim) s[c] = 0xff800000u;  // -inf
+      }
+      float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < 128; c += 8) {
+        mx0 = fmaxf(mx0, fmaxf(__uint_as_float(s[c]), __uint_as_float(s[c + 1])));
+        mx1 = fmaxf(mx1, fmaxf(__uint_as_float(s[c + 2]), __uint_as_float(s[c + 3])));
+        mx2 = fmaxf(mx2, fmaxf(__uint_as_float(s[c + 4]), __uint_as_float(s[c + 5])));
+        mx3 = fmaxf(mx3, fmaxf(__uint_as_float(s[c + 6]), __uint_as_float(s[c + 7])));
+      }
+      const float mx = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * a.scale_log2;
+      const bool moved = mx > m + kLazyLog2;
+      if (__any_sync(0xffffffffu, moved)) {
+        // tcgen05 loads and stores are warp-collective: rows that stay scale by 1
+        const float alpha = moved ? exp2_ftz(m - mx) : 1.f;
+        if (moved) m = mx;
+        l *= alpha;
+        if (j > 0) {
+#pragma unroll 1
+          for (int c = 0; c < kD; c += 32) {
+            uint32_t o[32];
+            ld32(o_addr + c, o);
+            ld_wait();
+            after_wait(o);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+            st32(o_addr + c, o);
+          }
+        }
+      }
+      const float neg = m == -INFINITY ? 0.f : -m;  // a row that saw nothing yet: P = 0
+      float l0 = 0.f, l1 = 0.f;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        uint32_t p[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const int c = half * 64 + 2 * i;
+          const float x = exp2_ftz(fmaf(__uint_as_float(s[c]), a.scale_log2, neg));
+          const float y = exp2_ftz(fmaf(__uint_as_float(s[c + 1]), a.scale_log2, neg));
+          l0 += x;
+          l1 += y;
+          p[i] = pack16<T>(x, y);
+        }
+        st32(s_addr + 32 * half, p);
+      }
+      l += l0 + l1;
+      if (masked) {
+        // V_j landed? (it follows K_j in the ring)
+        const int i = 2 * j + 1;
+        if (mbar_wait(kv_full + i % kSlots, (i / kSlots) & 1, a.status)) {
+          uint8_t* v = sKV + (i % kSlots) * kTileBytes + r * 128;
+          bool clear = r >= it.lk - j * kTile;
+          if (!clear) {
+            bool fin = true;
+#pragma unroll
+            for (int c = 0; c < 16; ++c)  // 16-byte chunks, rotated by row: no bank conflicts
+              fin &= finite8<T>(
+                  *reinterpret_cast<const uint4*>(v + (c >> 3) * kHalf + (((c + r) & 7) << 4)));
+            if (!fin) {
+              clear = true;
+              atomicMin(poison, j * kTile + r);
+            }
+          }
+          if (clear) {
+#pragma unroll
+            for (int c = 0; c < 16; ++c)
+              *reinterpret_cast<uint4*>(v + (c >> 3) * kHalf + (((c + r) & 7) << 4)) =
+                  make_uint4(0u, 0u, 0u, 0u);
+          }
+        }
+        fence_proxy_async_smem();  // the cleared rows -> the tensor core's view
+      }
+      __syncwarp();
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(p_full + t);
+    }
+    const bool live = it.live && row < it.lq;
+    bool fin = ok;
+    if (my_nb > 0) fin = ok && !abort_flag[0] && mbar_wait(o_done + t, 0, a.status);
+    fin = __all_sync(0xffffffffu, fin);
+    if (!fin) abort_flag[0] = 1;
+    if (fin && it.live) {
+      tc_fence_after();
+      float inv = l > 0.f || l != l ? 1.f / l : 0.f;  // a row that sees no key: 0
+      if (seen > *reinterpret_cast<volatile int*>(poison)) inv = __uint_as_float(0x7fc00000u);
+      T* orow = reinterpret_cast<T*>(a.out) + (size_t)(it.q0 + row) * a.o_stride + h * kD;
+#pragma unroll 1
+      for (int c = 0; c < kD; c += 32) {
+        uint32_t o[32];
+        if (my_nb > 0) {
+          ld32(o_addr + c, o);
+          ld_wait();
+          after_wait(o);
+        }
+        if (live) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) {
+            uint4 w = make_uint4(0u, 0u, 0u, 0u);
+            if (my_nb > 0 && inv != 0.f) {
+              float f[8];
+#pragma unroll
+              for (int k = 0; k < 8; ++k) f[k] = __uint_as_float(o[i + k]) * inv;
+              w = make_uint4(pack16<T>(f[0], f[1]), pack16<T>(f[2], f[3]), pack16<T>(f[4], f[5]),
+                             pack16<T>(f[6], f[7]));
+            }
+            *reinterpret_cast<uint4*>(orow + c + i) = w;
+          }
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+}  // namespace pra
+}  // namespace ps
+
+using namespace ps;
+
+extern "C" int ps_prompt_attention(const void* q, long long q_stride, const void* k,
+                                   long long k_stride, const void* v, long long v_stride,
+                                   void* out, long long o_stride, const int32_t* cu_q,
+                                   const int32_t* cu_k, int n_seqs, int Tq, int Tk, int n_heads,
+                                   int n_kv_heads, float scale, int dtype, int32_t* status,
+                                   ps_stream_t stream) {
+  PS_CHECK_ARG(n_seqs >= 0 && Tq >= 0 && Tk >= 0 && n_heads > 0 && n_kv_heads > 0 &&
+               n_heads % n_kv_heads == 0);
+  PS_CHECK_ARG(dtype == PS_DTYPE_F16 || dtype == PS_DTYPE_BF16);
+  PS_CHECK_ARG(scale > 0.f && scale < 3.0e38f);
+  if (n_seqs == 0 || Tq == 0) return PS_OK;
+  PS_CHECK_ARG(q && out && cu_q && cu_k && aligned16(q) && aligned16(out));
+  PS_CHECK_ARG(Tk == 0 || (k && v && aligned16(k) && aligned16(v)));
+  PS_CHECK_ARG(q_stride >= (long long)n_heads * pra::kD && q_stride % 8 == 0 &&
+               o_stride >= (long long)n_heads * pra::kD && o_stride % 8 == 0);
+  PS_CHECK_ARG(Tk == 0 || (k_stride >= (long long)n_kv_heads * pra::kD && k_stride % 8 == 0 &&
+                           v_stride >= (long long)n_kv_heads * pra::kD && v_stride % 8 == 0));
+  const long long grid = ((long long)Tq / pra::kRows + n_seqs) * n_heads;
+  if (grid > 0x7fffffffll || Tk > (1 << 30) || Tq > (1 << 30)) return PS_ERR_UNSUPPORTED;
+  const int device = current_device();
+  if (!is_sm100(device)) return PS_ERR_UNSUPPORTED;
+  const bool bf = dtype == PS_DTYPE_BF16;
+  const uint32_t box[2] = {64, (uint32_t)pra::kTile};
+  CUtensorMap tq, tk, tv;
+  auto make = [&](CUtensorMap* map, const void* p, long long stride, int heads, int rows) {
+    const uint64_t dims[2] = {(uint64_t)heads * pra::kD, (uint64_t)rows};
+    const uint64_t strides[1] = {(uint64_t)stride * 2};
+    return make_tmap_16bit(map, p, 2, dims, strides, box, bf);
+  };
+  if (!make(&tq, q, q_stride, n_heads, Tq)) return PS_ERR_CUDA;
+  if (Tk == 0) {  // no keys at all: no block is ever loaded
+    tk = tv = tq;
+  } else if (!make(&tk, k, k_stride, n_kv_heads, Tk) || !make(&tv, v, v_stride, n_kv_heads, Tk)) {
+    return PS_ERR_CUDA;
+  }
+  pra::Args a{};
+  a.out = out;
+  a.o_stride = o_stride;
+  a.cu_q = cu_q;
+  a.cu_k = cu_k;
+  a.n = n_seqs;
+  a.Tq = Tq;
+  a.Tk = Tk;
+  a.n_heads = n_heads;
+  a.group = n_heads / n_kv_heads;
+  a.bf16 = bf ? 1 : 0;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.status = status;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (bf) {
+    PS_CUDA_RET(allow_dynamic_smem(pra::prompt_attention_kernel<__nv_bfloat16>, pra::kSmem));
+    PS_CUDA_RET(launch(pra::prompt_attention_kernel<__nv_bfloat16>, dim3((unsigned)grid),
+                       dim3(pra::kThreads), pra::kSmem, st, tq, tk, tv, a));
+  } else {
+    PS_CUDA_RET(allow_dynamic_smem(pra::prompt_attention_kernel<__half>, pra::kSmem));
+    PS_CUDA_RET(launch(pra::prompt_attention_kernel<__half>, dim3((unsigned)grid),
+                       dim3(pra::kThreads), pra::kSmem, st, tq, tk, tv, a));
+  }
+  return PS_OK;
+}

@@ -718,3 +718,51 @@ def kv4_decode_attention(q: torch.Tensor, pools: tuple, pos: torch.Tensor, *, ma
                                           ptr(_lib.status_tensor(dev)), _lib.stream_handle(dev)),
               "ps_kv4_decode_attention")
     return out
+
+
+def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor,
+                     cu_k: torch.Tensor | None = None, *, scale: float | None = None,
+                     out: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention over packed prompts of different lengths, grouped heads.
+
+    Sequence i's queries are rows ``cu_q[i]`` to ``cu_q[i + 1]`` of ``q`` [tokens,
+    n_heads, 128], its keys and values rows ``cu_k[i]`` to ``cu_k[i + 1]`` (default:
+    the same rows) of ``k``, ``v`` [keys, n_kv_heads, 128]; the last query sees every
+    key, so keys that precede the queries are their history. A query that sees
+    no key gets 0. q, k, v may be views of one qkv row. ``cu_q``, ``cu_k`` are int32
+    on the device. Returns [tokens, n_heads * 128].
+    """
+    Tq, nh, qs = _heads(q, "q")
+    Tk, nkv, ks = _heads(k, "k")
+    Tv, nv, vs = _heads(v, "v")
+    dev, dt = q.device, q.dtype
+    code = _lib.dtype_code(dt)
+    _same(dev, dt, k=k, v=v, out=out)
+    if (Tv, nv) != (Tk, nkv):
+        raise ValueError("k and v must have the same shape")
+    if nh % nkv:
+        raise ValueError(f"{nh} query heads do not divide over {nkv} KV heads")
+    n = cu_q.numel() - 1
+    if n < 0:
+        raise ValueError("cu_q needs at least one entry")
+    if cu_k is None:
+        if Tk != Tq:
+            raise ValueError("without cu_k, k must have one row per query")
+        cu_k = cu_q
+    elif cu_k.numel() != n + 1:
+        raise ValueError("cu_q and cu_k must have the same length")
+    scale = 1.0 / math.sqrt(_HD) if scale is None else float(scale)
+    if not 0.0 < scale < 3e38:
+        raise ValueError("scale must be positive and finite")
+    if out is None:
+        out = torch.empty(Tq, nh * _HD, dtype=dt, device=dev)
+    To, no, os_ = _heads(out, "out")
+    if (To, no) != (Tq, nh):
+        raise ValueError("out must have a row of n_heads * 128 per query")
+    with _device_of(dev):
+        check(lib.ps_prompt_attention(q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs,
+                                      out.data_ptr(), os_, _int32(cu_q, "cu_q", 1, dev),
+                                      _int32(cu_k, "cu_k", 1, dev), n, Tq, Tk, nh, nkv, scale,
+                                      code, ptr(_lib.status_tensor(dev)), _lib.stream_handle(dev)),
+              "ps_prompt_attention")
+    return out
