@@ -62,14 +62,49 @@ struct Args {
   int32_t* status;
 };
 
-// D[tmem] (+)= A[tmem, 16-bit pairs] * B[smem desc], kind::f16.
-PS_DEV void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
-                        uint32_t accumulate) {
+// The MMA warp runs as one: every lane computes the same operands and waits on
+// the same barriers, and the instructions themselves are predicated to one lane.
+// Inside a single-lane branch each operand would have to be moved to a uniform
+// register first, which made issuing a product take longer than the product
+// (155 instead of 64 cycles).
+PS_DEV uint32_t elect_lane() {
+  uint32_t e;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(e));
+  return e;
+}
+// D[tmem] (+)= A[smem desc] * B[smem desc], kind::f16, by the elected lane.
+PS_DEV void mma_ss(uint32_t elected, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                   uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t"
+      "setp.ne.b32 e, %5, 0;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(elected)
+      : "memory");
+}
+// The same with A[tmem, 16-bit pairs].
+PS_DEV void mma_ts(uint32_t elected, uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
+                   uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t"
+      "setp.ne.b32 e, %5, 0;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(elected)
+      : "memory");
+}
+PS_DEV void mma_commit(uint32_t elected, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t"
+      "setp.ne.b32 e, %1, 0;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(
+          smem_u32(bar)),
+      "r"(elected)
       : "memory");
 }
 
@@ -131,6 +166,89 @@ template <>
 PS_DEV uint32_t pack16<__nv_bfloat16>(float lo, float hi) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Two fp32 lanes of one 64-bit register (one issue slot for both).
+PS_DEV uint64_t pair(float lo, float hi) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+  return d;
+}
+PS_DEV void unpair(uint64_t d, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(d));
+}
+PS_DEV uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+PS_DEV uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
+// The row's largest score of a block (raw, before the scale).
+PS_DEV void block_max(uint32_t s_addr, bool masked, int lim, float& mx) {
+  mx = -INFINITY;
+#pragma unroll 1
+  for (int c = 0; c < kTile; c += 32) {
+    uint32_t s[32];
+    ld32(s_addr + c, s);
+    ld_wait();
+    after_wait(s);
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      mx = fmaxf(mx, masked && c + i >= lim ? -INFINITY : __uint_as_float(s[i]));
+  }
+}
+
+// P = 2^(s * scale + neg) of the row's 128 scores in 16 bits, their sum, and the
+// largest score: one pass over S, in chunks of 32 columns whose next one is on
+// its way while this one is worked on. P stays in registers until the caller
+// knows that neg was good enough; S is then overwritten.
+template <typename T>
+PS_DEV void softmax_block(uint32_t s_addr, bool masked, int lim, float scale, float neg,
+                          uint32_t* p, float& lsum, float& mx) {
+  const uint64_t scale2 = pair(scale, scale), neg2 = pair(neg, neg);
+  uint64_t l0 = pair(0.f, 0.f), l1 = l0;
+  float m0 = -INFINITY, m1 = -INFINITY;
+  uint32_t s[2][32];
+  ld32(s_addr, s[0]);
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    uint32_t* v = s[c & 1];
+    ld_wait();
+    after_wait(v);
+    if (c < 3) ld32(s_addr + 32 * (c + 1), s[(c + 1) & 1]);
+    if (masked) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (32 * c + i >= lim) v[i] = 0xff800000u;  // -inf
+    }
+#pragma unroll
+    for (int i = 0; i < 32; i += 4) {
+      const float a0 = __uint_as_float(v[i]), a1 = __uint_as_float(v[i + 1]);
+      const float b0 = __uint_as_float(v[i + 2]), b1 = __uint_as_float(v[i + 3]);
+      m0 = fmaxf(m0, fmaxf(a0, a1));
+      m1 = fmaxf(m1, fmaxf(b0, b1));
+      float x0, x1, y0, y1;
+      unpair(fma2(pair(a0, a1), scale2, neg2), x0, x1);
+      unpair(fma2(pair(b0, b1), scale2, neg2), y0, y1);
+      x0 = exp2_ftz(x0);
+      x1 = exp2_ftz(x1);
+      y0 = exp2_ftz(y0);
+      y1 = exp2_ftz(y1);
+      l0 = add2(l0, pair(x0, x1));
+      l1 = add2(l1, pair(y0, y1));
+      p[16 * c + i / 2] = pack16<T>(x0, x1);
+      p[16 * c + i / 2 + 1] = pack16<T>(y0, y1);
+    }
+  }
+  float s0, s1;
+  unpair(add2(l0, l1), s0, s1);
+  lsum = s0 + s1;
+  mx = fmaxf(m0, m1);
 }
 
 // Whether 8 16-bit values are all finite (an exponent of ones is not).
@@ -203,7 +321,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* poison = reinterpret_cast<int*>(tmem_slot + 2);  // first cleared key that was not finite
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(q_full + i, 1);
@@ -227,19 +345,20 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   pdl_wait();
   pdl_launch_dependents();
 
   const int h = blockIdx.x % a.n_heads;
   const Item it = item_at(a, blockIdx.x / a.n_heads);
-  const int nb0 = it.live ? blocks_of(it, 0) : 0, nb1 = it.live ? blocks_of(it, 1) : 0;
+  const int nb0 = __shfl_sync(0xffffffffu, it.live ? blocks_of(it, 0) : 0, 0);
+  const int nb1 = __shfl_sync(0xffffffffu, it.live ? blocks_of(it, 1) : 0, 0);
   const int nb = max(nb0, nb1);
 
-  // 384 threads x 168 registers at launch = 64512 = 128 x 40 + 256 x 232: a
+  // 384 threads x 168 registers at launch = 64512 = 128 x 56 + 256 x 224: a
   // softmax thread holds its 128 scores in registers.
   if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     // ------------------------------------------------------------- producer
     if (warp == 8 && lane == 0 && nb > 0) {
       const uint64_t pol = l2_policy_evict_last();  // a head's K / V serve all its tiles
@@ -273,13 +392,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     // ------------------------------------------------------------------ MMA
-    if (warp == 9 && lane == 0 && nb > 0) {
+    if (warp == 9 && nb > 0) {
+      const uint32_t elected = elect_lane();
       const uint32_t idesc_s = idesc_f16(a.bf16, 0, 0, kTile, kTile);  // Q, K both K-major
       const uint32_t idesc_o = idesc_f16(a.bf16, 0, 1, kTile, kD);     // P K-major, V MN-major
-      const uint32_t q_addr = smem_u32(sQ), kv_addr = smem_u32(sKV);
+      const uint64_t q_desc = smem_desc_sw128(smem_u32(sQ), 16, 1024);
+      const uint64_t k_desc = smem_desc_sw128(smem_u32(sKV), 16, 1024);
+      const uint64_t v_desc = smem_desc_sw128(smem_u32(sKV), kHalf, 1024);
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t parity) {
-        if (ok) ok = !abort_flag[0] && mbar_wait(bar, parity, a.status);
+        if (ok) ok = __all_sync(0xffffffffu, !abort_flag[0] && mbar_wait(bar, parity, a.status));
       };
       auto scores = [&](int t, int j) {  // S_t = Q_t K_j^T
         const int i = 2 * j;
@@ -287,14 +409,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (j == 0) wait(q_full + t, 0);
         if (!ok) return;
         tc_fence_after();
-        const uint32_t qa = q_addr + t * kTileBytes, ka = kv_addr + (i % kSlots) * kTileBytes;
+        const uint64_t qd = q_desc + (t * kTileBytes >> 4);
+        const uint64_t kd = k_desc + ((i % kSlots) * kTileBytes >> 4);
 #pragma unroll
         for (int kk = 0; kk < kD / 16; ++kk) {
-          const uint32_t o = (kk >> 2) * kHalf + (kk & 3) * 32;
-          umma_f16(tmem + t * kTile, smem_desc_sw128(qa + o, 16, 1024),
-                   smem_desc_sw128(ka + o, 16, 1024), idesc_s, kk > 0 ? 1u : 0u);
+          const uint64_t o = ((kk >> 2) * kHalf + (kk & 3) * 32) >> 4;
+          mma_ss(elected, tmem + t * kTile, qd + o, kd + o, idesc_s, kk > 0 ? 1u : 0u);
         }
-        umma_commit(s_full + t);
+        mma_commit(elected, s_full + t);
       };
       auto values = [&](int t, int j) {  // O_t += P_t V_j
         const int i = 2 * j + 1;
@@ -302,17 +424,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         wait(p_full + t, j & 1);
         if (!ok) return;
         tc_fence_after();
-        const uint32_t va = kv_addr + (i % kSlots) * kTileBytes;
+        const uint64_t vd = v_desc + ((i % kSlots) * kTileBytes >> 4);
 #pragma unroll
         for (int kk = 0; kk < kTile / 16; ++kk)
-          umma_f16_ts(tmem + kTmemO + t * kD, tmem + t * kTile + kk * 8,
-                      smem_desc_sw128(va + kk * 2048, kHalf, 1024), idesc_o,
-                      (j > 0 || kk > 0) ? 1u : 0u);
+          mma_ts(elected, tmem + kTmemO + t * kD, tmem + t * kTile + kk * 8,
+                 vd + (kk * 2048 >> 4), idesc_o, (j > 0 || kk > 0) ? 1u : 0u);
       };
       // A slot is free when the last tile that reads it has: tile 1 if it sees
       // the block, else tile 0 (nb0 <= nb1 unless tile 1 has no rows).
       auto release = [&](int i) {
-        if (ok) umma_commit(kv_empty + i % kSlots);
+        if (ok) mma_commit(elected, kv_empty + i % kSlots);
       };
       if (nb0) scores(0, 0);
       if (nb1) scores(1, 0);
@@ -321,13 +442,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (j < nb0) {
           values(0, j);
           if (j + 1 < nb0) scores(0, j + 1);
-          else if (ok) umma_commit(o_done);
+          else if (ok) mma_commit(elected, o_done);
         }
         if (j < nb1) {
           values(1, j);
           release(2 * j + 1);
           if (j + 1 < nb1) scores(1, j + 1);
-          else if (ok) umma_commit(o_done + 1);
+          else if (ok) mma_commit(elected, o_done + 1);
         } else {
           release(2 * j + 1);
         }
@@ -335,11 +456,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (!ok) abort_flag[0] = 1;
       // every MMA of this CTA completes before TMEM is released
-      umma_commit(drain);
+      mma_commit(elected, drain);
       mbar_wait(drain, 0, a.status);
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     // -------------------------------------------------------------- softmax
     const int t = warp >> 2;
     const int r = (warp & 3) * 32 + lane;  // TMEM lane = row of the tile
@@ -360,28 +481,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         break;
       }
       tc_fence_after();
-      uint32_t s[128];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) ld32(s_addr + 32 * c, s + 32 * c);
-      ld_wait();
-#pragma unroll
-      for (int c = 0; c < 4; ++c) after_wait(s + 32 * c);
       const bool masked = j * kTile + kTile > all_seen;  // the diagonal, or the end
-      if (masked) {
-        const int lim = seen - j * kTile;
-#pragma unroll
-        for (int c = 0; c < 128; ++c)
-          if (c >= lim) s[c] = 0xff800000u;  // -inf
+      const int lim = seen - j * kTile;                  // this row's keys of the block
+      uint32_t p[64];
+      float lsum, mx;
+      if (j == 0) {  // nothing to go by yet: the row's maximum first
+        block_max(s_addr, masked, lim, mx);
+        mx *= a.scale_log2;
+        m = mx;
       }
-      float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
-#pragma unroll
-      for (int c = 0; c < 128; c += 8) {
-        mx0 = fmaxf(mx0, fmaxf(__uint_as_float(s[c]), __uint_as_float(s[c + 1])));
-        mx1 = fmaxf(mx1, fmaxf(__uint_as_float(s[c + 2]), __uint_as_float(s[c + 3])));
-        mx2 = fmaxf(mx2, fmaxf(__uint_as_float(s[c + 4]), __uint_as_float(s[c + 5])));
-        mx3 = fmaxf(mx3, fmaxf(__uint_as_float(s[c + 6]), __uint_as_float(s[c + 7])));
-      }
-      const float mx = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * a.scale_log2;
+      // a row that saw nothing yet (m = -inf): every score is -inf, P = 0
+      softmax_block<T>(s_addr, masked, lim, a.scale_log2, m == -INFINITY ? 0.f : -m, p, lsum, mx);
+      mx *= a.scale_log2;
       const bool moved = mx > m + kLazyLog2;
       if (__any_sync(0xffffffffu, moved)) {
         // tcgen05 loads and stores are warp-collective: rows that stay scale by 1
@@ -400,24 +511,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             st32(o_addr + c, o);
           }
         }
+        softmax_block<T>(s_addr, masked, lim, a.scale_log2, m == -INFINITY ? 0.f : -m, p, lsum, mx);
       }
-      const float neg = m == -INFINITY ? 0.f : -m;  // a row that saw nothing yet: P = 0
-      float l0 = 0.f, l1 = 0.f;
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint32_t p[32];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const int c = half * 64 + 2 * i;
-          const float x = exp2_ftz(fmaf(__uint_as_float(s[c]), a.scale_log2, neg));
-          const float y = exp2_ftz(fmaf(__uint_as_float(s[c + 1]), a.scale_log2, neg));
-          l0 += x;
-          l1 += y;
-          p[i] = pack16<T>(x, y);
-        }
-        st32(s_addr + 32 * half, p);
-      }
-      l += l0 + l1;
+      st32(s_addr, p);
+      st32(s_addr + 32, p + 32);
+      l += lsum;
       if (masked) {
         // V_j landed? (it follows K_j in the ring)
         const int i = 2 * j + 1;
