@@ -9,20 +9,26 @@
 // core must never wait. One CTA per SM works on 256 queries of one (sequence,
 // head) as two tiles of 128 that take turns: while one tile's scores are in
 // softmax, the other's products run.
-//   warps 0-3, 4-7  softmax of tile 0 / 1, one thread per query row: the row of
-//                   S (128 scores) goes TMEM -> registers in one read, its
-//                   maximum and exponentials stay there, P goes back to TMEM in
-//                   16 bits over S's own columns. P never touches shared memory.
+//   warps 0-3, 4-7  softmax of tile 0 / 1, one thread per query row: S (128 keys) goes
+//                   TMEM -> registers in chunks, P goes back in 16 bits over S's
+//                   own columns, in two halves of 64 keys, so that the first half
+//                   is multiplied while the second is still in softmax. P never
+//                   touches shared memory.
 //   warp 8          TMA: Q, then K and V blocks of 128 keys through a 5-slot ring
-//   warp 9          MMA issue, in the order
-//                   PV0(j) S0(j+1) PV1(j) S1(j+1): products of one thread run in
-//                   order, so S(j+1) may overwrite P(j), and a completed S(j+1)
-//                   says that O is at rest. No further barriers are needed.
+//   warp 9          MMA issue, per block and tile: O += P V for both halves, then the
+//                   next S = Q K^T over the columns that P leaves. Products of
+//                   one warp run in order, so no barrier says that.
 // TMEM (512 columns): S0 S1 (128 fp32 columns each), O0 O1.
+// Steps of 64 keys with two S buffers per tile were measured too (2.16 ms where this
+// takes SHORTER): a 128 x 64 product reads 6 KB of shared memory in 32 cycles' work
+// and so runs at two thirds of the rate.
 //
-// The running maximum moves only when a score exceeds it by 2^8 (P and the row
-// sum share it, so the result is exact either way): rescaling O, a read and
-// write of 128 columns, is rare after the first blocks. Sums and maxima are fp32;
+// P = 2^(s - m) needs no exact maximum, only one reference m for P, the row sum and
+// O that keeps P within 16 bits: m is the row's maximum over its first block and
+// moves only when the sum of 64 P exceeds 2^8 (so no P does otherwise). Then the
+// half is looked at again, O and the sum are rescaled (a read and write of 128
+// columns) and its P recomputed: rare after the first block, and until then no
+// maximum is taken at all. Sums and maxima are fp32;
 // P is rounded to the 16-bit type of V, its only rounding.
 //
 // A masked key's P is 0, but 0 * NaN is not: in the blocks that need a mask (the
@@ -45,12 +51,13 @@ constexpr int kTiles = 2;               // tiles of a CTA
 constexpr int kRows = kTile * kTiles;   // queries of a CTA
 constexpr int kTileBytes = kTile * kD * 2;
 constexpr int kHalf = kTileBytes / 2;   // one 64-column TMA box (128 rows x 128 bytes)
+constexpr int kKeys = 64;               // keys of half a block
 constexpr int kSlots = 5;
-constexpr int kThreads = 384;          // warps 10 and 11 only fill their warpgroup
+constexpr int kThreads = 320;
 constexpr int kSmem = 1024 + kTileBytes * (kTiles + kSlots) + 256;
 constexpr int kTmemCols = 512;
 constexpr int kTmemO = 256;             // S tiles at 0, 128; O tiles at 256, 384
-constexpr float kLazyLog2 = 8.f;
+constexpr float kMaxSum = 256.f;        // of 64 P, before the reference moves
 
 struct Args {
   void* out;
@@ -67,45 +74,64 @@ struct Args {
 // Inside a single-lane branch each operand would have to be moved to a uniform
 // register first, which made issuing a product take longer than the product
 // (155 instead of 64 cycles).
-PS_DEV uint32_t elect_lane() {
-  uint32_t e;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "elect.sync _|p, 0xffffffff;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}\n"
-      : "=r"(e));
-  return e;
-}
-// D[tmem] (+)= A[smem desc] * B[smem desc], kind::f16, by the elected lane.
-PS_DEV void mma_ss(uint32_t elected, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
-                   uint32_t idesc, uint32_t accumulate) {
+// A value that all lanes share, known as such to the compiler (a warp reduction
+// ends in a uniform register): loops over it and addresses made from it stay in
+// the uniform data path, which the product instructions take their operands from.
+PS_DEV uint32_t uniform(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
+
+// D[tmem] (+)= A[smem desc] * B[smem desc], kind::f16.
+PS_DEV void mma_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                   uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .pred p, e;\n\t"
-      "setp.ne.b32 e, %5, 0;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
       "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
-      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(elected)
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 // The same with A[tmem, 16-bit pairs].
-PS_DEV void mma_ts(uint32_t elected, uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
-                   uint32_t idesc, uint32_t accumulate) {
+PS_DEV void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                   uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .pred p, e;\n\t"
-      "setp.ne.b32 e, %5, 0;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
       "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(elected)
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-PS_DEV void mma_commit(uint32_t elected, uint64_t* bar) {
+PS_DEV void mma_commit(uint32_t bar) {
   asm volatile(
       "{\n\t.reg .pred e;\n\t"
-      "setp.ne.b32 e, %1, 0;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
       "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(
-          smem_u32(bar)),
-      "r"(elected)
+          bar)
       : "memory");
+}
+PS_DEV bool try_wait_at(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// mbar_wait on a shared-memory address.
+PS_DEV bool wait_at(uint32_t bar, uint32_t parity, int32_t* status) {
+  if (try_wait_at(bar, parity)) return true;
+  const uint64_t t0 = globaltimer_ns();
+  while (true) {
+    for (int i = 0; i < 64; ++i)
+      if (try_wait_at(bar, parity)) return true;
+    if (globaltimer_ns() - t0 > kWaitLimitNs) {
+      set_status(status, PS_ERR_TIMEOUT);
+      return false;
+    }
+  }
 }
 
 #define PS_R32(r)                                                                             \
@@ -188,11 +214,12 @@ PS_DEV uint64_t add2(uint64_t a, uint64_t b) {
   return d;
 }
 
-// The row's largest score of a block (raw, before the scale).
-PS_DEV void block_max(uint32_t s_addr, bool masked, int lim, float& mx) {
-  mx = -INFINITY;
+// The row's largest score of kCols columns (raw, before the scale).
+template <int kCols>
+PS_DEV float row_max(uint32_t s_addr, bool masked, int lim) {
+  float mx = -INFINITY;
 #pragma unroll 1
-  for (int c = 0; c < kTile; c += 32) {
+  for (int c = 0; c < kCols; c += 32) {
     uint32_t s[32];
     ld32(s_addr + c, s);
     ld_wait();
@@ -201,26 +228,25 @@ PS_DEV void block_max(uint32_t s_addr, bool masked, int lim, float& mx) {
     for (int i = 0; i < 32; ++i)
       mx = fmaxf(mx, masked && c + i >= lim ? -INFINITY : __uint_as_float(s[i]));
   }
+  return mx;
 }
 
-// P = 2^(s * scale + neg) of the row's 128 scores in 16 bits, their sum, and the
-// largest score: one pass over S, in chunks of 32 columns whose next one is on
-// its way while this one is worked on. P stays in registers until the caller
-// knows that neg was good enough; S is then overwritten.
+// P = 2^(s * scale + neg) of half a block, the row's 64 scores, in 16 bits, and
+// their sum. P stays in registers until the caller knows that neg was good
+// enough; S is then overwritten.
 template <typename T>
-PS_DEV void softmax_block(uint32_t s_addr, bool masked, int lim, float scale, float neg,
-                          uint32_t* p, float& lsum, float& mx) {
+PS_DEV float softmax_half(uint32_t s_addr, bool masked, int lim, float scale, float neg,
+                          uint32_t* p) {
   const uint64_t scale2 = pair(scale, scale), neg2 = pair(neg, neg);
   uint64_t l0 = pair(0.f, 0.f), l1 = l0;
-  float m0 = -INFINITY, m1 = -INFINITY;
   uint32_t s[2][32];
   ld32(s_addr, s[0]);
 #pragma unroll
-  for (int c = 0; c < 4; ++c) {
+  for (int c = 0; c < kKeys / 32; ++c) {
     uint32_t* v = s[c & 1];
     ld_wait();
     after_wait(v);
-    if (c < 3) ld32(s_addr + 32 * (c + 1), s[(c + 1) & 1]);
+    if (c + 1 < kKeys / 32) ld32(s_addr + 32 * (c + 1), s[(c + 1) & 1]);
     if (masked) {
 #pragma unroll
       for (int i = 0; i < 32; ++i)
@@ -228,13 +254,10 @@ PS_DEV void softmax_block(uint32_t s_addr, bool masked, int lim, float scale, fl
     }
 #pragma unroll
     for (int i = 0; i < 32; i += 4) {
-      const float a0 = __uint_as_float(v[i]), a1 = __uint_as_float(v[i + 1]);
-      const float b0 = __uint_as_float(v[i + 2]), b1 = __uint_as_float(v[i + 3]);
-      m0 = fmaxf(m0, fmaxf(a0, a1));
-      m1 = fmaxf(m1, fmaxf(b0, b1));
       float x0, x1, y0, y1;
-      unpair(fma2(pair(a0, a1), scale2, neg2), x0, x1);
-      unpair(fma2(pair(b0, b1), scale2, neg2), y0, y1);
+      unpair(fma2(pair(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), scale2, neg2), x0, x1);
+      unpair(fma2(pair(__uint_as_float(v[i + 2]), __uint_as_float(v[i + 3])), scale2, neg2), y0,
+             y1);
       x0 = exp2_ftz(x0);
       x1 = exp2_ftz(x1);
       y0 = exp2_ftz(y0);
@@ -247,8 +270,7 @@ PS_DEV void softmax_block(uint32_t s_addr, bool masked, int lim, float scale, fl
   }
   float s0, s1;
   unpair(add2(l0, l1), s0, s1);
-  lsum = s0 + s1;
-  mx = fmaxf(m0, m1);
+  return s0 + s1;
 }
 
 // Whether 8 16-bit values are all finite (an exponent of ones is not).
@@ -314,21 +336,23 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* kv_full = q_full + 2;      // [kSlots]
   uint64_t* kv_empty = kv_full + kSlots;
   uint64_t* s_full = kv_empty + kSlots;  // [2]
-  uint64_t* p_full = s_full + 2;         // [2]
-  uint64_t* o_done = p_full + 2;         // [2]
+  uint64_t* p_full = s_full + 2;         // [2 tiles][2 halves]
+  uint64_t* pv_done = p_full + 4;        // [2]: O += P V of a block's first half
+  uint64_t* o_done = pv_done + 2;        // [2]
   uint64_t* drain = o_done + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* poison = reinterpret_cast<int*>(tmem_slot + 2);  // first cleared key that was not finite
 
-  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int warp = (int)uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(q_full + i, 1);
       mbar_init(s_full + i, 1);
-      mbar_init(p_full + i, 4);
+      mbar_init(pv_done + i, 1);
       mbar_init(o_done + i, 1);
     }
+    for (int i = 0; i < 4; ++i) mbar_init(p_full + i, 4);
     for (int i = 0; i < kSlots; ++i) {
       mbar_init(kv_full + i, 1);
       mbar_init(kv_empty + i, 1);
@@ -345,20 +369,17 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+  const uint32_t tmem = uniform(*tmem_slot);
   pdl_wait();
   pdl_launch_dependents();
 
   const int h = blockIdx.x % a.n_heads;
   const Item it = item_at(a, blockIdx.x / a.n_heads);
-  const int nb0 = __shfl_sync(0xffffffffu, it.live ? blocks_of(it, 0) : 0, 0);
-  const int nb1 = __shfl_sync(0xffffffffu, it.live ? blocks_of(it, 1) : 0, 0);
+  const int nb0 = (int)uniform(it.live ? blocks_of(it, 0) : 0);
+  const int nb1 = (int)uniform(it.live ? blocks_of(it, 1) : 0);
   const int nb = max(nb0, nb1);
 
-  // 384 threads x 168 registers at launch = 64512 = 128 x 56 + 256 x 224: a
-  // softmax thread holds its 128 scores in registers.
   if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     // ------------------------------------------------------------- producer
     if (warp == 8 && lane == 0 && nb > 0) {
       const uint64_t pol = l2_policy_evict_last();  // a head's K / V serve all its tiles
@@ -393,80 +414,96 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     // ------------------------------------------------------------------ MMA
     if (warp == 9 && nb > 0) {
-      const uint32_t elected = elect_lane();
       const uint32_t idesc_s = idesc_f16(a.bf16, 0, 0, kTile, kTile);  // Q, K both K-major
       const uint32_t idesc_o = idesc_f16(a.bf16, 0, 1, kTile, kD);     // P K-major, V MN-major
       const uint64_t q_desc = smem_desc_sw128(smem_u32(sQ), 16, 1024);
       const uint64_t k_desc = smem_desc_sw128(smem_u32(sKV), 16, 1024);
       const uint64_t v_desc = smem_desc_sw128(smem_u32(sKV), kHalf, 1024);
+      // Between a wait and the next product the queue of issued products covers
+      // about 100 cycles, so this loop keeps addresses, slots and phases in
+      // registers and waits as rarely as it can: once for each P, once for
+      // each K and V block. What a wait that ran out leads to is decided once
+      // a block; an aborting warp is not looked for, its waits run out too.
+      const uint32_t bar0 = smem_u32(bars);
+      const uint32_t kv_full_a = bar0 + 16, kv_empty_a = kv_full_a + 8 * kSlots;
+      const uint32_t s_full_a = kv_empty_a + 8 * kSlots, p_full_a = s_full_a + 16;
+      const uint32_t pv_done_a = p_full_a + 32, o_done_a = pv_done_a + 16;
       bool ok = true;
-      auto wait = [&](uint64_t* bar, uint32_t parity) {
-        if (ok) ok = __all_sync(0xffffffffu, !abort_flag[0] && mbar_wait(bar, parity, a.status));
+      auto wait = [&](uint32_t bar, uint32_t parity) {
+        ok = wait_at(bar, parity, a.status) && ok;
       };
-      auto scores = [&](int t, int j) {  // S_t = Q_t K_j^T
-        const int i = 2 * j;
-        wait(kv_full + i % kSlots, (i / kSlots) & 1);
-        if (j == 0) wait(q_full + t, 0);
-        if (!ok) return;
-        tc_fence_after();
+      // S_t = Q_t K^T, K's block in ring slot `slot`
+      auto scores = [&](int t, int slot) {
         const uint64_t qd = q_desc + (t * kTileBytes >> 4);
-        const uint64_t kd = k_desc + ((i % kSlots) * kTileBytes >> 4);
+        const uint64_t kd = k_desc + (uint32_t)(slot * (kTileBytes >> 4));
 #pragma unroll
         for (int kk = 0; kk < kD / 16; ++kk) {
           const uint64_t o = ((kk >> 2) * kHalf + (kk & 3) * 32) >> 4;
-          mma_ss(elected, tmem + t * kTile, qd + o, kd + o, idesc_s, kk > 0 ? 1u : 0u);
+          mma_ss(tmem + t * kTile, qd + o, kd + o, idesc_s, kk > 0 ? 1u : 0u);
         }
-        mma_commit(elected, s_full + t);
+        mma_commit(s_full_a + 8 * t);
       };
-      auto values = [&](int t, int j) {  // O_t += P_t V_j
-        const int i = 2 * j + 1;
-        wait(kv_full + i % kSlots, (i / kSlots) & 1);
-        wait(p_full + t, j & 1);
-        if (!ok) return;
-        tc_fence_after();
-        const uint64_t vd = v_desc + ((i % kSlots) * kTileBytes >> 4);
+      // O_t += P_t V of one half of a block
+      auto values = [&](int t, int half, int slot, bool first) {
+        const uint64_t vd = v_desc + (uint32_t)(slot * (kTileBytes >> 4) + half * (kKeys * 128 >> 4));
 #pragma unroll
-        for (int kk = 0; kk < kTile / 16; ++kk)
-          mma_ts(elected, tmem + kTmemO + t * kD, tmem + t * kTile + kk * 8,
-                 vd + (kk * 2048 >> 4), idesc_o, (j > 0 || kk > 0) ? 1u : 0u);
+        for (int kk = 0; kk < kKeys / 16; ++kk)
+          mma_ts(tmem + kTmemO + t * kD, tmem + t * kTile + half * kKeys + kk * 8,
+                 vd + (kk * 2048 >> 4), idesc_o, kk > 0 || !first ? 1u : 0u);
       };
-      // A slot is free when the last tile that reads it has: tile 1 if it sees
-      // the block, else tile 0 (nb0 <= nb1 unless tile 1 has no rows).
-      auto release = [&](int i) {
-        if (ok) mma_commit(elected, kv_empty + i % kSlots);
-      };
-      if (nb0) scores(0, 0);
-      if (nb1) scores(1, 0);
-      release(0);
+      wait(kv_full_a, 0);
+      if (nb0) wait(bar0, 0);
+      if (nb1) wait(bar0 + 8, 0);
+      tc_fence_after();
+      ok = __all_sync(0xffffffffu, ok);
+      if (ok) {
+        if (nb0) scores(0, 0);
+        if (nb1) scores(1, 0);
+        mma_commit(kv_empty_a);
+      }
+      // block j: V in slot vs, and the next block's K in slot ks
+      int vs = 1, ks = 2;
+      uint32_t vph = 0, kph = 0;
+#pragma unroll 1
       for (int j = 0; ok && j < nb; ++j) {
-        if (j < nb0) {
-          values(0, j);
-          if (j + 1 < nb0) scores(0, j + 1);
-          else if (ok) mma_commit(elected, o_done);
+        wait(kv_full_a + 8 * vs, vph);
+        if (j + 1 < nb) wait(kv_full_a + 8 * ks, kph);
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) {
+          const int n = t ? nb1 : nb0;
+          if (j < n) {
+            wait(p_full_a + 16 * t, j & 1);
+            tc_fence_after();
+            values(t, 0, vs, j == 0);
+            mma_commit(pv_done_a + 8 * t);
+            wait(p_full_a + 16 * t + 8, j & 1);
+            tc_fence_after();
+            values(t, 1, vs, false);
+            if (j + 1 < n)
+              scores(t, ks);
+            else
+              mma_commit(o_done_a + 8 * t);
+          }
         }
-        if (j < nb1) {
-          values(1, j);
-          release(2 * j + 1);
-          if (j + 1 < nb1) scores(1, j + 1);
-          else if (ok) mma_commit(elected, o_done + 1);
-        } else {
-          release(2 * j + 1);
-        }
-        if (j + 1 < nb) release(2 * j + 2);
+        // Everything that reads these slots has been issued: free them when done
+        mma_commit(kv_empty_a + 8 * vs);
+        if (j + 1 < nb) mma_commit(kv_empty_a + 8 * ks);
+        vs += 2, ks += 2;
+        if (vs >= kSlots) vs -= kSlots, vph ^= 1;
+        if (ks >= kSlots) ks -= kSlots, kph ^= 1;
+        ok = __all_sync(0xffffffffu, ok);
       }
       if (!ok) abort_flag[0] = 1;
       // every MMA of this CTA completes before TMEM is released
-      mma_commit(elected, drain);
+      mma_commit(smem_u32(drain));
       mbar_wait(drain, 0, a.status);
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     // -------------------------------------------------------------- softmax
     const int t = warp >> 2;
     const int r = (warp & 3) * 32 + lane;  // TMEM lane = row of the tile
     const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_addr = tmem + t * kTile + lane_off;
-    const uint32_t o_addr = tmem + kTmemO + t * kD + lane_off;
+      const uint32_t o_addr = tmem + kTmemO + t * kD + lane_off;
     const int first = it.row + t * kTile;
     const int row = first + r;
     const int my_nb = t ? nb1 : nb0;
@@ -474,8 +511,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int all_seen = first + 1 + it.lk - it.lq;  // seen by every row of the tile
     float m = -INFINITY, l = 0.f;
     bool ok = true;
-    for (int j = 0; j < my_nb; ++j) {
-      const bool got = !abort_flag[0] && mbar_wait(s_full + t, j & 1, a.status);
+    const uint32_t s_addr = tmem + t * kTile + lane_off;
+    for (int j = 0; j < my_nb && ok; ++j) {
+      const bool got = !abort_flag[0] && wait_at(smem_u32(s_full + t), j & 1, a.status);
       if (!__all_sync(0xffffffffu, got)) {  // the warp leaves together (collective TMEM ops)
         ok = false;
         break;
@@ -483,70 +521,79 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after();
       const bool masked = j * kTile + kTile > all_seen;  // the diagonal, or the end
       const int lim = seen - j * kTile;                  // this row's keys of the block
-      uint32_t p[64];
-      float lsum, mx;
-      if (j == 0) {  // nothing to go by yet: the row's maximum first
-        block_max(s_addr, masked, lim, mx);
-        mx *= a.scale_log2;
-        m = mx;
+      if (j == 0) {  // nothing to go by yet: the row's maximum (0 for a row of -inf)
+        m = row_max<kTile>(s_addr, masked, lim) * a.scale_log2;
+        if (m == -INFINITY) m = 0.f;
       }
-      // a row that saw nothing yet (m = -inf): every score is -inf, P = 0
-      softmax_block<T>(s_addr, masked, lim, a.scale_log2, m == -INFINITY ? 0.f : -m, p, lsum, mx);
-      mx *= a.scale_log2;
-      const bool moved = mx > m + kLazyLog2;
-      if (__any_sync(0xffffffffu, moved)) {
-        // tcgen05 loads and stores are warp-collective: rows that stay scale by 1
-        const float alpha = moved ? exp2_ftz(m - mx) : 1.f;
-        if (moved) m = mx;
-        l *= alpha;
-        if (j > 0) {
 #pragma unroll 1
-          for (int c = 0; c < kD; c += 32) {
-            uint32_t o[32];
-            ld32(o_addr + c, o);
-            ld_wait();
-            after_wait(o);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-            st32(o_addr + c, o);
+      for (int half = 0; half < 2; ++half) {
+        const uint32_t h_addr = s_addr + half * kKeys;
+        const int hlim = lim - half * kKeys;
+        uint32_t p[32];
+        float lsum = softmax_half<T>(h_addr, masked, hlim, a.scale_log2, -m, p);
+        if (__any_sync(0xffffffffu, lsum > kMaxSum)) {
+          // tcgen05 loads and stores are warp-collective: rows that stay scale by 1
+          const float mx = row_max<kKeys>(h_addr, masked, hlim) * a.scale_log2;
+          const bool moved = lsum > kMaxSum && mx > m;
+          const float alpha = moved ? exp2_ftz(m - mx) : 1.f;
+          if (moved) m = mx;
+          l *= alpha;
+          // O is at rest: S(j) says that block j - 1 is in it, and of this block
+          // only the first half can be on its way, when this is the second.
+          bool rest = true;
+          if (half) rest = mbar_wait(pv_done + t, j & 1, a.status);
+          if (!__all_sync(0xffffffffu, rest)) {
+            ok = false;
+            break;
           }
-        }
-        softmax_block<T>(s_addr, masked, lim, a.scale_log2, m == -INFINITY ? 0.f : -m, p, lsum, mx);
-      }
-      st32(s_addr, p);
-      st32(s_addr + 32, p + 32);
-      l += lsum;
-      if (masked) {
-        // V_j landed? (it follows K_j in the ring)
-        const int i = 2 * j + 1;
-        if (mbar_wait(kv_full + i % kSlots, (i / kSlots) & 1, a.status)) {
-          uint8_t* v = sKV + (i % kSlots) * kTileBytes + r * 128;
-          bool clear = r >= it.lk - j * kTile;
-          if (!clear) {
-            bool fin = true;
+          if (j > 0 || half) {
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < kD; c += 32) {
+              uint32_t o[32];
+              ld32(o_addr + c, o);
+              ld_wait();
+              after_wait(o);
 #pragma unroll
-            for (int c = 0; c < 16; ++c)  // 16-byte chunks, rotated by row: no bank conflicts
-              fin &= finite8<T>(
-                  *reinterpret_cast<const uint4*>(v + (c >> 3) * kHalf + (((c + r) & 7) << 4)));
-            if (!fin) {
-              clear = true;
-              atomicMin(poison, j * kTile + r);
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+              st32(o_addr + c, o);
             }
           }
-          if (clear) {
-#pragma unroll
-            for (int c = 0; c < 16; ++c)
-              *reinterpret_cast<uint4*>(v + (c >> 3) * kHalf + (((c + r) & 7) << 4)) =
-                  make_uint4(0u, 0u, 0u, 0u);
-          }
+          lsum = softmax_half<T>(h_addr, masked, hlim, a.scale_log2, -m, p);
         }
-        fence_proxy_async_smem();  // the cleared rows -> the tensor core's view
+        st32(h_addr, p);
+        l += lsum;
+        if (masked) {
+          // V landed? (it follows K in the ring). Two threads to a row, 128 bytes each.
+          const int i = 2 * j + 1, key = j * kTile + half * kKeys + (r & (kKeys - 1));
+          if (mbar_wait(kv_full + i % kSlots, (i / kSlots) & 1, a.status)) {
+            uint8_t* v = sKV + (i % kSlots) * kTileBytes + (r >> 6) * kHalf +
+                         (key & (kTile - 1)) * 128;
+            bool clear = key >= it.lk;
+            if (!clear) {
+              bool fin = true;
+#pragma unroll
+              for (int c = 0; c < 8; ++c)  // 16-byte chunks, rotated by row: no bank conflicts
+                fin &= finite8<T>(*reinterpret_cast<const uint4*>(v + (((c + r) & 7) << 4)));
+              if (!fin) {
+                clear = true;
+                atomicMin(poison, key);
+              }
+            }
+            if (clear) {
+#pragma unroll
+              for (int c = 0; c < 8; ++c)
+                *reinterpret_cast<uint4*>(v + (((c + r) & 7) << 4)) = make_uint4(0u, 0u, 0u, 0u);
+            }
+          }
+          fence_proxy_async_smem();  // the cleared rows -> the tensor core's view
+        }
+        __syncwarp();
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full + 2 * t + half);
       }
-      __syncwarp();
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(p_full + t);
     }
     const bool live = it.live && row < it.lq;
     bool fin = ok;
