@@ -52,18 +52,6 @@ class GemmEpilogue(ctypes.Structure):
         ("w_packed", _p), ("max_ctas", _i),
     ]
 
-
-class KV4PoolDesc(ctypes.Structure):
-    """ps_kv4_pool_t (one model's 4-bit K and V pools)."""
-    _fields_ = [("k_codes", _p), ("k_meta", _p), ("v_codes", _p), ("v_meta", _p), ("rows", _i)]
-
-
-class KV4CacheDesc(ctypes.Structure):
-    """ps_kv4_cache_t (both models' pools and their paging)."""
-    _fields_ = [("pool", KV4PoolDesc * 2), ("block_table", _p), ("n_kv_heads", _i),
-                ("L_cap", _i), ("page_size", _i), ("max_pages", _i), ("table_rows", _i)]
-
-
 PS_JOB_GEMM, PS_JOB_ALLREDUCE = 0, 1
 
 
@@ -108,11 +96,11 @@ SIGNATURES: dict[str, tuple] = {
                                   _i, _i, _f, _i, _p, _p]),
     "ps_qk_norm_rope": (_i, [_p, _ll, _p, _ll, _p, _ll, _p, _ll, _p, _p, _f, _p, _p, _i, _i, _i,
                              _p, _p, _i, _i, _i, _i, _i, _p, _p]),
-    "ps_kv4_append": (_i, [_p, _ll, _p, _ll, _p, _ll, _p, _ll, ctypes.POINTER(KV4CacheDesc), _p,
+    "ps_kv4_append": (_i, [_p, _ll, _p, _ll, _p, _ll, _p, _ll, _p, _p,
                            _p, _f, _p, _p, _i, _i, _i, _p, _p, _p, _i, _i, _i, _i, _p, _p]),
-    "ps_kv4_gather": (_i, [ctypes.POINTER(KV4CacheDesc), _p, _p, _i, _i, _p, _p, _i, _p, _p]),
+    "ps_kv4_gather": (_i, [_p, _p, _p, _i, _i, _p, _p, _i, _p, _p]),
     "ps_kv4_decode_attention_workspace_bytes": (_sz, [_i, _i, _i, _i]),
-    "ps_kv4_decode_attention": (_i, [_p, _ll, ctypes.POINTER(KV4CacheDesc), _p, _p, _p, _p, _i,
+    "ps_kv4_decode_attention": (_i, [_p, _ll, _p, _p, _p, _p, _p, _i,
                                      _i, _i, _i, _f, _i, _p, _sz, _p, _p]),
     "ps_prompt_attention": (_i, [_p, _ll, _p, _ll, _p, _ll, _p, _ll, _p, _p, _i, _i, _i, _i, _i,
                                  _f, _i, _p, _p]),
@@ -195,6 +183,17 @@ def status_tensor(device: torch.device) -> torch.Tensor:
         return t
 
 
+_status_ptrs: dict[int, int] = {}
+
+
+def status_ptr(idx: int) -> int:
+    """Address of device idx's status word."""
+    p = _status_ptrs.get(idx)
+    if p is None:
+        p = _status_ptrs[idx] = status_tensor(torch.device("cuda", idx)).data_ptr()
+    return p
+
+
 def read_status(device: torch.device, clear: bool = True) -> int:
     """Synchronizes, returns the device status bits and (by default) clears them."""
     t = status_tensor(device)
@@ -212,8 +211,12 @@ def workspace(device: torch.device, nbytes: int, tag: str) -> torch.Tensor:
     only when first allocated or grown.
     """
     dev = torch.device(device)
-    idx = dev.index or 0
-    key = (idx, torch.cuda.current_stream(dev).cuda_stream, tag)
+    return stream_workspace(dev.index or 0, torch.cuda.current_stream(dev).cuda_stream, nbytes, tag)
+
+
+def stream_workspace(idx: int, stream: int, nbytes: int, tag: str) -> torch.Tensor:
+    """``workspace`` of device idx's stream handle."""
+    key = (idx, stream, tag)
     with _lock:
         buf = _workspaces.get(key)
         if buf is None or buf.numel() < nbytes:

@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 
 import torch
 
@@ -382,152 +383,161 @@ def positions_routed(seq_len: torch.Tensor, perm: torch.Tensor | None, out: torc
 
 
 # ---------------------------------------------------------------- 4-bit KV cache, head norms
+#
+# These calls follow one another every few microseconds in a decode step, so
+# their host side is kept short: plain comparisons, no keyword dictionaries, and
+# descriptors packed as bytes.
 
 _HD = 128
+_CACHE = struct.Struct("=4Qi4x4Qi4xQ5i4x")       # ps_kv4_cache_t
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
 
 
 def _heads(t: torch.Tensor, name: str) -> tuple[int, int, int]:
     """(tokens, heads, token stride) of ``[tokens, heads, 128]`` or ``[tokens,
     heads * 128]`` whose heads lie one after another (views of a qkv row do)."""
-    if not t.is_cuda:
-        raise ValueError("parallel-serve ops take CUDA tensors")
-    if t.dim() == 3:
-        n, h, d = t.shape
-        ok = d == _HD and t.stride(2) == 1 and (h == 1 or t.stride(1) == _HD)
-    elif t.dim() == 2:
-        n, d = t.shape
+    sh, st = t.shape, t.stride()
+    if len(sh) == 3:
+        n, h, d = sh
+        ok = d == _HD and st[2] == 1 and (h == 1 or st[1] == _HD)
+    elif len(sh) == 2:
+        n, d = sh
         h = d // _HD
-        ok = d % _HD == 0 and t.stride(1) == 1
+        ok = d % _HD == 0 and st[1] == 1
     else:
         ok = False
     if not ok or h == 0:
         raise ValueError(f"{name} must be [tokens, heads, 128] (or [tokens, heads * 128]) with "
                          "contiguous heads")
-    stride = t.stride(0) if n > 1 else h * _HD
+    stride = st[0] if n > 1 else h * _HD
     if stride < h * _HD or stride % 8:
         raise ValueError(f"{name}: token stride {stride} must be a multiple of 8 and hold every head")
     return n, h, stride
 
 
-def _int32(t: torch.Tensor | None, name: str, n: int, device: torch.device) -> int | None:
-    """Pointer of a contiguous int32 vector of at least n entries (None stays None)."""
+def _int32(t: torch.Tensor | None, name: str, n: int, idx: int) -> int | None:
+    """Pointer of a contiguous int32 tensor of at least n entries (None stays None)."""
     if t is None:
         return None
-    if t.dtype != torch.int32 or t.device != device or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous int32 tensor on {device}")
+    if t.dtype != torch.int32 or t.get_device() != idx or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor on cuda:{idx}")
     if t.numel() < n:
         raise ValueError(f"{name} needs {n} entries, has {t.numel()}")
     return t.data_ptr()
 
 
-def _same(device: torch.device, dtype: torch.dtype | None, **ts) -> None:
-    for name, t in ts.items():
-        if t is None:
-            continue
-        if t.device != device:
-            raise ValueError(f"{name} is on {t.device}, expected {device}")
-        if dtype is not None and t.dtype != dtype:
-            raise TypeError(f"{name} is {t.dtype}, expected {dtype}")
+def _on(t: torch.Tensor, name: str, idx: int, dtype: torch.dtype) -> None:
+    if t.get_device() != idx:
+        raise ValueError(f"{name} is on {t.device}, expected cuda:{idx}")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} is {t.dtype}, expected {dtype}")
 
 
-def _head_weight(w: torch.Tensor | None, name: str, device, dtype) -> int | None:
+def _first(t: torch.Tensor) -> tuple[int, int]:
+    """(device index, dtype code) that the other tensors of a call have to match."""
+    idx = t.get_device()
+    if idx < 0:
+        raise ValueError("parallel-serve ops take CUDA tensors")
+    return idx, _lib.dtype_code(t.dtype)
+
+
+def _head_weight(w: torch.Tensor | None, name: str, idx: int, dtype: torch.dtype) -> int | None:
     if w is None:
         return None
-    _same(device, dtype, **{name: w})
+    _on(w, name, idx, dtype)
     if w.shape != (2, _HD) or not w.is_contiguous():
         raise ValueError(f"{name} must be contiguous [2, 128] (one row per model)")
     return w.data_ptr()
 
 
-def _rope_args(cos, sin, device) -> tuple:
+def _rope_args(cos, sin, idx: int) -> tuple:
     """(cos, sin pointers, positions, rotary_dim) of the rotation tables."""
-    if (cos is None) != (sin is None):
-        raise ValueError("rope_cos and rope_sin come together")
-    if cos is None:
+    if cos is None and sin is None:
         return None, None, 0, 0
-    _same(device, torch.float32, rope_cos=cos, rope_sin=sin)
-    if cos.dim() != 2 or cos.shape != sin.shape or not (cos.is_contiguous() and sin.is_contiguous()):
+    if cos is None or sin is None:
+        raise ValueError("rope_cos and rope_sin come together")
+    _on(cos, "rope_cos", idx, torch.float32)
+    _on(sin, "rope_sin", idx, torch.float32)
+    sh = cos.shape
+    if len(sh) != 2 or sh != sin.shape or not (cos.is_contiguous() and sin.is_contiguous()):
         raise ValueError("rope tables must be contiguous [positions, rotary_dim / 2]")
-    rotary = 2 * cos.shape[1]
-    if rotary % 16 or not 0 < rotary <= _HD or cos.shape[0] == 0:
+    n, rotary = sh[0], 2 * sh[1]
+    if rotary % 16 or not 0 < rotary <= _HD or n == 0:
         raise ValueError("rotary_dim must be a multiple of 16 up to 128, with at least one position")
-    return cos.data_ptr(), sin.data_ptr(), cos.shape[0], rotary
+    return cos.data_ptr(), sin.data_ptr(), n, rotary
 
 
-def _split(split_point: int | None, M: int) -> int:
+def _split_counts(split_point: int | None, counts: torch.Tensor | None, M: int,
+                  idx: int) -> tuple[int, int | None]:
+    """(split point, counts pointer); neither given: every token is model 0's."""
+    if counts is not None:
+        return 0, _int32(counts, "counts", 2, idx)
     if split_point is None:
-        return M
+        return M, None
     if not 0 <= split_point <= M:
         raise ValueError(f"split_point must be in [0, {M}]")
-    return split_point
+    return split_point, None
 
 
-class _device_of:
-    """Makes the tensors' device current for the launch when it is not."""
-    __slots__ = ("idx", "prev")
-
-    def __init__(self, device: torch.device):
-        self.idx = device.index
-
-    def __enter__(self):
-        self.prev = torch.cuda.current_device()
-        if self.prev != self.idx:
-            torch.cuda.set_device(self.idx)
-
-    def __exit__(self, *exc):
-        if self.prev != self.idx:
-            torch.cuda.set_device(self.prev)
+def _call(fn, what: str, idx: int, *args) -> None:
+    """Launch on the tensors' device (made current for the call when it is not),
+    on its current torch stream, with its status word."""
+    if _current_device() == idx:
+        rc = fn(*args, _lib.status_ptr(idx), _raw_stream(idx))
+    else:
+        with torch.cuda.device(idx):
+            rc = fn(*args, _lib.status_ptr(idx), _raw_stream(idx))
+    if rc:
+        check(rc, what)
 
 
-def _kv4_cache(pools, block_table: torch.Tensor | None, device, dtype) -> _lib.KV4CacheDesc:
-    """Validate both models' 4-bit pools (``KV4Pool`` or None) and the block table."""
-    c = _lib.KV4CacheDesc()
+def _kv4_cache(pools, block_table: torch.Tensor | None, idx: int,
+               dtype: torch.dtype) -> tuple[bytes, int, int]:
+    """Both models' 4-bit pools (``KV4Pool`` or None) and the block table, checked:
+    (ps_kv4_cache_t as bytes, KV heads, positions a sequence can have)."""
     if len(pools) != 2:
         raise ValueError("pools are (model 0's, model 1's), either may be None")
     n_kv = length = 0
-    for m, p in enumerate(pools):
+    desc = []
+    for p in pools:
         if p is None or p[0].shape[0] == 0:
+            desc += (0, 0, 0, 0, 0)
             continue
         kc, km, vc, vm = p
-        sh = kc.shape
-        if len(sh) != 4 or sh[3] != 64 or vc.shape != sh or km.shape != (*sh[:3], 4, 2) or \
-                vm.shape != km.shape:
+        sh, ms = kc.shape, km.shape
+        if len(sh) != 4 or sh[3] != 64 or vc.shape != sh or len(ms) != 5 or \
+                ms[:3] != sh[:3] or ms[3:] != (4, 2) or vm.shape != ms:
             raise ValueError("a 4-bit pool is codes [rows, n_kv_heads, length, 64] and meta "
                              "[rows, n_kv_heads, length, 4, 2], for K and for V")
         if kc.dtype != torch.uint8 or vc.dtype != torch.uint8 or km.dtype != dtype or \
                 vm.dtype != dtype:
             raise TypeError(f"a 4-bit pool holds uint8 codes and {dtype} meta here")
         for t in p:
-            if t.device != device or not t.is_contiguous():
-                raise ValueError(f"4-bit pools must be contiguous tensors on {device}")
+            if t.get_device() != idx or not t.is_contiguous():
+                raise ValueError(f"4-bit pools must be contiguous tensors on cuda:{idx}")
         if n_kv and (n_kv, length) != (sh[1], sh[2]):
             raise ValueError("both models' pools must have the same heads and length")
         n_kv, length = sh[1], sh[2]
-        d = c.pool[m]
-        d.k_codes, d.k_meta, d.v_codes, d.v_meta = (kc.data_ptr(), km.data_ptr(), vc.data_ptr(),
-                                                    vm.data_ptr())
-        d.rows = sh[0]
+        desc += (kc.data_ptr(), km.data_ptr(), vc.data_ptr(), vm.data_ptr(), sh[0])
     if not n_kv or not length:
         raise ValueError("at least one model needs a 4-bit pool")
-    c.n_kv_heads = n_kv
     if block_table is None:
-        c.L_cap = length
-    else:
-        if block_table.dim() != 2:
-            raise ValueError("block_table must be int32 [rows, max_pages]")
-        c.block_table = _int32(block_table, "block_table", 1, device)
-        c.table_rows, c.max_pages = block_table.shape
-        c.page_size = length
-        if length < 8 or length > 4096 or length & (length - 1):
-            raise ValueError("page_size must be a power of two in [8, 4096]")
-    return c
+        return _CACHE.pack(*desc, 0, n_kv, length, 0, 0, 0), n_kv, length
+    sh = block_table.shape
+    if len(sh) != 2 or not sh[0] or not sh[1]:
+        raise ValueError("block_table must be int32 [rows, max_pages]")
+    if length < 8 or length > 4096 or length & (length - 1):
+        raise ValueError("page_size must be a power of two in [8, 4096]")
+    return (_CACHE.pack(*desc, _int32(block_table, "block_table", 1, idx), n_kv, 0, length, sh[1],
+                        sh[0]), n_kv, sh[1] * length)
 
 
-def _home_arg(rows, block_table, M: int, device) -> int | None:
+def _home_arg(rows, block_table, M: int, idx: int) -> int | None:
     """Pointer of the tokens' cache rows; without them a table needs a row per token."""
     if rows is None and block_table is not None and block_table.shape[0] < M:
         raise ValueError("block_table needs a row per token when rows is not given")
-    return _int32(rows, "rows", M, device)
+    return _int32(rows, "rows", M, idx)
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, pos: torch.Tensor, *,
@@ -546,32 +556,36 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, pos: torch.Tensor, *,
     rotary_dim channels, as pairs (i, i + rotary_dim / 2), or (2i, 2i + 1) when
     ``interleaved``. Tokens are in routed order: the first ``split_point`` (or
     counts[0], read on the device; default: all) belong to model 0.
-    ``q_out`` / ``k_out`` may be the inputs themselves.
+    ``q_out`` / ``k_out`` may be the inputs themselves. A position outside the
+    tables raises PS_ERR_BAD_INDEX in the status word and leaves its rows unwritten.
     """
+    idx, code = _first(q)
+    dt = q.dtype
     M, nh, qs = _heads(q, "q")
     Mk, nkv, ks = _heads(k, "k")
-    dev, dt = q.device, q.dtype
-    code = _lib.dtype_code(dt)
+    _on(k, "k", idx, dt)
     if Mk != M:
         raise ValueError("q and k must have the same tokens")
-    _same(dev, dt, k=k, q_out=q_out, k_out=k_out)
-    _same(dev, None, counts=counts)
-    q_out = torch.empty(q.shape, dtype=dt, device=dev) if q_out is None else q_out
-    k_out = torch.empty(k.shape, dtype=dt, device=dev) if k_out is None else k_out
-    Mq, nho, qos = _heads(q_out, "q_out")
-    Mo, nko, kos = _heads(k_out, "k_out")
-    if (Mq, nho, Mo, nko) != (M, nh, M, nkv):
-        raise ValueError("q_out / k_out must have the shapes of q / k")
-    rc, rs, rope_len, rotary = _rope_args(rope_cos, rope_sin, dev)
-    with _device_of(dev):
-        check(lib.ps_qk_norm_rope(q.data_ptr(), qs, k.data_ptr(), ks, q_out.data_ptr(), qos,
-                                  k_out.data_ptr(), kos, _head_weight(q_weight, "q_weight", dev, dt),
-                                  _head_weight(k_weight, "k_weight", dev, dt), float(eps), rc, rs,
-                                  rope_len, rotary, 1 if interleaved else 0,
-                                  _int32(pos, "pos", M, dev), _counts_arg(counts),
-                                  _split(split_point, M), M, nh, nkv, code,
-                                  ptr(_lib.status_tensor(dev)), _lib.stream_handle(dev)),
-              "ps_qk_norm_rope")
+    if q_out is None:
+        q_out, qos = q.new_empty(q.shape), nh * _HD
+    else:
+        _on(q_out, "q_out", idx, dt)
+        n, h, qos = _heads(q_out, "q_out")
+        if (n, h) != (M, nh):
+            raise ValueError("q_out must have the shape of q")
+    if k_out is None:
+        k_out, kos = k.new_empty(k.shape), nkv * _HD
+    else:
+        _on(k_out, "k_out", idx, dt)
+        n, h, kos = _heads(k_out, "k_out")
+        if (n, h) != (M, nkv):
+            raise ValueError("k_out must have the shape of k")
+    rc, rs, rope_len, rotary = _rope_args(rope_cos, rope_sin, idx)
+    split, cnt = _split_counts(split_point, counts, M, idx)
+    _call(lib.ps_qk_norm_rope, "ps_qk_norm_rope", idx, q.data_ptr(), qs, k.data_ptr(), ks,
+          q_out.data_ptr(), qos, k_out.data_ptr(), kos, _head_weight(q_weight, "q_weight", idx, dt),
+          _head_weight(k_weight, "k_weight", idx, dt), eps, rc, rs, rope_len, rotary,
+          1 if interleaved else 0, _int32(pos, "pos", M, idx), cnt, split, M, nh, nkv, code)
     return q_out, k_out
 
 
@@ -593,36 +607,40 @@ def kv4_append(k: torch.Tensor, v: torch.Tensor, pools: tuple, pos: torch.Tensor
     returns in 16 bits. Two tokens of a call must not share a position of a
     sequence. Returns q_out, or None without ``q``.
     """
+    idx, code = _first(k)
+    dt = k.dtype
     M, nkv, ks = _heads(k, "k")
     Mv, nv, vs = _heads(v, "v")
-    dev, dt = k.device, k.dtype
-    code = _lib.dtype_code(dt)
+    _on(v, "v", idx, dt)
     if (Mv, nv) != (M, nkv):
         raise ValueError("k and v must have the same shape")
-    _same(dev, dt, v=v, q=q, q_out=q_out)
-    _same(dev, None, counts=counts)
-    cache = _kv4_cache(pools, block_table, dev, dt)
-    if cache.n_kv_heads != nkv:
-        raise ValueError(f"k has {nkv} heads, the pools {cache.n_kv_heads}")
+    cache, n, _ = _kv4_cache(pools, block_table, idx, dt)
+    if n != nkv:
+        raise ValueError(f"k has {nkv} heads, the pools {n}")
     nh = qs = qos = 0
+    qp = qop = None
     if q is not None:
+        _on(q, "q", idx, dt)
         Mq, nh, qs = _heads(q, "q")
-        q_out = torch.empty(q.shape, dtype=dt, device=dev) if q_out is None else q_out
-        Mo, nho, qos = _heads(q_out, "q_out")
-        if Mq != M or (Mo, nho) != (M, nh):
-            raise ValueError("q and q_out must have one row per token of k")
+        if Mq != M:
+            raise ValueError("q must have one row per token of k")
+        if q_out is None:
+            q_out, qos = q.new_empty(q.shape), nh * _HD
+        else:
+            _on(q_out, "q_out", idx, dt)
+            n, h, qos = _heads(q_out, "q_out")
+            if (n, h) != (M, nh):
+                raise ValueError("q_out must have the shape of q")
+        qp, qop = q.data_ptr(), q_out.data_ptr()
     elif q_out is not None:
         raise ValueError("q_out needs q")
-    rc, rs, rope_len, rotary = _rope_args(rope_cos, rope_sin, dev)
-    with _device_of(dev):
-        check(lib.ps_kv4_append(ptr(q), qs, k.data_ptr(), ks, v.data_ptr(), vs, ptr(q_out), qos,
-                                ctypes.byref(cache), _head_weight(q_weight, "q_weight", dev, dt),
-                                _head_weight(k_weight, "k_weight", dev, dt), float(eps), rc, rs,
-                                rope_len, rotary, 1 if interleaved else 0,
-                                _int32(pos, "pos", M, dev), _home_arg(rows, block_table, M, dev),
-                                _counts_arg(counts), _split(split_point, M), M, nh, code,
-                                ptr(_lib.status_tensor(dev)), _lib.stream_handle(dev)),
-              "ps_kv4_append")
+    rc, rs, rope_len, rotary = _rope_args(rope_cos, rope_sin, idx)
+    split, cnt = _split_counts(split_point, counts, M, idx)
+    _call(lib.ps_kv4_append, "ps_kv4_append", idx, qp, qs, k.data_ptr(), ks, v.data_ptr(), vs, qop,
+          qos, cache, _head_weight(q_weight, "q_weight", idx, dt),
+          _head_weight(k_weight, "k_weight", idx, dt), eps, rc, rs, rope_len, rotary,
+          1 if interleaved else 0, _int32(pos, "pos", M, idx),
+          _home_arg(rows, block_table, M, idx), cnt, split, M, nh, code)
     return q_out
 
 
@@ -636,43 +654,42 @@ def kv4_gather(pools: tuple, seqs: torch.Tensor, cu: torch.Tensor, total: int, *
     position) fills rows ``cu[i]`` to ``cu[i + 1]`` (``cu`` int32 [n + 1] on the
     device). Rows behind the last sequence are left as ``out`` had them.
     """
-    live = [p for p in pools if p is not None and p[0].shape[0]]
-    if not live:
+    p = pools[0] if pools[0] is not None and pools[0][0].shape[0] else pools[1]
+    if p is None:
         raise ValueError("at least one model needs a 4-bit pool")
-    dev, dt = live[0][0].device, live[0][1].dtype
-    if dev.type != "cuda":
-        raise ValueError("parallel-serve ops take CUDA tensors")
-    code = _lib.dtype_code(dt)
-    cache = _kv4_cache(pools, block_table, dev, dt)
-    if seqs.dim() != 2 or seqs.shape[1] != 3:
+    meta = p[1]
+    idx, code = _first(meta)
+    dt = meta.dtype
+    cache, nkv, _ = _kv4_cache(pools, block_table, idx, dt)
+    sh = seqs.shape
+    if len(sh) != 2 or sh[1] != 3:
         raise ValueError("seqs must be int32 [n, 3] (model, slot or block-table row, first position)")
-    n = seqs.shape[0]
+    n = sh[0]
     if total < 0:
         raise ValueError("total must be >= 0")
     if out is None:
-        out = tuple(torch.empty(total, cache.n_kv_heads, _HD, dtype=dt, device=dev)
-                    for _ in range(2))
-    for t in out:
-        _same(dev, dt, out=t)
-        if t.shape != (total, cache.n_kv_heads, _HD) or not t.is_contiguous():
-            raise ValueError("out must be two contiguous [total, n_kv_heads, 128] tensors")
-    with _device_of(dev):
-        check(lib.ps_kv4_gather(ctypes.byref(cache), _int32(seqs, "seqs", 3 * n, dev),
-                                _int32(cu, "cu", n + 1, dev), n, total, out[0].data_ptr(),
-                                out[1].data_ptr(), code, ptr(_lib.status_tensor(dev)),
-                                _lib.stream_handle(dev)), "ps_kv4_gather")
-    return out[0], out[1]
+        k, v = meta.new_empty((total, nkv, _HD)), meta.new_empty((total, nkv, _HD))
+    else:
+        k, v = out
+        for t in out:
+            _on(t, "out", idx, dt)
+            if t.shape != (total, nkv, _HD) or not t.is_contiguous():
+                raise ValueError("out must be two contiguous [total, n_kv_heads, 128] tensors")
+    _call(lib.ps_kv4_gather, "ps_kv4_gather", idx, cache, _int32(seqs, "seqs", 3 * n, idx),
+          _int32(cu, "cu", n + 1, idx), n, total, k.data_ptr(), v.data_ptr(), code)
+    return k, v
 
 
-def _counter_workspace(device: torch.device, nbytes: int, tag: str, counter_bytes: int) -> torch.Tensor:
+def _counter_workspace(like: torch.Tensor, idx: int, nbytes: int, tag: str,
+                       counter_bytes: int) -> torch.Tensor:
     """Workspace whose first ``counter_bytes`` are zero at rest. Under graph capture
     a workspace of the graph's own (two captured graphs may run at the same
     time), else the stream's."""
     if torch.cuda.is_current_stream_capturing():
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        ws = like.new_empty(nbytes, dtype=torch.uint8)
         ws[:counter_bytes].zero_()
         return ws
-    return _lib.workspace(device, nbytes, tag)
+    return _lib.stream_workspace(idx, _raw_stream(idx), nbytes, tag)
 
 
 def kv4_decode_attention(q: torch.Tensor, pools: tuple, pos: torch.Tensor, *, max_len: int,
@@ -686,37 +703,39 @@ def kv4_decode_attention(q: torch.Tensor, pools: tuple, pos: torch.Tensor, *, ma
 
     ``q`` [M, n_heads, 128] (or [M, n_heads * 128]); ``rows``, ``block_table``,
     ``split_point`` and ``counts`` as in ``kv4_append``; ``max_len`` bounds
-    pos[j] + 1. Returns [M, n_heads * 128].
+    pos[j] + 1. ``workspace`` (default: the stream's own) has
+    ps_kv4_decode_attention_workspace_bytes bytes, the first 4096 zero before its
+    first use. Returns [M, n_heads * 128].
     """
+    idx, code = _first(q)
+    dt = q.dtype
     M, nh, qs = _heads(q, "q")
-    dev, dt = q.device, q.dtype
-    code = _lib.dtype_code(dt)
-    _same(dev, None, counts=counts, workspace=workspace)
-    _same(dev, dt, out=out)
-    cache = _kv4_cache(pools, block_table, dev, dt)
-    nkv = cache.n_kv_heads
+    cache, nkv, cap = _kv4_cache(pools, block_table, idx, dt)
     if nh % nkv:
         raise ValueError(f"{nh} query heads do not divide over {nkv} KV heads")
-    cap = cache.L_cap if block_table is None else cache.max_pages * cache.page_size
     if not 0 < max_len <= cap:
         raise ValueError(f"max_len must be in [1, {cap}]")
     if out is None:
-        out = torch.empty(M, nh * _HD, dtype=dt, device=dev)
-    elif out.shape != (M, nh * _HD) or not out.is_contiguous():
-        raise ValueError("out must be contiguous [M, n_heads * 128]")
-    scale = 1.0 / math.sqrt(_HD) if scale is None else scale
-    with _device_of(dev):
-        if workspace is None:
+        out = q.new_empty((M, nh * _HD))
+    else:
+        _on(out, "out", idx, dt)
+        if out.shape != (M, nh * _HD) or not out.is_contiguous():
+            raise ValueError("out must be contiguous [M, n_heads * 128]")
+    split, cnt = _split_counts(split_point, counts, M, idx)
+    pp, home = _int32(pos, "pos", M, idx), _home_arg(rows, block_table, M, idx)
+    if workspace is None:
+        if _current_device() == idx:
             nbytes = lib.ps_kv4_decode_attention_workspace_bytes(M, nh, nkv, max_len)
-            workspace = _counter_workspace(dev, nbytes, "kv4_attn", 4096)
-        check(lib.ps_kv4_decode_attention(q.data_ptr(), qs, ctypes.byref(cache), out.data_ptr(),
-                                          _int32(pos, "pos", M, dev),
-                                          _home_arg(rows, block_table, M, dev),
-                                          _counts_arg(counts), _split(split_point, M), M, nh,
-                                          max_len, float(scale), code, workspace.data_ptr(),
-                                          workspace.numel() * workspace.element_size(),
-                                          ptr(_lib.status_tensor(dev)), _lib.stream_handle(dev)),
-              "ps_kv4_decode_attention")
+        else:
+            with torch.cuda.device(idx):
+                nbytes = lib.ps_kv4_decode_attention_workspace_bytes(M, nh, nkv, max_len)
+        workspace = _counter_workspace(q, idx, nbytes, "kv4_attn", 4096)
+    elif workspace.get_device() != idx or not workspace.is_contiguous():
+        raise ValueError(f"workspace must be a contiguous tensor on cuda:{idx}")
+    _call(lib.ps_kv4_decode_attention, "ps_kv4_decode_attention", idx, q.data_ptr(), qs, cache,
+          out.data_ptr(), pp, home, cnt, split, M, nh, max_len,
+          0.08838834764831845 if scale is None else scale, code, workspace.data_ptr(),
+          workspace.nbytes)
     return out
 
 
@@ -732,12 +751,13 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     no key gets 0. q, k, v may be views of one qkv row. ``cu_q``, ``cu_k`` are int32
     on the device. Returns [tokens, n_heads * 128].
     """
+    idx, code = _first(q)
+    dt = q.dtype
     Tq, nh, qs = _heads(q, "q")
     Tk, nkv, ks = _heads(k, "k")
     Tv, nv, vs = _heads(v, "v")
-    dev, dt = q.device, q.dtype
-    code = _lib.dtype_code(dt)
-    _same(dev, dt, k=k, v=v, out=out)
+    _on(k, "k", idx, dt)
+    _on(v, "v", idx, dt)
     if (Tv, nv) != (Tk, nkv):
         raise ValueError("k and v must have the same shape")
     if nh % nkv:
@@ -751,18 +771,18 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
         cu_k = cu_q
     elif cu_k.numel() != n + 1:
         raise ValueError("cu_q and cu_k must have the same length")
-    scale = 1.0 / math.sqrt(_HD) if scale is None else float(scale)
-    if not 0.0 < scale < 3e38:
+    if scale is None:
+        scale = 0.08838834764831845
+    elif not 0.0 < scale < 3e38:
         raise ValueError("scale must be positive and finite")
     if out is None:
-        out = torch.empty(Tq, nh * _HD, dtype=dt, device=dev)
-    To, no, os_ = _heads(out, "out")
-    if (To, no) != (Tq, nh):
-        raise ValueError("out must have a row of n_heads * 128 per query")
-    with _device_of(dev):
-        check(lib.ps_prompt_attention(q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs,
-                                      out.data_ptr(), os_, _int32(cu_q, "cu_q", 1, dev),
-                                      _int32(cu_k, "cu_k", 1, dev), n, Tq, Tk, nh, nkv, scale,
-                                      code, ptr(_lib.status_tensor(dev)), _lib.stream_handle(dev)),
-              "ps_prompt_attention")
+        out, os_ = q.new_empty((Tq, nh * _HD)), nh * _HD
+    else:
+        _on(out, "out", idx, dt)
+        To, no, os_ = _heads(out, "out")
+        if (To, no) != (Tq, nh):
+            raise ValueError("out must have a row of n_heads * 128 per query")
+    _call(lib.ps_prompt_attention, "ps_prompt_attention", idx, q.data_ptr(), qs, k.data_ptr(), ks,
+          v.data_ptr(), vs, out.data_ptr(), os_, _int32(cu_q, "cu_q", 1, idx),
+          _int32(cu_k, "cu_k", 1, idx), n, Tq, Tk, nh, nkv, scale, code)
     return out
