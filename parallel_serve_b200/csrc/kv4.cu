@@ -43,7 +43,7 @@ struct RowArgs {
   Pool pool[2];
   int32_t* status;
   int M, n_heads, n_kv, split_point, rotary, interleaved, rope_len;
-  int L_cap, page_size, max_pages, table_rows;  // append
+  int L_cap, page_size, page_shift, max_pages, table_rows;  // append
   float eps;
 };
 
@@ -66,42 +66,72 @@ PS_DEV Vec8 pack8(const float* f) {
 
 // Quantise this lane's 8 channels with the 3 other lanes of its group and store
 // its word of codes (and the group's (s, z), by its first lane).
+//
+// The quotient is a product with 1 / s, whose error (below 4e-6 for quotients up
+// to 16) can only matter next to a half-integer; there, the sign of the exact
+// remainder x - z - (c + 1/2) s decides. With 16-bit inputs exact halves are
+// common (2 in 1000), so that is looked at for every lane, but a division for each
+// channel took most of this kernel's time. Rounding and packing go through the low
+// mantissa bits of 1.5 * 2^23 + quotient, which a conversion to integer would take
+// four times as long for.
 template <typename T>
 PS_DEV void store_row4(const float* x, int lane, unsigned mask, uint8_t* codes, uint8_t* meta) {
-  float lo = x[0], hi = x[0];
-  bool fin = isfinite(x[0]);
+  float lo = x[0], hi = x[0], zero = 0.f;  // zero: NaN when an x is not finite
 #pragma unroll
-  for (int i = 1; i < 8; ++i) {
+  for (int i = 0; i < 8; ++i) {
     lo = fminf(lo, x[i]);
     hi = fmaxf(hi, x[i]);
-    fin = fin && isfinite(x[i]);
+    zero = fmaf(x[i], 0.f, zero);
   }
-  float bad = fin ? 0.f : 1.f;
 #pragma unroll
   for (int o = 1; o <= 2; o <<= 1) {
     lo = fminf(lo, __shfl_xor_sync(mask, lo, o));
     hi = fmaxf(hi, __shfl_xor_sync(mask, hi, o));
-    bad = fmaxf(bad, __shfl_xor_sync(mask, bad, o));
   }
+  const int g = lane >> 2, w = lane & 3;
+  const unsigned nonfinite = __ballot_sync(mask, zero != zero);
+  const bool bad = (nonfinite >> ((threadIdx.x & 16) + 4 * g)) & 15u;
   T zt = saturate<T>(lo);
   const float z = to_f32<T>(zt);
   float range = __fdiv_rn(__fsub_rn(hi, z), 15.f);
   if (isinf(range)) range = hi / 15.f - z / 15.f;  // max - min beyond fp32
   T st = saturate<T>(range);
   float s = to_f32<T>(st);
+  if (s == 0.f) s = 1.f;  // a constant group: every code 0
+  const float r = __frcp_rn(s);
+  const float kMagic = 12582912.f;
+  float near_half = 0.f;
   uint32_t word = 0;
-  if (bad != 0.f) {
-    st = from_f32<T>(0.f);
-    zt = from_f32<T>(__uint_as_float(0x7fc00000u));
-  } else {
-    if (s == 0.f) s = 1.f;  // a constant group: every code 0
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float c = rintf(__fdiv_rn(__fsub_rn(x[i], z), s));
-      word |= (uint32_t)fminf(fmaxf(c, 0.f), 15.f) << (4 * i);
+  for (int i = 7; i >= 0; --i) {
+    const float y = fminf(fmaxf(__fsub_rn(x[i], z) * r, 0.f), 15.f);
+    const float f = __fadd_rn(y, kMagic);
+    near_half = fmaxf(near_half, fabsf(y - (f - kMagic)));
+    word = word * 16u + __float_as_uint(f);  // the magic's bits are taken out below
+  }
+  word -= 0x3f400000u;  // 0x4b400000 (1 + 16 + 256 + ...) in 32 bits
+  const bool tiny = s < 1.1754944e-38f;  // subnormal: 1 / s may not exist
+  if ((near_half > 0.499996f || tiny) && !bad) {
+    word = 0;
+#pragma unroll
+    for (int i = 7; i >= 0; --i) {
+      const float d = __fsub_rn(x[i], z);
+      const float y = fminf(fmaxf(tiny ? __fdiv_rn(d, s) : d * r, 0.f), 15.f);
+      float c = floorf(y);
+      if (y - c > 0.25f && y - c < 0.75f) {  // between c and c + 1
+        const float rest = fmaf(-(c + 0.5f), s, d);  // exact next to the half
+        if (rest > 0.f || (rest == 0.f && ((int)c & 1))) c += 1.f;
+      } else {
+        c = rintf(y);
+      }
+      word = word * 16u + (uint32_t)c;
     }
   }
-  const int g = lane >> 2, w = lane & 3;
+  if (bad) {
+    word = 0;
+    st = from_f32<T>(0.f);
+    zt = from_f32<T>(__uint_as_float(0x7fc00000u));
+  }
   reinterpret_cast<uint32_t*>(codes)[4 * w + g] = word;
   if (w == 0) {
     T pair[2] = {st, zt};
@@ -133,9 +163,10 @@ __global__ void __launch_bounds__(kThreads) norm_rope_kernel(const RowArgs a) {
     int at = p, row = home;
     if (a.block_table) {
       cache_len = a.page_size;
-      ok = ok && home < a.table_rows && p / a.page_size < a.max_pages;
-      row = ok ? a.block_table[(size_t)home * a.max_pages + p / a.page_size] : -1;
-      at = p % a.page_size;
+      const int page = p >> a.page_shift;
+      ok = ok && home < a.table_rows && page < a.max_pages;
+      row = ok ? a.block_table[(size_t)home * a.max_pages + page] : -1;
+      at = p & (cache_len - 1);
     } else {
       cache_len = a.L_cap;
       ok = ok && p < a.L_cap;
@@ -148,19 +179,19 @@ __global__ void __launch_bounds__(kThreads) norm_rope_kernel(const RowArgs a) {
     return;
   }
   const int r0 = blockIdx.y * (kHalfWarps * kRows) + hw;
-  Vec8 in[kRows];
-#pragma unroll
-  for (int u = 0; u < kRows; ++u) {
-    const int r = r0 + u * kHalfWarps;
-    const T* src = nullptr;
-    if (r < nq)
-      src = (const T*)a.q + (size_t)j * a.q_stride + r * kD;
-    else if (r < nq + a.n_kv)
-      src = (const T*)a.k + (size_t)j * a.k_stride + (r - nq) * kD;
-    else if (kAppend && r < total)
-      src = (const T*)a.v + (size_t)j * a.v_stride + (r - nq - a.n_kv) * kD;
-    if (src) in[u] = reinterpret_cast<const Vec8*>(src)[lane];
-  }
+  const T* qj = (const T*)a.q + (size_t)j * a.q_stride;
+  const T* kj = (const T*)a.k + (size_t)j * a.k_stride;
+  const T* vj = kAppend ? (const T*)a.v + (size_t)j * a.v_stride : nullptr;
+  auto load = [&](int r) {  // this lane's 16 bytes of row r (zeros behind the last)
+    Vec8 x = {{0u, 0u, 0u, 0u}};
+    if (r < total) {
+      const T* src = r < nq ? qj + r * kD
+                            : (r < nq + a.n_kv ? kj + (r - nq) * kD : vj + (r - nq - a.n_kv) * kD);
+      x = reinterpret_cast<const Vec8*>(src)[lane];
+    }
+    return x;
+  };
+  Vec8 next = load(r0);
   // cos / sin of this lane's channels: half layout channel i < rotary/2 pairs
   // with i + rotary/2; interleaved pairs are (2i, 2i + 1)
   const int half = a.rotary >> 1;
@@ -184,13 +215,15 @@ __global__ void __launch_bounds__(kThreads) norm_rope_kernel(const RowArgs a) {
   const bool upper = 8 * lane >= half;  // the second element of its half-layout pairs
   const int partner = turned ? (upper ? lane - half / 8 : lane + half / 8) : lane;
 
-#pragma unroll
+#pragma unroll 1
   for (int u = 0; u < kRows; ++u) {
     const int r = r0 + u * kHalfWarps;
     if (r >= total) break;  // the same for the whole half warp
+    const Vec8 in = next;
+    if (u + 1 < kRows) next = load(r + kHalfWarps);  // one row ahead
     const bool is_q = r < nq, is_v = r >= nq + a.n_kv;
     float x[8];
-    unpack8<T>(in[u], x);
+    unpack8<T>(in, x);
     const T* w = (const T*)(is_q ? a.q_w : a.k_w);
     if (!is_v && w) {
       float ss = 0.f;
@@ -251,20 +284,44 @@ struct GatherArgs {
   void* k_out;  // [total, n_kv, 128]
   void* v_out;
   int32_t* status;
-  int n, total, n_kv, L_cap, page_size, max_pages, table_rows;
+  int n, total, n_kv, L_cap, page_size, page_shift, max_pages, table_rows;
 };
 
 template <typename T>
+struct Pair;
+template <>
+struct Pair<__half> {
+  using type = __half2;
+  static constexpr uint32_t kBias = 0x64006400u;  // 1024 twice: low mantissa bits are units
+};
+template <>
+struct Pair<__nv_bfloat16> {
+  using type = __nv_bfloat162;
+  static constexpr uint32_t kBias = 0x43004300u;  // 128
+};
+
+// The 8 values of a word of codes, two at a time in packed 16-bit arithmetic: a
+// nibble placed in the low mantissa bits of a bias is bias + c exactly, and one
+// fused s * c + z rounds once.
+template <typename T>
 PS_DEV Vec8 values8(uint32_t word, uint32_t meta) {
-  float s, z, f[8];
-  unpack2<T>(meta, s, z);
+  using T2 = typename Pair<T>::type;
+  const uint32_t bias = Pair<T>::kBias, sb = __byte_perm(meta, 0, 0x1010),
+                 zb = __byte_perm(meta, 0, 0x3232);
+  const T2 s = *reinterpret_cast<const T2*>(&sb), z = *reinterpret_cast<const T2*>(&zb);
+  const T2 b = *reinterpret_cast<const T2*>(&bias);
+  T top[2] = {from_f32<T>(max_finite<T>()), from_f32<T>(max_finite<T>())};
+  Vec8 out;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t t = word >> (8 * i);
+    const uint32_t n = (t & 0xfu) | ((t << 12) & 0xf0000u) | bias;  // low nibble, high nibble
     // 15 s + z may lie half a step of (s, z) above T's largest value; NaN stays
-    const float v = s * (float)((word >> (4 * i)) & 15) + z;
-    f[i] = z == z ? fminf(v, max_finite<T>()) : z;
+    const T2 v = __hmin2_nan(__hfma2(s, __hsub2(*reinterpret_cast<const T2*>(&n), b), z),
+                             *reinterpret_cast<const T2*>(top));
+    out.u[i] = *reinterpret_cast<const uint32_t*>(&v);
   }
-  return pack8<T>(f);
+  return out;
 }
 
 template <typename T>
@@ -280,25 +337,37 @@ __global__ void __launch_bounds__(kThreads) kv4_gather_kernel(const GatherArgs a
     const int mid = (lo + hi + 1) >> 1;
     if (a.cu[mid] <= base) lo = mid; else hi = mid - 1;
   }
-  int i = lo;
+  const int g = lane >> 2, w = lane & 3;
+  // of the current sequence: its rows [begin, end), home, first position, model
+  int i = lo - 1, begin = 0, end = base, home = 0, first = 0, m = 0;
+  bool known = false;
   uint32_t kw[kRows], vw[kRows], km[kRows], vm[kRows];
-  bool live[kRows];
+  unsigned live = 0;
 #pragma unroll
   for (int u = 0; u < kRows; ++u) {
     const int r = base + u * kHalfWarps;
-    live[u] = false;
-    if (r >= a.total) continue;
-    while (i < a.n && a.cu[i + 1] <= r) ++i;
-    if (i >= a.n || r < a.cu[i]) continue;  // rows behind the last sequence stay as they are
-    const int m = a.seqs[3 * i], home = a.seqs[3 * i + 1];
-    const long long p = (long long)a.seqs[3 * i + 2] + r - a.cu[i];
-    bool ok = (m == 0 || m == 1) && home >= 0 && a.seqs[3 * i + 2] >= 0;
+    while (end <= r && i + 1 < a.n) {
+      ++i;
+      begin = a.cu[i];
+      end = a.cu[i + 1];
+      known = false;
+    }
+    if (r >= a.total || i < 0 || r < begin || r >= end) continue;  // no sequence's row
+    if (!known) {
+      m = a.seqs[3 * i];
+      home = a.seqs[3 * i + 1];
+      first = a.seqs[3 * i + 2];
+      known = true;
+    }
+    const long long p = (long long)first + r - begin;
+    bool ok = (m == 0 || m == 1) && home >= 0 && first >= 0;
     int row = home, len = a.L_cap, at = (int)p;
     if (a.block_table) {
       len = a.page_size;
-      ok = ok && home < a.table_rows && p / a.page_size < a.max_pages;
-      row = ok ? a.block_table[(size_t)home * a.max_pages + p / a.page_size] : -1;
-      at = (int)(p % a.page_size);
+      const long long page = p >> a.page_shift;
+      ok = ok && home < a.table_rows && page < a.max_pages;
+      row = ok ? a.block_table[(size_t)home * a.max_pages + page] : -1;
+      at = (int)p & (len - 1);
     } else {
       ok = ok && p < a.L_cap;
     }
@@ -308,9 +377,8 @@ __global__ void __launch_bounds__(kThreads) kv4_gather_kernel(const GatherArgs a
       if (lane == 0 && h == 0) set_status(a.status, PS_ERR_BAD_INDEX);
       continue;
     }
-    live[u] = true;
+    live |= 1u << u;
     const size_t src = ((size_t)row * a.n_kv + h) * len + at;
-    const int g = lane >> 2, w = lane & 3;
     kw[u] = reinterpret_cast<const uint32_t*>(pool.k_codes + src * kCodeBytes)[4 * w + g];
     vw[u] = reinterpret_cast<const uint32_t*>(pool.v_codes + src * kCodeBytes)[4 * w + g];
     km[u] = reinterpret_cast<const uint32_t*>(pool.k_meta + src * kMetaBytes)[g];
@@ -318,7 +386,7 @@ __global__ void __launch_bounds__(kThreads) kv4_gather_kernel(const GatherArgs a
   }
 #pragma unroll
   for (int u = 0; u < kRows; ++u) {
-    if (!live[u]) continue;
+    if (!(live >> u & 1)) continue;
     const size_t dst = ((size_t)(base + u * kHalfWarps) * a.n_kv + h) * kD;
     reinterpret_cast<Vec8*>((T*)a.k_out + dst)[lane] = values8<T>(kw[u], km[u]);
     reinterpret_cast<Vec8*>((T*)a.v_out + dst)[lane] = values8<T>(vw[u], vm[u]);
@@ -463,6 +531,7 @@ extern "C" int ps_kv4_append(const void* q, long long q_stride, const void* k, l
   a.pool[1] = kv4::to_pool(&cache->pool[1]);
   a.L_cap = cache->L_cap;
   a.page_size = cache->page_size;
+  while (cache->block_table && (1 << a.page_shift) < cache->page_size) ++a.page_shift;
   a.max_pages = cache->max_pages;
   a.table_rows = cache->table_rows;
   return kv4::launch_rows<true>(a, dtype, (cudaStream_t)stream);
@@ -490,6 +559,7 @@ extern "C" int ps_kv4_gather(const ps_kv4_cache_t* cache, const int32_t* seqs, c
   a.n_kv = cache->n_kv_heads;
   a.L_cap = cache->L_cap;
   a.page_size = cache->page_size;
+  while (cache->block_table && (1 << a.page_shift) < cache->page_size) ++a.page_shift;
   a.max_pages = cache->max_pages;
   a.table_rows = cache->table_rows;
   const dim3 grid(cdiv(total, kv4::kHalfWarps * kv4::kRows), cache->n_kv_heads);
