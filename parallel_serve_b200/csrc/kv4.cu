@@ -23,7 +23,7 @@ namespace kv4 {
 
 constexpr int kThreads = 128;
 constexpr int kHalfWarps = kThreads / 16;
-constexpr int kRows = 4;  // rows of one half warp
+constexpr int kRows = 4;  // rows of one half warp in the read-back
 
 struct RowArgs {
   const void* q;  // [M, n_heads, 128], token stride q_stride (elements); nullable
@@ -43,6 +43,7 @@ struct RowArgs {
   Pool pool[2];
   int32_t* status;
   int M, n_heads, n_kv, split_point, rotary, interleaved, rope_len;
+  int rows_per;  // rows of one half warp
   int L_cap, page_size, page_shift, max_pages, table_rows;  // append
   float eps;
 };
@@ -67,15 +68,15 @@ PS_DEV Vec8 pack8(const float* f) {
 // Quantise this lane's 8 channels with the 3 other lanes of its group and store
 // its word of codes (and the group's (s, z), by its first lane).
 //
-// The quotient is a product with 1 / s, whose error (below 4e-6 for quotients up
-// to 16) can only matter next to a half-integer; there, the sign of the exact
-// remainder x - z - (c + 1/2) s decides. With 16-bit inputs exact halves are
-// common (2 in 1000), so that is looked at for every lane, but a division for each
-// channel took most of this kernel's time. Rounding and packing go through the low
-// mantissa bits of 1.5 * 2^23 + quotient, which a conversion to integer would take
-// four times as long for.
+// The quotient d / s is y = d r with r = 1 / s, corrected once by its own remainder,
+// y + (d - s y) r (Markstein's step): where d / s is a half-integer, which with
+// 16-bit inputs happens 2 times in 1000, the result is that half exactly and the
+// rounding to even is the one that a division would give. (A division for each
+// channel took most of this kernel's time.) Rounding and packing go through the
+// low mantissa bits of 1.5 * 2^23 + quotient; a conversion to integer takes four
+// times as long.
 template <typename T>
-PS_DEV void store_row4(const float* x, int lane, unsigned mask, uint8_t* codes, uint8_t* meta) {
+PS_DEV void store_row4(const float (&x)[8], int lane, unsigned mask, uint8_t* codes, uint8_t* meta) {
   float lo = x[0], hi = x[0], zero = 0.f;  // zero: NaN when an x is not finite
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -93,39 +94,36 @@ PS_DEV void store_row4(const float* x, int lane, unsigned mask, uint8_t* codes, 
   const bool bad = (nonfinite >> ((threadIdx.x & 16) + 4 * g)) & 15u;
   T zt = saturate<T>(lo);
   const float z = to_f32<T>(zt);
-  float range = __fdiv_rn(__fsub_rn(hi, z), 15.f);
-  if (isinf(range)) range = hi / 15.f - z / 15.f;  // max - min beyond fp32
+  const float span = __fsub_rn(hi, z);
+  float range = span * (1.f / 15.f);
+  range = fmaf(fmaf(-15.f, range, span), 1.f / 15.f, range);
+  if (isinf(span)) range = hi / 15.f - z / 15.f;  // max - min beyond fp32
   T st = saturate<T>(range);
   float s = to_f32<T>(st);
   if (s == 0.f) s = 1.f;  // a constant group: every code 0
-  const float r = __frcp_rn(s);
-  const float kMagic = 12582912.f;
-  float near_half = 0.f;
   uint32_t word = 0;
-#pragma unroll
-  for (int i = 7; i >= 0; --i) {
-    const float y = fminf(fmaxf(__fsub_rn(x[i], z) * r, 0.f), 15.f);
-    const float f = __fadd_rn(y, kMagic);
-    near_half = fmaxf(near_half, fabsf(y - (f - kMagic)));
-    word = word * 16u + __float_as_uint(f);  // the magic's bits are taken out below
-  }
-  word -= 0x3f400000u;  // 0x4b400000 (1 + 16 + 256 + ...) in 32 bits
-  const bool tiny = s < 1.1754944e-38f;  // subnormal: 1 / s may not exist
-  if ((near_half > 0.499996f || tiny) && !bad) {
-    word = 0;
+  if (s < 1.1754944e-38f || isinf(span)) {
+    // 1 / s or a difference may not exist in fp32: divide
 #pragma unroll
     for (int i = 7; i >= 0; --i) {
-      const float d = __fsub_rn(x[i], z);
-      const float y = fminf(fmaxf(tiny ? __fdiv_rn(d, s) : d * r, 0.f), 15.f);
-      float c = floorf(y);
-      if (y - c > 0.25f && y - c < 0.75f) {  // between c and c + 1
-        const float rest = fmaf(-(c + 0.5f), s, d);  // exact next to the half
-        if (rest > 0.f || (rest == 0.f && ((int)c & 1))) c += 1.f;
-      } else {
-        c = rintf(y);
-      }
-      word = word * 16u + (uint32_t)c;
+      const float y = __fdiv_rn(__fsub_rn(x[i], z), s);
+      word = word * 16u + (uint32_t)rintf(fminf(fmaxf(y, 0.f), 15.f));
     }
+  } else {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
+    const uint64_t zz = f32x2(-z, -z), rr = f32x2(r, r), ss = f32x2(-s, -s);
+#pragma unroll
+    for (int i = 6; i >= 0; i -= 2) {
+      const uint64_t d = f32x2_add(f32x2(x[i], x[i + 1]), zz);
+      const uint64_t y0 = f32x2_mul(d, rr);
+      float lo_y, hi_y;
+      f32x2_split(f32x2_fma(f32x2_fma(ss, y0, d), rr, y0), lo_y, hi_y);
+      hi_y = __fadd_rn(fminf(fmaxf(hi_y, 0.f), 15.f), 12582912.f);
+      lo_y = __fadd_rn(fminf(fmaxf(lo_y, 0.f), 15.f), 12582912.f);
+      word = (word * 16u + __float_as_uint(hi_y)) * 16u + __float_as_uint(lo_y);
+    }
+    word -= 0x3f400000u;  // 0x4b400000 (1 + 16 + 256 + ...) in 32 bits
   }
   if (bad) {
     word = 0;
@@ -139,10 +137,10 @@ PS_DEV void store_row4(const float* x, int lane, unsigned mask, uint8_t* codes, 
   }
 }
 
-// grid (M, ceil(rows per token / (kHalfWarps * kRows))). Rows of a token: its q
+// grid (M, ceil(rows per token / (kHalfWarps * rows_per))). Rows of a token: its q
 // heads, its k heads, then (append) its v heads.
 template <typename T, bool kAppend>
-__global__ void __launch_bounds__(kThreads) norm_rope_kernel(const RowArgs a) {
+__global__ void __launch_bounds__(kThreads, 8) norm_rope_kernel(const RowArgs a) {
   pdl_wait();
   pdl_launch_dependents();
   const int j = blockIdx.x;
@@ -178,7 +176,7 @@ __global__ void __launch_bounds__(kThreads) norm_rope_kernel(const RowArgs a) {
     if (threadIdx.x == 0 && blockIdx.y == 0) set_status(a.status, PS_ERR_BAD_INDEX);
     return;
   }
-  const int r0 = blockIdx.y * (kHalfWarps * kRows) + hw;
+  const int r0 = blockIdx.y * (kHalfWarps * a.rows_per) + hw;
   const T* qj = (const T*)a.q + (size_t)j * a.q_stride;
   const T* kj = (const T*)a.k + (size_t)j * a.k_stride;
   const T* vj = kAppend ? (const T*)a.v + (size_t)j * a.v_stride : nullptr;
@@ -191,13 +189,13 @@ __global__ void __launch_bounds__(kThreads) norm_rope_kernel(const RowArgs a) {
     }
     return x;
   };
-  Vec8 next = load(r0);
+  Vec8 next = load(r0), after = load(r0 + kHalfWarps);  // two rows ahead
   // cos / sin of this lane's channels: half layout channel i < rotary/2 pairs
   // with i + rotary/2; interleaved pairs are (2i, 2i + 1)
   const int half = a.rotary >> 1;
   const bool turned = a.rc && 8 * lane < a.rotary;
   const int pair0 = a.interleaved ? 4 * lane : (8 * lane < half ? 8 * lane : 8 * lane - half);
-  float co[8], si[8];
+  float co[8] = {}, si[8] = {};
   if (turned) {
     const float* rc = a.rc + (size_t)p * half + pair0;
     const float* rs = a.rs + (size_t)p * half + pair0;
@@ -214,13 +212,18 @@ __global__ void __launch_bounds__(kThreads) norm_rope_kernel(const RowArgs a) {
   }
   const bool upper = 8 * lane >= half;  // the second element of its half-layout pairs
   const int partner = turned ? (upper ? lane - half / 8 : lane + half / 8) : lane;
+  if (!a.interleaved && !upper) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) si[i] = -si[i];
+  }
 
 #pragma unroll 1
-  for (int u = 0; u < kRows; ++u) {
+  for (int u = 0; u < a.rows_per; ++u) {
     const int r = r0 + u * kHalfWarps;
     if (r >= total) break;  // the same for the whole half warp
     const Vec8 in = next;
-    if (u + 1 < kRows) next = load(r + kHalfWarps);  // one row ahead
+    next = after;
+    if (u + 2 < a.rows_per) after = load(r + 2 * kHalfWarps);
     const bool is_q = r < nq, is_v = r >= nq + a.n_kv;
     float x[8];
     unpack8<T>(in, x);
@@ -249,12 +252,13 @@ __global__ void __launch_bounds__(kThreads) norm_rope_kernel(const RowArgs a) {
         }
       } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float y = __shfl_sync(mask, x[i], partner, 16);
-          if (turned) {
-            const float b = __fmul_rn(y, si[i]);
-            x[i] = upper ? __fadd_rn(__fmul_rn(x[i], co[i]), b) : __fsub_rn(__fmul_rn(x[i], co[i]), b);
-          }
+        for (int i = 0; i < 8; i += 2) {
+          const float y0 = __shfl_sync(mask, x[i], partner, 16);
+          const float y1 = __shfl_sync(mask, x[i + 1], partner, 16);
+          if (turned)  // si is - sin in the first elements of the pairs
+            f32x2_split(f32x2_add(f32x2_mul(f32x2(x[i], x[i + 1]), f32x2(co[i], co[i + 1])),
+                                  f32x2_mul(f32x2(y0, y1), f32x2(si[i], si[i + 1]))),
+                        x[i], x[i + 1]);
         }
       }
     }
@@ -275,7 +279,7 @@ __global__ void __launch_bounds__(kThreads) norm_rope_kernel(const RowArgs a) {
 
 // Read-back: output row r of sequence i (cu[i] <= r < cu[i+1]) is position
 // seqs[i].first + (r - cu[i]). grid (ceil(total / 32), n_kv), 8 half warps with
-// 4 rows each.
+// 4 rows each, whose loads are all issued before the first is used.
 struct GatherArgs {
   Pool pool[2];
   const int32_t* seqs;  // [n][3]: model, slot or block-table row, first position
@@ -338,14 +342,17 @@ __global__ void __launch_bounds__(kThreads) kv4_gather_kernel(const GatherArgs a
     if (a.cu[mid] <= base) lo = mid; else hi = mid - 1;
   }
   const int g = lane >> 2, w = lane & 3;
-  // of the current sequence: its rows [begin, end), home, first position, model
-  int i = lo - 1, begin = 0, end = base, home = 0, first = 0, m = 0;
-  bool known = false;
+  // of the current sequence: its rows [begin, end), home, first position, pool
+  int i = lo - 1, begin = 0, end = base, home = 0, first = 0;
+  bool known = false, good = false;
+  Pool pool{};
+  size_t src = 0;  // cache row of this lane's row (contiguous: moves with it)
   uint32_t kw[kRows], vw[kRows], km[kRows], vm[kRows];
   unsigned live = 0;
 #pragma unroll
   for (int u = 0; u < kRows; ++u) {
     const int r = base + u * kHalfWarps;
+    src += kHalfWarps;
     while (end <= r && i + 1 < a.n) {
       ++i;
       begin = a.cu[i];
@@ -354,31 +361,32 @@ __global__ void __launch_bounds__(kThreads) kv4_gather_kernel(const GatherArgs a
     }
     if (r >= a.total || i < 0 || r < begin || r >= end) continue;  // no sequence's row
     if (!known) {
-      m = a.seqs[3 * i];
+      const int m = a.seqs[3 * i];
       home = a.seqs[3 * i + 1];
       first = a.seqs[3 * i + 2];
+      pool = m == 1 ? a.pool[1] : a.pool[0];
+      good = (m == 0 || m == 1) && home >= 0 && first >= 0 &&
+             home < (a.block_table ? a.table_rows : pool.rows);
+      if (!a.block_table)
+        src = ((size_t)home * a.n_kv + h) * a.L_cap + (size_t)((long long)first + r - begin);
       known = true;
     }
     const long long p = (long long)first + r - begin;
-    bool ok = (m == 0 || m == 1) && home >= 0 && first >= 0;
-    int row = home, len = a.L_cap, at = (int)p;
+    bool ok = good;
     if (a.block_table) {
-      len = a.page_size;
       const long long page = p >> a.page_shift;
-      ok = ok && home < a.table_rows && page < a.max_pages;
-      row = ok ? a.block_table[(size_t)home * a.max_pages + page] : -1;
-      at = (int)p & (len - 1);
+      ok = ok && page < a.max_pages;
+      const int row = ok ? a.block_table[(size_t)home * a.max_pages + page] : -1;
+      ok = ok && row >= 0 && row < pool.rows;
+      src = ((size_t)row * a.n_kv + h) * a.page_size + ((int)p & (a.page_size - 1));
     } else {
       ok = ok && p < a.L_cap;
     }
-    const Pool pool = m == 1 ? a.pool[1] : a.pool[0];
-    ok = ok && row >= 0 && row < pool.rows;
     if (!ok) {
       if (lane == 0 && h == 0) set_status(a.status, PS_ERR_BAD_INDEX);
       continue;
     }
     live |= 1u << u;
-    const size_t src = ((size_t)row * a.n_kv + h) * len + at;
     kw[u] = reinterpret_cast<const uint32_t*>(pool.k_codes + src * kCodeBytes)[4 * w + g];
     vw[u] = reinterpret_cast<const uint32_t*>(pool.v_codes + src * kCodeBytes)[4 * w + g];
     km[u] = reinterpret_cast<const uint32_t*>(pool.k_meta + src * kMetaBytes)[g];
@@ -425,10 +433,20 @@ bool valid_cache(const ps_kv4_cache_t* c) {
   return c->L_cap > 0 && c->L_cap <= (1 << 30);
 }
 
+// Rows of a half warp: what a token's rows come to in as few blocks as hold at
+// most 6 each (its setup, a table row of cos and sin among it, is shared by them);
+// fewer when the tokens alone do not fill the GPU.
+static int rows_per_half_warp(int M, int total, int device) {
+  const int most = M >= 4 * sm_count(device) ? 6 : 2;
+  const int blocks = cdiv(total, kHalfWarps * most);
+  return cdiv(total, kHalfWarps * blocks);
+}
+
 template <bool kAppend>
-static int launch_rows(const RowArgs& a, int dtype, cudaStream_t st) {
+static int launch_rows(RowArgs& a, int dtype, cudaStream_t st) {
   const int total = (a.q ? a.n_heads : 0) + (kAppend ? 2 : 1) * a.n_kv;
-  const dim3 grid(a.M, cdiv(total, kHalfWarps * kRows));
+  a.rows_per = rows_per_half_warp(a.M, total, current_device());
+  const dim3 grid(a.M, cdiv(total, kHalfWarps * a.rows_per));
   if (dtype == PS_DTYPE_BF16)
     PS_CUDA_RET(launch(norm_rope_kernel<__nv_bfloat16, kAppend>, grid, dim3(kThreads), 0, st, a));
   else

@@ -194,26 +194,6 @@ PS_DEV uint32_t pack16<__nv_bfloat16>(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Two fp32 lanes of one 64-bit register (one issue slot for both).
-PS_DEV uint64_t pair(float lo, float hi) {
-  uint64_t d;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
-  return d;
-}
-PS_DEV void unpair(uint64_t d, float& lo, float& hi) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(d));
-}
-PS_DEV uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-PS_DEV uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-
 // The row's largest score of kCols columns (raw, before the scale).
 template <int kCols>
 PS_DEV float row_max(uint32_t s_addr, bool masked, int lim) {
@@ -237,8 +217,8 @@ PS_DEV float row_max(uint32_t s_addr, bool masked, int lim) {
 template <typename T>
 PS_DEV float softmax_half(uint32_t s_addr, bool masked, int lim, float scale, float neg,
                           uint32_t* p) {
-  const uint64_t scale2 = pair(scale, scale), neg2 = pair(neg, neg);
-  uint64_t l0 = pair(0.f, 0.f), l1 = l0;
+  const uint64_t scale2 = f32x2(scale, scale), neg2 = f32x2(neg, neg);
+  uint64_t l0 = f32x2(0.f, 0.f), l1 = l0;
   uint32_t s[2][32];
   ld32(s_addr, s[0]);
 #pragma unroll
@@ -255,21 +235,21 @@ PS_DEV float softmax_half(uint32_t s_addr, bool masked, int lim, float scale, fl
 #pragma unroll
     for (int i = 0; i < 32; i += 4) {
       float x0, x1, y0, y1;
-      unpair(fma2(pair(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), scale2, neg2), x0, x1);
-      unpair(fma2(pair(__uint_as_float(v[i + 2]), __uint_as_float(v[i + 3])), scale2, neg2), y0,
+      f32x2_split(f32x2_fma(f32x2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), scale2, neg2), x0, x1);
+      f32x2_split(f32x2_fma(f32x2(__uint_as_float(v[i + 2]), __uint_as_float(v[i + 3])), scale2, neg2), y0,
              y1);
       x0 = exp2_ftz(x0);
       x1 = exp2_ftz(x1);
       y0 = exp2_ftz(y0);
       y1 = exp2_ftz(y1);
-      l0 = add2(l0, pair(x0, x1));
-      l1 = add2(l1, pair(y0, y1));
+      l0 = f32x2_add(l0, f32x2(x0, x1));
+      l1 = f32x2_add(l1, f32x2(y0, y1));
       p[16 * c + i / 2] = pack16<T>(x0, x1);
       p[16 * c + i / 2 + 1] = pack16<T>(y0, y1);
     }
   }
   float s0, s1;
-  unpair(add2(l0, l1), s0, s1);
+  f32x2_split(f32x2_add(l0, l1), s0, s1);
   return s0 + s1;
 }
 
