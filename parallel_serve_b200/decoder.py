@@ -42,6 +42,7 @@ import torch
 
 from . import _lib, ops
 from ._lib import check, lib, ptr
+from .kv4 import KV4Pool
 
 
 @dataclass
@@ -179,6 +180,12 @@ class TwoModelDecoder:
     a workload whose KV caches exceed the GPU's memory (Llama-13B shapes at
     256 sequences per model and 4096 positions) be timed, and its outputs are
     not those of the model.
+
+    ``kv_bits=4`` holds the KV cache in 4 bits (``kv4.KV4Pool``, contiguous or paged):
+    160 bytes per position and head instead of 512. The QKV projection then
+    writes a plain qkv row, ``ops.kv4_append`` rotates and quantises it, and
+    attention reads the quantised history, in the prefill too (read back and
+    packed per chunk), so chunk boundaries do not change the result.
     """
 
     def __init__(self, cfg: DecoderConfig, model_id, L_cap: int, *, device="cuda",
@@ -186,7 +193,7 @@ class TwoModelDecoder:
                  allreduce: str = "nvlink", fused_epilogues: bool = True,
                  page_size: int | None = None, prefill_chunk: int = 256,
                  kv_layers: int | None = None, chain: bool = False, packed: bool = True,
-                 auto_grid: bool = True):
+                 auto_grid: bool = True, kv_bits: int = 16):
         self.cfg = cfg
         self.device = torch.device(device)
         self.dt = cfg.dtype
@@ -211,6 +218,11 @@ class TwoModelDecoder:
         if self.counts_host[0] + self.counts_host[1] != self.B:
             raise ValueError("model ids must be 0 or 1")
         self.L_cap = L_cap
+        if kv_bits not in (4, 16):
+            raise ValueError(f"kv_bits must be 4 or 16, got {kv_bits}")
+        if kv_bits == 4 and chain:
+            raise ValueError("the projection chain appends to 16-bit pools: kv_bits=4 runs without it")
+        self.kv_bits = kv_bits
         dev, dt = self.device, self.dt
         H, FF, V = cfg.hidden, cfg.ffn, cfg.vocab
         gen = torch.Generator(device=dev).manual_seed(seed + 1000 * self.rank)
@@ -245,6 +257,9 @@ class TwoModelDecoder:
         # The norm statistics come from the all-reduce kernel or the GEMM
         # epilogue; a plain NCCL all-reduce produces none.
         self.fused = fused_epilogues and (self.tp == 1 or allreduce.startswith("nvlink"))
+        if kv_bits == 4 and not self.fused:
+            raise ValueError("kv_bits=4 runs with the fused epilogues (fused_epilogues=True and, "
+                             "under tensor parallelism, allreduce='nvlink')")
         if self.fused:
             for L in self.layers:
                 L["W_qkv"] = fold_norm(L.pop("W_qkv"), L.pop("ln1"))
@@ -292,7 +307,12 @@ class TwoModelDecoder:
         if kv_layers is not None and not 1 <= self.kv_layers <= cfg.n_layers:
             raise ValueError(f"kv_layers must be in [1, {cfg.n_layers}], got {kv_layers}")
         self.kpool, self.vpool = [], []
+        self.kv4 = []                           # kv_bits=4: (model 0's KV4Pool, model 1's) per layer
         for li in range(cfg.n_layers):
+            if kv_bits == 4:
+                self.kv4.append(self.kv4[li % self.kv_layers] if li >= self.kv_layers else tuple(
+                    KV4Pool.zeros(*sh[:3], dt, dev) if sh[0] else None for sh in shapes))
+                continue
             if li >= self.kv_layers:            # aliased: share set li % kv_layers
                 self.kpool.append(self.kpool[li % self.kv_layers])
                 self.vpool.append(self.vpool[li % self.kv_layers])
@@ -341,7 +361,10 @@ class TwoModelDecoder:
                  for n, e in ((3 * self.Hl, 0), (H, 0), (2 * self.FFl, 1), (self.Vl, 0)))
         self.gemm_ws = torch.zeros(gw, dtype=torch.uint8, device=dev)
         with torch.cuda.device(dev):
-            if page_size is None:
+            if kv_bits == 4:
+                aw = max(lib.ps_kv4_decode_attention_workspace_bytes(m, self.nh, self.nh, L_cap)
+                         for m in (B, s0, s1) if m > 0)
+            elif page_size is None:
                 aw = max(lib.ps_decode_attention_workspace_bytes(m, self.nh, L_cap, 0)
                          for m in (B, s0, s1) if m > 0)
             else:
@@ -386,6 +409,13 @@ class TwoModelDecoder:
             for t in ks + vs:
                 if t is not None:
                     t.normal_(0.0, 1.0, generator=gen)
+        for pools in self.kv4[:self.kv_layers]:     # random codes of a unit normal's range
+            for p in pools:
+                if p is not None:
+                    for codes, meta in ((p.k_codes, p.k_meta), (p.v_codes, p.v_meta)):
+                        codes.random_(0, 256, generator=gen)
+                        meta[..., 0] = 0.27
+                        meta[..., 1] = -2.0
         self.seq_len.fill_(length)
         self._host_len = length
         self.reserve(1)
@@ -417,6 +447,17 @@ class TwoModelDecoder:
         """Store a contiguous history k / v [slots, heads, L, 128] of one model's
         sequences (slots in routed order) into the layer's pools."""
         L = k.shape[2]
+        if self.kv_bits == 4:
+            n, (seqs, _) = k.shape[0], self._kv4_sequences(model, L)
+            if L == 0 or n == 0:
+                return
+            pos = torch.arange(L, dtype=torch.int32, device=self.device).repeat(n)
+            rows = [t.to(self.device, self.dt).transpose(1, 2).reshape(n * L, self.nh, 128)
+                    for t in (k, v)]
+            ops.kv4_append(*rows, self.kv4[layer], pos, rows=seqs[:, 1].repeat_interleave(L),
+                           block_table=None if self.block_table is None else self.block_table.device,
+                           split_point=0 if model else n * L)
+            return
         if self.block_table is None:
             self.kpool[layer][model][:, :, :L].copy_(k)
             self.vpool[layer][model][:, :, :L].copy_(v)
@@ -434,6 +475,13 @@ class TwoModelDecoder:
 
     def read_kv(self, layer: int, model: int, L: int) -> tuple[torch.Tensor, torch.Tensor]:
         """The contiguous history [slots, heads, L, 128] of one model's sequences."""
+        if self.kv_bits == 4:
+            n = self.counts_host[model]
+            seqs, cu = self._kv4_sequences(model, L)
+            k, v = ops.kv4_gather(self.kv4[layer], seqs, cu, n * L,
+                                  block_table=None if self.block_table is None
+                                  else self.block_table.device)
+            return tuple(t.view(n, L, self.nh, 128).transpose(1, 2).contiguous() for t in (k, v))
         if self.block_table is None:
             return (self.kpool[layer][model][:, :, :L].clone(),
                     self.vpool[layer][model][:, :, :L].clone())
@@ -449,6 +497,14 @@ class TwoModelDecoder:
                 k[s, :, i * ps:i * ps + c] = self.kpool[layer][model][pages[i], :, :c]
                 v[s, :, i * ps:i * ps + c] = self.vpool[layer][model][pages[i], :, :c]
         return k, v
+
+    def _kv4_sequences(self, model: int, L: int) -> tuple[torch.Tensor, torch.Tensor]:
+        """(seqs, cu) of positions [0, L) of every sequence of one model, as kv4_gather takes them."""
+        n = self.counts_host[model]
+        base = 0 if model == 0 or self.block_table is None else self.counts_host[0]
+        seqs = torch.tensor([[model, base + s, 0] for s in range(n)], dtype=torch.int32,
+                            device=self.device).view(n, 3)
+        return seqs, torch.arange(n + 1, dtype=torch.int32, device=self.device) * L
 
     # ------------------------------------------------------------ launches
     def _gemm(self, x, W, out, counts, *, residual=None, epilogue=0, M=None) -> None:
@@ -533,6 +589,17 @@ class TwoModelDecoder:
         (slot, or block-table row when paged) if rows share sequences."""
         H, eps = self.cfg.hidden, float(self.cfg.eps)
         for li, L in enumerate(self.layers):
+            if self.kv_bits == 4:
+                e = ops.gemm_epilogue(_lib.PS_EPI_STORE, in_sumsq=sq_in, norm_dim=H, eps=eps)
+                qkv = (self._pf["qkv"] if self._in_prefill else self.qkv)[:x.shape[0]]
+                self._gemm_ex(x, L["W_qkv"], qkv, counts, e)
+                self._attention4(qkv, q, self.kv4[li], attn, pos, counts, bt, kv_rows)
+                self._residual_proj(attn, L["W_o"], x, counts, sq_b)
+                e = ops.gemm_epilogue(_lib.PS_EPI_SWIGLU, in_sumsq=sq_b, norm_dim=H, eps=eps)
+                self._gemm_ex(x, L["W_gu"], a, counts, e)
+                self._residual_proj(a, L["W_d"], x, counts, sq_a)
+                sq_in = sq_a
+                continue
             kp, vp = tuple(self.kpool[li]), tuple(self.vpool[li])
             e = ops.gemm_epilogue(_lib.PS_EPI_QKV_ROPE, in_sumsq=sq_in, norm_dim=H, eps=eps,
                                   k_pools=kp, v_pools=vp, pos=pos, rope_cos=self.rope_cos,
@@ -582,6 +649,21 @@ class TwoModelDecoder:
                                                 scale, dtc, ptr(ws), ws.numel(),
                                                 ptr(self.status), stream),
                   "ps_paged_decode_attention")
+
+    def _attention4(self, qkv, q, pools, attn, pos, counts, bt, kv_rows) -> None:
+        """kv_bits=4: rotate q and the new k, quantise k and v into the cache, attend
+        over the cache (prompt tokens: over their sequences' read-back rows)."""
+        nh = self.nh
+        ops.kv4_append(qkv[:, self.Hl:2 * self.Hl], qkv[:, 2 * self.Hl:], pools, pos,
+                       q=qkv[:, :self.Hl], q_out=q, rope_cos=self.rope_cos, rope_sin=self.rope_sin,
+                       rows=kv_rows, block_table=bt, counts=counts)
+        if not self._in_prefill:
+            ops.kv4_decode_attention(q, pools, pos, max_len=self.L_cap, block_table=bt,
+                                     counts=counts, out=attn, workspace=self.attn_ws)
+            return
+        seqs, cu_q, cu_k, keys = self._pf_seqs
+        k, v = ops.kv4_gather(pools, seqs, cu_k, keys, block_table=bt)
+        ops.prompt_attention(q.view(-1, nh, 128), k, v, cu_q, cu_k, out=attn)
 
     def _residual_proj(self, inp, W, x, counts, sq_out) -> None:
         """x += inp @ W (summed over ranks), and the per-row sums of squares of
@@ -830,7 +912,9 @@ class TwoModelDecoder:
         gw = max(lib.ps_routed_gemm_workspace_bytes(C, n, e, idx)
                  for n, e in ((3 * self.Hl, 0), (H, 0), (2 * self.FFl, 1), (self.Vl, 0)))
         with torch.cuda.device(dev):
-            if self.page_size is None:
+            if self.kv_bits == 4:
+                aw = 0                          # the prompt attention needs no workspace
+            elif self.page_size is None:
                 aw = lib.ps_decode_attention_workspace_bytes(C, self.nh, self.L_cap, 0)
             else:
                 aw = lib.ps_paged_decode_attention_workspace_bytes(C, self.nh, self.L_cap, 0,
@@ -847,6 +931,8 @@ class TwoModelDecoder:
             pick_dst=torch.zeros(self.B, **i32),
             gemm_ws=torch.zeros(gw, dtype=torch.uint8, device=dev),
             attn_ws=torch.zeros(max(aw, 256), dtype=torch.uint8, device=dev))
+        if self.kv_bits == 4:
+            self._pf["qkv"] = torch.zeros(C, 3 * self.Hl, dtype=dt, device=dev)
         return self._pf
 
     def prefill(self, prompts) -> torch.Tensor:
@@ -892,6 +978,8 @@ class TwoModelDecoder:
                 nb = len(ch["qblocks"])
                 pf["qblocks"][:nb].copy_(torch.tensor(ch["qblocks"], dtype=torch.int32))
                 self._pf_nblocks = nb
+                if self.kv_bits == 4:
+                    self._pf_seqs = self._chunk_sequences(ch["qblocks"])
                 x, sq_emb = pf["x"][:n], pf["sq_emb"][:n]
                 check(lib.ps_embed_routed(ptr(self.emb), ptr(pf["tok"]), None, ptr(pf["counts"]),
                                           ptr(x), n, H, self.cfg.vocab, ptr(sq_emb), dtc,
@@ -933,6 +1021,23 @@ class TwoModelDecoder:
         self.reserve(1)
         return self.next_tokens
 
+    def _chunk_sequences(self, qblocks) -> tuple:
+        """The sequences of a prefill chunk, from its runs [row0, nq, p0, model, kv
+        row]: (seqs, cu_q, cu_k, total keys) on the device, keys [0, last position]."""
+        seqs, lens, keys = [], [], []
+        for _, nq, p0, model, row in qblocks:
+            if seqs and seqs[-1][:2] == [model, row] and keys[-1] == p0:
+                lens[-1] += nq
+                keys[-1] += nq
+            else:
+                seqs.append([model, row, 0])
+                lens.append(nq)
+                keys.append(p0 + nq)
+
+        def cum(a):
+            return torch.tensor([0, *a], dtype=torch.int32).cumsum(0, dtype=torch.int32).to(self.device)
+        return (torch.tensor(seqs, dtype=torch.int32).to(self.device), cum(lens), cum(keys), sum(keys))
+
     def launches_per_step(self) -> int:
         """Kernels of this library one fused decode step launches (the torch
         copy of next -> tokens at one GPU and, with allreduce='nccl', the NCCL /
@@ -943,7 +1048,8 @@ class TwoModelDecoder:
             # layer 0's QKV, then attention + one projection chain per layer
             return 3 + 1 + 2 * len(self.layers) + pick
         if self.fused:
-            per_layer, head = 5 + (2 if nvlink else 0), 1
+            # kv_bits=4: rotation and append are a launch of their own
+            per_layer, head = 5 + (self.kv_bits == 4) + (2 if nvlink else 0), 1
         else:
             per_layer, head = 8 + (2 if nvlink else 0), 2
         return 3 + per_layer * len(self.layers) + head + pick
