@@ -14,6 +14,17 @@ implementation, so they appear as single operators to the profiler, to
   parallel_serve::decode_attention(Tensor q, Tensor? k0, Tensor? v0, Tensor? k1, Tensor? v1,
                                    Tensor pos, Tensor counts, int n_heads, int max_len) -> Tensor
   parallel_serve::deltazip_linear(Tensor x, Tensor W_base, Tensor packed, int split_point) -> Tensor
+  parallel_serve::qk_norm_rope(Tensor q, Tensor k, Tensor pos, Tensor? q_weight, Tensor? k_weight,
+                               Tensor? cos, Tensor? sin, Tensor counts, float eps,
+                               bool interleaved) -> (Tensor q, Tensor k)
+  parallel_serve::kv4_append(Tensor k, Tensor v, Tensor(a!)[] pool0, Tensor(b!)[] pool1, Tensor pos,
+                             Tensor counts, Tensor? rows, Tensor? block_table) -> ()
+  parallel_serve::kv4_decode_attention(Tensor q, Tensor[] pool0, Tensor[] pool1, Tensor pos,
+                                       Tensor counts, int max_len, Tensor? rows,
+                                       Tensor? block_table) -> Tensor
+  parallel_serve::prompt_attention(Tensor q, Tensor k, Tensor v, Tensor cu_q, Tensor cu_k) -> Tensor
+
+A 4-bit pool is the four tensors of ``KV4Pool`` as a list, empty for a model without sequences.
 
 Every CUDA implementation is the same ctypes call into libparallel_serve.so
 that the Python API makes (one kernel launch on the current stream, no host
@@ -31,7 +42,8 @@ from .routed_gemm import routed_gemm as _routed_gemm
 __all__ = ["OPS"]
 
 OPS = ("routed_gemm", "routed_gemm_counts", "routed_gemm_model_id", "route_partition",
-       "rmsnorm_routed", "decode_attention", "deltazip_linear")
+       "rmsnorm_routed", "decode_attention", "deltazip_linear", "qk_norm_rope", "kv4_append",
+       "kv4_decode_attention", "prompt_attention")
 
 
 @torch.library.custom_op("parallel_serve::routed_gemm", mutates_args=(), device_types="cuda")
@@ -121,3 +133,65 @@ def deltazip_linear(x: torch.Tensor, W_base: torch.Tensor, packed: torch.Tensor,
 @deltazip_linear.register_fake
 def _(x, W_base, packed, split_point):
     return x.new_empty(x.shape[0], W_base.shape[-1])
+
+
+def _pools(pool0: list[torch.Tensor], pool1: list[torch.Tensor]) -> tuple:
+    return tuple(tuple(p) if p else None for p in (pool0, pool1))
+
+
+@torch.library.custom_op("parallel_serve::qk_norm_rope", mutates_args=(), device_types="cuda")
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, pos: torch.Tensor,
+                 q_weight: torch.Tensor | None, k_weight: torch.Tensor | None,
+                 cos: torch.Tensor | None, sin: torch.Tensor | None, counts: torch.Tensor,
+                 eps: float, interleaved: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    """RMSNorm of every q and k head and the position rotation, in one pass."""
+    return ops.qk_norm_rope(q, k, pos, q_weight=q_weight, k_weight=k_weight, rope_cos=cos,
+                            rope_sin=sin, counts=counts, eps=eps, interleaved=interleaved)
+
+
+@qk_norm_rope.register_fake
+def _(q, k, pos, q_weight, k_weight, cos, sin, counts, eps, interleaved):
+    return q.new_empty(q.shape), k.new_empty(k.shape)
+
+
+@torch.library.custom_op("parallel_serve::kv4_append", mutates_args=("pool0", "pool1"),
+                         device_types="cuda")
+def kv4_append(k: torch.Tensor, v: torch.Tensor, pool0: list[torch.Tensor],
+               pool1: list[torch.Tensor], pos: torch.Tensor, counts: torch.Tensor,
+               rows: torch.Tensor | None, block_table: torch.Tensor | None) -> None:
+    """Quantise k and v into the 4-bit cache at positions pos."""
+    ops.kv4_append(k, v, _pools(pool0, pool1), pos, counts=counts, rows=rows,
+                   block_table=block_table)
+
+
+@kv4_append.register_fake
+def _(k, v, pool0, pool1, pos, counts, rows, block_table):
+    return None
+
+
+@torch.library.custom_op("parallel_serve::kv4_decode_attention", mutates_args=(),
+                         device_types="cuda")
+def kv4_decode_attention(q: torch.Tensor, pool0: list[torch.Tensor], pool1: list[torch.Tensor],
+                         pos: torch.Tensor, counts: torch.Tensor, max_len: int,
+                         rows: torch.Tensor | None,
+                         block_table: torch.Tensor | None) -> torch.Tensor:
+    """Decode attention over the 4-bit cache, grouped heads."""
+    return ops.kv4_decode_attention(q, _pools(pool0, pool1), pos, max_len=max_len, counts=counts,
+                                    rows=rows, block_table=block_table)
+
+
+@kv4_decode_attention.register_fake
+def _(q, pool0, pool1, pos, counts, max_len, rows, block_table):
+    return q.new_empty(q.shape[0], q.shape[1] * (q.shape[2] if q.dim() == 3 else 1))
+
+
+@torch.library.custom_op("parallel_serve::prompt_attention", mutates_args=(), device_types="cuda")
+def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor,
+                     cu_k: torch.Tensor) -> torch.Tensor:
+    """Causal attention over packed prompts, grouped heads."""
+    return ops.prompt_attention(q, k, v, cu_q, cu_k)
+
+
+@prompt_attention.register_fake
+def _(q, k, v, cu_q, cu_k):
+    return q.new_empty(q.shape[0], q.shape[1] * (q.shape[2] if q.dim() == 3 else 1))

@@ -474,3 +474,93 @@ def test_step_in_a_graph_and_on_another_stream():
     graph.replay()
     assert torch.equal(got, want)
     assert _status() == 0
+
+
+def test_registered_operators_run_together():
+    """norm + rotation, cache write, decode and prompt attention through torch.ops: what
+    a prompt and the step after it do."""
+    from parallel_serve_b200 import KV4Pool, ops
+    P = torch.ops.parallel_serve
+    dt, nh, nkv, T = torch.bfloat16, 8, 2, 37
+    qkv = cpu_randn((T, nh + 2 * nkv, 128), 101, 1.0, dt).to(DEV)
+    w = _weights(6, dt).to(DEV)
+    cos, sin = _tables(64, 128)
+    pos = torch.arange(T, dtype=torch.int32, device=DEV)
+    counts = torch.tensor([T, 0], dtype=torch.int32, device=DEV)
+    q, k = P.qk_norm_rope(qkv[:, :nh], qkv[:, nh:nh + nkv], pos, w, w, cos, sin, counts, 1e-6, False)
+    v = qkv[:, nh + nkv:]
+    pool = KV4Pool.zeros(1, nkv, 64, dt, DEV)
+    rows = torch.zeros(T, dtype=torch.int32, device=DEV)
+    P.kv4_append(k, v, list(pool), [], pos, counts, rows, None)
+    cu = torch.tensor([0, T], dtype=torch.int32, device=DEV)
+    seqs = torch.zeros(1, 3, dtype=torch.int32, device=DEV)
+    k4, v4 = ops.kv4_gather((pool, None), seqs, cu, T)
+    prompt = P.prompt_attention(q, k4, v4, cu, cu)
+    step = P.kv4_decode_attention(q, list(pool), [], pos, counts, 64, rows, None)
+    # the same attention twice: over the read-back rows on the tensor core, over the
+    # codes row by row. They differ by their own roundings (eps/2 of P and of the
+    # output, and the read-back's eps/2 of k and v; scores here stay below 2^4).
+    eps = torch.finfo(dt).eps
+    _, size = __import__("oracle").grouped_attention(to_np(q), to_np(k4), to_np(v4))
+    err = np.abs(to_np(prompt) - to_np(step)).reshape(size.shape)
+    assert np.all(err <= eps * np.abs(to_np(step)).reshape(size.shape) + (2 + 2 ** 4) * eps * size)
+    assert _status() == 0
+
+
+def test_wrappers_refuse():
+    from parallel_serve_b200 import KV4Pool, ops
+    dt = torch.float16
+    q = torch.zeros(2, 4, 128, dtype=dt, device=DEV)
+    k = torch.zeros(2, 2, 128, dtype=dt, device=DEV)
+    i = torch.zeros(2, dtype=torch.int32, device=DEV)
+    pool = KV4Pool.zeros(2, 2, 16, dt, DEV)
+    cos, sin = _tables(16, 128)
+    tab = torch.zeros(2, 1, dtype=torch.int32, device=DEV)
+    seqs = torch.zeros(2, 3, dtype=torch.int32, device=DEV)
+    cu = torch.tensor([0, 1, 2], dtype=torch.int32, device=DEV)
+    for call in (
+            lambda: ops.qk_norm_rope(q, k[:1], i),
+            lambda: ops.qk_norm_rope(q[..., :64], k, i),
+            lambda: ops.qk_norm_rope(q.transpose(0, 1), k, i),
+            lambda: ops.qk_norm_rope(q, k.bfloat16(), i),
+            lambda: ops.qk_norm_rope(q, k, i.long()),
+            lambda: ops.qk_norm_rope(q, k, i[:1]),
+            lambda: ops.qk_norm_rope(q, k, i, rope_cos=cos),
+            lambda: ops.qk_norm_rope(q, k, i, rope_cos=cos[:, :5], rope_sin=sin[:, :5]),
+            lambda: ops.qk_norm_rope(q, k, i, q_weight=torch.ones(128, dtype=dt, device=DEV)),
+            lambda: ops.qk_norm_rope(q, k, i, split_point=3),
+            lambda: ops.qk_norm_rope(q, k, i, q_out=k),
+            lambda: ops.kv4_append(k, k, (None, None), i),
+            lambda: ops.kv4_append(k, k, (pool,), i),
+            lambda: ops.kv4_append(k[:, :1], k[:, :1], (pool, None), i),
+            lambda: ops.kv4_append(k, k[:1], (pool, None), i),
+            lambda: ops.kv4_append(k.bfloat16(), k.bfloat16(), (pool, None), i),
+            lambda: ops.kv4_append(k, k, (pool, KV4Pool.zeros(2, 2, 8, dt, DEV)), i),
+            lambda: ops.kv4_append(k, k, (pool, None), i, q_out=q),
+            lambda: ops.kv4_append(k, k, (pool, None), i, rows=i[:1]),
+            lambda: ops.kv4_append(k, k, (pool, None), i, block_table=tab[:1]),
+            lambda: ops.kv4_append(k, k, (pool, None), i, block_table=i),
+            lambda: ops.kv4_append(k, k, (KV4Pool.zeros(2, 2, 12, dt, DEV), None), i, block_table=tab),
+            lambda: ops.kv4_append(k, k, (KV4Pool(pool[0], pool[1], pool[2], pool[3][..., :1]), None), i),
+            lambda: ops.kv4_gather((pool, None), seqs[:, :2], cu, 2),
+            lambda: ops.kv4_gather((pool, None), seqs, cu[:2], 2),
+            lambda: ops.kv4_gather((pool, None), seqs, cu, -1),
+            lambda: ops.kv4_gather((pool, None), seqs, cu, 2, out=(k, q)),
+            lambda: ops.kv4_decode_attention(q[:, :3], (pool, None), i, max_len=16),
+            lambda: ops.kv4_decode_attention(q, (pool, None), i, max_len=17),
+            lambda: ops.kv4_decode_attention(q, (pool, None), i, max_len=0),
+            lambda: ops.kv4_decode_attention(q, (pool, None), i, max_len=16, out=q),
+            lambda: ops.kv4_decode_attention(q, (pool, None), i.cpu(), max_len=16),
+            lambda: ops.prompt_attention(q, k, k[:1], cu),
+            lambda: ops.prompt_attention(q[:, :3], k, k, cu),
+            lambda: ops.prompt_attention(q, k, k, cu, cu[:2]),
+            lambda: ops.prompt_attention(q, k[:1], k[:1], cu),
+            lambda: ops.prompt_attention(q, k, k, cu, scale=0.0),
+            lambda: ops.prompt_attention(q, k, k, cu, out=k)):
+        with pytest.raises((ValueError, TypeError)):
+            call()
+    from parallel_serve_b200 import _lib
+    with pytest.raises(_lib.PSError):
+        ops.kv4_decode_attention(q, (pool, None), i, max_len=16,
+                                 workspace=torch.zeros(64, dtype=torch.uint8, device=DEV))
+    assert _status() == 0
