@@ -18,10 +18,10 @@
 //   O = sum_pos (P s_g) (c - 8)  (P s_g / ref rounded to fp16)
 //       + sum_pos P (z_g + 8 s_g)  (fp32)
 // with ref a running power of two >= every s seen, rescaled like the softmax's
-// running maximum, so bf16 scales of any exponent fit. The - 8 (one more
-// instruction per product, with a constant operand) keeps the summands of O as
-// small as the values themselves: around c alone, the rounding of P s_g weighs
-// about twice as much and a long sum loses the digits that z then cancels.
+// running maximum, so bf16 scales of any exponent fit. The - 8 (one packed
+// subtraction of subnormals, exact) keeps the summands of O as small as the values
+// themselves: around c alone, the rounding of P s_g weighs about twice as much and a
+// long sum loses the digits that z then cancels.
 // The z term of S is a product too: the sums of q, cut into 16-bit parts that
 // together carry fp32's digits, against the stored zeros. q is scaled per head by a
 // power of two into fp16's range (exact down to 2^-24 of the head's largest).
@@ -142,6 +142,13 @@ PS_DEV uint32_t max16x2(uint32_t a, uint32_t b) {
   return *reinterpret_cast<const uint32_t*>(&m);
 }
 
+// a - b of two pairs of fp16 values (exact for codes and 8: subnormals).
+PS_DEV uint32_t centre(uint32_t a, uint32_t b) {
+  const __half2 d =
+      __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&d);
+}
+
 PS_DEV uint32_t half2_bits(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -161,42 +168,37 @@ PS_DEV int token_len(const AttnArgs& a, int j, int c0) {
 
 PS_DEV int tiles_of(int len) { return (len + kTile - 1) / kTile; }
 
-// One piece of a CTA's range: tiles [t0, t1) of item (token j, KV head kvh,
-// head block hb).
+// One piece of a CTA's range [b S, b S + S) of tiles: tiles [t0, t1) of item
+// (token j, KV head kvh, head block hb), which starts at tile number `start`.
 struct Piece {
-  int j, len, kvh, hb, t0, t1, slot, nsplit;
-  long long first_cta, item_start, end;
+  int j, len, kvh, hb, t0, t1, start, nt, end;
 };
 
-PS_DEV Piece piece_at(const AttnArgs& a, const int32_t* P, int entries, int c0, long long S,
-                      long long g, long long g1, int b) {
+PS_DEV Piece piece_at(const AttnArgs& a, const int32_t* first, int entries, int c0, int g,
+                      int g1) {
   const int HB = a.n_kv * a.hblocks;
   int lo = 0, hi = entries - 1;  // last entry that starts at or before g
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if ((long long)P[mid] * HB <= g) lo = mid; else hi = mid - 1;
+    if (first[mid] * HB <= g) lo = mid; else hi = mid - 1;
   }
-  long long at = (long long)P[lo] * HB;
+  int at = first[lo] * HB;
   int j = lo * a.per_entry, len = token_len(a, j, c0);
-  while ((long long)tiles_of(len) * HB + at <= g && j + 1 < a.M) {  // within the entry
-    at += (long long)tiles_of(len) * HB;
+  while (at + tiles_of(len) * HB <= g && j + 1 < a.M) {  // within the entry
+    at += tiles_of(len) * HB;
     len = token_len(a, ++j, c0);
   }
   Piece p;
   p.j = j;
   p.len = len;
-  const int nt = max(1, tiles_of(len));
-  const int it = (int)((g - at) / nt);
+  p.nt = max(1, tiles_of(len));
+  const int it = (g - at) / p.nt;
   p.kvh = it / a.hblocks;
-  p.hb = it % a.hblocks;
-  p.t0 = (int)((g - at) % nt);
-  p.item_start = at + (long long)it * nt;
-  const long long iend = p.item_start + nt;
-  p.end = g1 < iend ? g1 : iend;
-  p.t1 = p.t0 + (int)(p.end - g);
-  p.first_cta = p.item_start / S;
-  p.nsplit = (int)((iend - 1) / S - p.first_cta) + 1;
-  p.slot = g == (long long)b * S ? 0 : 1;
+  p.hb = it - p.kvh * a.hblocks;
+  p.start = at + it * p.nt;
+  p.t0 = g - p.start;
+  p.end = min(g1, p.start + p.nt);
+  p.t1 = p.end - p.start;
   return p;
 }
 
@@ -268,10 +270,10 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm)
     }
   }
   __syncthreads();
-  const long long W = (long long)P[entries] * a.n_kv * a.hblocks;
-  const long long S = (W + gridDim.x - 1) / gridDim.x;
-  const long long g0 = (long long)b * S;
-  const long long g1 = g0 + S < W ? g0 + S : W;
+  const int W = P[entries] * a.n_kv * a.hblocks;
+  const int S = (W + gridDim.x - 1) / gridDim.x;
+  const int g0 = min(W, b * S);
+  const int g1 = min(W, g0 + S);
   if (g0 >= g1) return;
 
   if (warp == kWarps) {
@@ -279,8 +281,8 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm)
     const uint64_t pol = l2_policy_evict_first();
     int gs = 0;
     bool dead = false;
-    for (long long g = g0; g < g1 && !dead;) {
-      const Piece pc = piece_at(a, P, entries, c0, S, g, g1, b);
+    for (int g = g0; g < g1 && !dead;) {
+      const Piece pc = piece_at(a, P, entries, c0, g, g1);
       const int m = pc.j >= c0 ? 1 : 0;
       const Pool pool = m ? a.pool[1] : a.pool[0];
       const int home = a.rows ? a.rows[pc.j] : (a.block_table ? pc.j : pc.j - (m ? c0 : 0));
@@ -368,12 +370,12 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm)
   const int sig0 = (2 * t4) ^ (t4 & 1), sig1 = (2 * t4 + 1) ^ (t4 & 1);
   const uint32_t vsel = (gr & 1) ? 0x7632u : 0x5410u;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
-  // -8 on the scale of a low and of a high nibble, twice
-  constexpr uint32_t kMinus8Low = 0x80088008u, kMinus8High = 0x80808080u;
+  // 8 on the scale of a low and of a high nibble, twice
+  constexpr uint32_t kLow8 = 0x00080008u, kHigh8 = 0x00800080u;
   int gs = 0;
   bool dead = false;
-  for (long long g = g0; g < g1;) {
-    const Piece pc = piece_at(a, P, entries, c0, S, g, g1, b);
+  for (int g = g0; g < g1;) {
+    const Piece pc = piece_at(a, P, entries, c0, g, g1);
     const int nh = min(kHB, a.group - pc.hb * kHB);
     const int head0 = pc.kvh * a.group + pc.hb * kHB;
     const T* qrow = reinterpret_cast<const T*>(a.q) + (size_t)pc.j * a.q_stride;
@@ -605,12 +607,11 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm)
             const uint32_t x = __byte_perm(v[0][gi], v[1][gi], vsel);
             const uint32_t y = __byte_perm(v[2][gi], v[3][gi], vsel);
             const uint32_t xh = x >> 8, yh = y >> 8;
-            mma16816(o[2 * gi], kMinus8Low, kMinus8High, kMinus8Low, kMinus8High, b0, b1);
-            mma16816(o[2 * gi + 1], kMinus8Low, kMinus8High, kMinus8Low, kMinus8High, b0, b1);
-            mma16816(o[2 * gi], x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu,
-                     y & 0x00f000f0u, b0, b1);
-            mma16816(o[2 * gi + 1], xh & 0x000f000fu, xh & 0x00f000f0u, yh & 0x000f000fu,
-                     yh & 0x00f000f0u, b0, b1);
+            mma16816(o[2 * gi], centre(x & 0x000f000fu, kLow8), centre(x & 0x00f000f0u, kHigh8),
+                     centre(y & 0x000f000fu, kLow8), centre(y & 0x00f000f0u, kHigh8), b0, b1);
+            mma16816(o[2 * gi + 1], centre(xh & 0x000f000fu, kLow8),
+                     centre(xh & 0x00f000f0u, kHigh8), centre(yh & 0x000f000fu, kLow8),
+                     centre(yh & 0x00f000f0u, kHigh8), b0, b1);
           }
         }
       }
@@ -652,7 +653,9 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm)
     bad |= dead;
     const int ch = tid;
     T* out = reinterpret_cast<T*>(a.out) + ((size_t)pc.j * a.n_heads + head0) * kD + ch;
-    const size_t slot = (size_t)b * 2 + pc.slot;
+    // CTAs [cf, cl] have pieces of this item; a CTA's slot 0 is its range's first piece
+    const int cf = pc.start / S, cl = (pc.start + pc.nt - 1) / S;
+    const size_t slot = (size_t)b * 2 + (g == g0 ? 0 : 1);
     for (int h = 0; h < nh; ++h) {
       float M = -INFINITY, L = 0.f, O = 0.f;
 #pragma unroll
@@ -664,7 +667,7 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm)
         L += sml[(w * kHB + h) * 2 + 1] * f;
         O += so[(w * kHB + h) * kD + ch] * f;
       }
-      if (pc.nsplit == 1) {
+      if (cf == cl) {
         if (!bad) out[h * kD] = from_f32<T>(O / L);
       } else {
         __stcg(a.ws_o + (slot * kHB + h) * kD + ch, O);
@@ -675,14 +678,14 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm)
       }
     }
     named_bar_sync(1, kWarps * 32);
-    if (pc.nsplit > 1) {
+    if (cf != cl) {
       // ranges are contiguous, so at most one item continues past each CTA's
       // end: its first CTA's number identifies it
-      int32_t* counter = a.counter + pc.first_cta;
+      int32_t* counter = a.counter + cf;
       if (tid == 0) {
         fence_acq_rel_gpu();
         const int old = atom_add_acq_rel_gpu(counter, 1);
-        const int last = old + 1 == pc.nsplit ? 1 : 0;
+        const int last = old == cl - cf ? 1 : 0;
         if (last) *counter = 0;
         last_flag[0] = last;
       }
@@ -693,9 +696,9 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm)
         for (int h = 0; h < nh; ++h) {
           float M = -INFINITY, L = 0.f, O = 0.f;
           bool any_bad = false;
-          for (int c = 0; c < pc.nsplit; ++c) {
-            const long long cb = pc.first_cta + c;
-            const size_t sl = (size_t)cb * 2 + (pc.item_start <= cb * S ? 0 : 1);
+#pragma unroll 4
+          for (int c = cf; c <= cl; ++c) {
+            const size_t sl = (size_t)c * 2 + (pc.start <= c * S ? 0 : 1);
             const float mc = __ldcg(a.ws_ml + (sl * kHB + h) * 2);
             const float lc = __ldcg(a.ws_ml + (sl * kHB + h) * 2 + 1);
             const float oc = __ldcg(a.ws_o + (sl * kHB + h) * kD + ch);
@@ -766,8 +769,9 @@ extern "C" int ps_kv4_decode_attention(const void* q, long long q_stride,
                q_stride % 8 == 0);
   PS_CHECK_ARG(!cache->block_table || rows || cache->table_rows >= M);
   const int hblocks = cdiv(n_heads / n_kv, kv4::kHB);
-  // the prefix sums of tiles are 32-bit
-  if ((long long)M * cdiv(max_len, kv4::kTile) > (1ll << 30)) return PS_ERR_UNSUPPORTED;
+  // tile numbers are 32-bit
+  if ((long long)M * n_kv * hblocks * cdiv(max_len, kv4::kTile) > (1ll << 30))
+    return PS_ERR_UNSUPPORTED;
   const int device = current_device();
   if (!is_sm100(device)) return PS_ERR_UNSUPPORTED;
   const kv4::AttnPlan p = kv4::plan_attention(M, n_kv, hblocks, max_len, device);
