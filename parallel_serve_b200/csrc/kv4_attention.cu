@@ -288,11 +288,19 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm)
       const int home = a.rows ? a.rows[pc.j] : (a.block_table ? pc.j : pc.j - (m ? c0 : 0));
       for (int t = pc.t0; t < pc.t1; ++t, ++gs) {
         const int st = gs % kStages;
+        const int pos0 = t * kTile;
+        const int npos = min(kTile, pc.len - pos0);
+        // one run per page (128 % page_size == 0 or page_size % 128 == 0, so runs
+        // start at multiples of page_size or fill the tile): lane l takes run l (at
+        // most 16 of them), and looks its page up while the stage is still in use
+        const int run = min(a.page_size, kTile);
+        const int nrun = a.block_table ? (npos + run - 1) / run : 0;
+        int page = 0;
+        if (lane < nrun)
+          page = a.block_table[(size_t)home * a.max_pages + ((pos0 + lane * run) >> a.page_shift)];
         if (!mbar_wait(empty + st, ((gs / kStages) & 1) ^ 1, a.status)) abort_flag[0] = 1;
         dead = __any_sync(0xffffffffu, abort_flag[0] != 0);
         if (dead) break;
-        const int pos0 = t * kTile;
-        const int npos = min(kTile, pc.len - pos0);
         uint8_t* buf = smem + st * kStageBytes;
         if (!a.block_table) {
           if (lane == 0) {
@@ -313,19 +321,8 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm)
             bulk_load(buf + 2 * kTileCodes + kTileMeta, pool.v_meta + row * kMetaBytes,
                       npos * kMetaBytes, full + st, pol);
         } else {
-          // one run per page (128 % page_size == 0 or page_size % 128 == 0, so
-          // runs start at multiples of page_size or fill the tile): lane l
-          // takes run l (at most 16 of them)
-          const int run = min(a.page_size, kTile);
-          const int nrun = (npos + run - 1) / run;
-          int page = 0;
-          bool bad = false;
-          if (lane < nrun) {
-            const int pi = (pos0 + lane * run) >> a.page_shift;
-            page = a.block_table[(size_t)home * a.max_pages + pi];
-            bad = page < 0 || page >= pool.rows;
-            if (bad) page = 0;  // read a page that exists; the piece's output is dropped
-          }
+          bool bad = page < 0 || page >= pool.rows;  // lanes without a run have page 0
+          if (bad) page = 0;  // read a page that exists; the piece's output is dropped
           const bool any_bad = __any_sync(0xffffffffu, bad);
           if (lane == 0) {
             if (any_bad) set_status(a.status, PS_ERR_BAD_INDEX);
