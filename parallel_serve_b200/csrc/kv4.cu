@@ -69,9 +69,9 @@ PS_DEV Vec8 pack8(const float* f) {
 // its word of codes (and the group's (s, z), by its first lane).
 //
 // The quotient d / s is y = d r with r = 1 / s, corrected once by its own remainder,
-// y + (d - s y) r (Markstein's step): where d / s is a half-integer, which with
-// 16-bit inputs happens 2 times in 1000, the result is that half exactly and the
-// rounding to even is the one that a division would give. (A division for each
+// y + (d - s y) r (Markstein's step): the correctly rounded quotient, so that next
+// to half-integers (with 16-bit inputs 2 in 1000 are exact halves) the code is the
+// one that a division would give. (A division for each
 // channel took most of this kernel's time.) Rounding and packing go through the
 // low mantissa bits of 1.5 * 2^23 + quotient; a conversion to integer takes four
 // times as long.
@@ -112,6 +112,7 @@ PS_DEV void store_row4(const float (&x)[8], int lane, unsigned mask, uint8_t* co
   } else {
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
+    r = fmaf(r, fmaf(-s, r, 1.f), r);  // to the last bit, which the step below wants
     const uint64_t zz = f32x2(-z, -z), rr = f32x2(r, r), ss = f32x2(-s, -s);
 #pragma unroll
     for (int i = 6; i >= 0; i -= 2) {
@@ -252,13 +253,11 @@ __global__ void __launch_bounds__(kThreads, 8) norm_rope_kernel(const RowArgs a)
         }
       } else {
 #pragma unroll
-        for (int i = 0; i < 8; i += 2) {
-          const float y0 = __shfl_sync(mask, x[i], partner, 16);
-          const float y1 = __shfl_sync(mask, x[i + 1], partner, 16);
-          if (turned)  // si is - sin in the first elements of the pairs
-            f32x2_split(f32x2_add(f32x2_mul(f32x2(x[i], x[i + 1]), f32x2(co[i], co[i + 1])),
-                                  f32x2_mul(f32x2(y0, y1), f32x2(si[i], si[i + 1]))),
-                        x[i], x[i + 1]);
+        for (int i = 0; i < 8; ++i) {
+          const float y = __shfl_sync(mask, x[i], partner, 16);
+          // si is - sin in the first elements of the pairs; the two products are
+          // rounded each (a packed mul and add would be contracted to one fma)
+          if (turned) x[i] = __fadd_rn(__fmul_rn(x[i], co[i]), __fmul_rn(y, si[i]));
         }
       }
     }
