@@ -3,11 +3,16 @@
 // all three is memory traffic, so every row is read once and written once, 16
 // bytes a lane.
 //
-// Half a warp owns a row (lane l of 16: channels 8l .. 8l+7), so the norm's sum
-// takes 4 shuffles, the half-layout rotation exchanges with the lane rotary/16
-// away (interleaved pairs stay inside a lane), and a 32-channel group is 4
-// lanes. A block works on one token; each half warp takes up to kRows of the
-// token's heads, issues their loads together and reuses the token's cos / sin.
+// Norm, rotation and write: four lanes own a row. Lane q has the 16-byte chunks 2q,
+// 2q + 1, 2q + 8 and 2q + 9, so both channels of a pair (i, i + 64) of the whole-head
+// rotation are in one lane, as interleaved pairs are, and a 32-channel group is two
+// lanes: what a group takes beside its channels (its zero, scale and reciprocal)
+// is done by two lanes, not by four with four times the calls. Instructions bounded
+// the write with 16 lanes to a row: writing and reading back 16 prompts of up to 2048
+// tokens with 32 + 32 heads took 575 us, with four lanes 382 (the bytes alone 299);
+// norm and rotation of 16384 tokens with 32 + 8 heads 74 and 63 (52). A block takes a
+// few tokens; each quad takes every Q-th of its token's rows, loads one ahead, and
+// keeps the token's cos / sin in registers.
 //
 // Arithmetic is fp32 throughout (norm, weight, rotation, quantisation) with one
 // rounding at the end: q / k to the 16-bit type, or straight to codes. The
@@ -22,8 +27,9 @@ namespace ps {
 namespace kv4 {
 
 constexpr int kThreads = 128;
-constexpr int kHalfWarps = kThreads / 16;
-constexpr int kRows = 4;  // rows of one half warp in the read-back
+constexpr int kQuads = kThreads / 4;
+constexpr int kHalfWarps = kThreads / 16;  // the read-back
+constexpr int kRows = 2;                   // rows of one half warp there
 
 struct RowArgs {
   const void* q;  // [M, n_heads, 128], token stride q_stride (elements); nullable
@@ -43,7 +49,8 @@ struct RowArgs {
   Pool pool[2];
   int32_t* status;
   int M, n_heads, n_kv, split_point, rotary, interleaved, rope_len;
-  int rows_per;  // rows of one half warp
+  int quads;     // of a token in a block: a power of two up to kQuads
+  int rows_per;  // rows of a quad
   int L_cap, page_size, page_shift, max_pages, table_rows;  // append
   float eps;
 };
@@ -65,33 +72,32 @@ PS_DEV Vec8 pack8(const float* f) {
   return a;
 }
 
-// Quantise this lane's 8 channels with the 3 other lanes of its group and store
-// its word of codes (and the group's (s, z), by its first lane).
+// Rotations that a kernel is made for: pairs (i, i + 64) of the whole head,
+// interleaved pairs, and half-layout pairs of a part of the head.
+enum Rotation { kNone, kWhole, kInterleaved, kPart };
+
+// Quantise a group: 16 channels of this lane, 16 of the lane beside it. Words of 8
+// codes and the group's (s, z).
 //
 // The quotient d / s is y = d r with r = 1 / s, corrected once by its own remainder,
 // y + (d - s y) r (Markstein's step): the correctly rounded quotient, so that next
 // to half-integers (with 16-bit inputs 2 in 1000 are exact halves) the code is the
-// one that a division would give. (A division for each
-// channel took most of this kernel's time.) Rounding and packing go through the
-// low mantissa bits of 1.5 * 2^23 + quotient; a conversion to integer takes four
-// times as long.
+// one that a division would give. A division for each channel took most of this
+// kernel's time. Rounding and packing go through the low mantissa bits of
+// 1.5 * 2^23 + quotient; a conversion to integer takes four times as long.
 template <typename T>
-PS_DEV void store_row4(const float (&x)[8], int lane, unsigned mask, uint8_t* codes, uint8_t* meta) {
-  float lo = x[0], hi = x[0], zero = 0.f;  // zero: NaN when an x is not finite
+PS_DEV void quantise_group(const float (&a)[8], const float (&b)[8], unsigned mask,
+                           uint32_t (&word)[2], uint32_t& meta) {
+  float lo = fminf(a[0], b[0]), hi = fmaxf(a[0], b[0]), zero = 0.f;  // NaN when not all finite
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    lo = fminf(lo, x[i]);
-    hi = fmaxf(hi, x[i]);
-    zero = fmaf(x[i], 0.f, zero);
+    lo = fminf(lo, fminf(a[i], b[i]));
+    hi = fmaxf(hi, fmaxf(a[i], b[i]));
+    zero = fmaf(a[i], 0.f, fmaf(b[i], 0.f, zero));
   }
-#pragma unroll
-  for (int o = 1; o <= 2; o <<= 1) {
-    lo = fminf(lo, __shfl_xor_sync(mask, lo, o));
-    hi = fmaxf(hi, __shfl_xor_sync(mask, hi, o));
-  }
-  const int g = lane >> 2, w = lane & 3;
-  const unsigned nonfinite = __ballot_sync(mask, zero != zero);
-  const bool bad = (nonfinite >> ((threadIdx.x & 16) + 4 * g)) & 15u;
+  lo = fminf(lo, __shfl_xor_sync(mask, lo, 1));
+  hi = fmaxf(hi, __shfl_xor_sync(mask, hi, 1));
+  zero += __shfl_xor_sync(mask, zero, 1);
   T zt = saturate<T>(lo);
   const float z = to_f32<T>(zt);
   const float span = __fsub_rn(hi, z);
@@ -101,58 +107,60 @@ PS_DEV void store_row4(const float (&x)[8], int lane, unsigned mask, uint8_t* co
   T st = saturate<T>(range);
   float s = to_f32<T>(st);
   if (s == 0.f) s = 1.f;  // a constant group: every code 0
-  uint32_t word = 0;
   if (s < 1.1754944e-38f || isinf(span)) {
     // 1 / s or a difference may not exist in fp32: divide
 #pragma unroll
-    for (int i = 7; i >= 0; --i) {
-      const float y = __fdiv_rn(__fsub_rn(x[i], z), s);
-      word = word * 16u + (uint32_t)rintf(fminf(fmaxf(y, 0.f), 15.f));
+    for (int k = 0; k < 2; ++k) {
+      word[k] = 0;
+#pragma unroll
+      for (int i = 7; i >= 0; --i) {
+        const float y = __fdiv_rn(__fsub_rn(k ? b[i] : a[i], z), s);
+        word[k] = word[k] * 16u + (uint32_t)rintf(fminf(fmaxf(y, 0.f), 15.f));
+      }
     }
   } else {
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
     r = fmaf(r, fmaf(-s, r, 1.f), r);  // to the last bit, which the step below wants
-    const uint64_t zz = f32x2(-z, -z), rr = f32x2(r, r), ss = f32x2(-s, -s);
 #pragma unroll
-    for (int i = 6; i >= 0; i -= 2) {
-      const uint64_t d = f32x2_add(f32x2(x[i], x[i + 1]), zz);
-      const uint64_t y0 = f32x2_mul(d, rr);
-      float lo_y, hi_y;
-      f32x2_split(f32x2_fma(f32x2_fma(ss, y0, d), rr, y0), lo_y, hi_y);
-      hi_y = __fadd_rn(fminf(fmaxf(hi_y, 0.f), 15.f), 12582912.f);
-      lo_y = __fadd_rn(fminf(fmaxf(lo_y, 0.f), 15.f), 12582912.f);
-      word = (word * 16u + __float_as_uint(hi_y)) * 16u + __float_as_uint(lo_y);
+    for (int k = 0; k < 2; ++k) {
+      word[k] = 0;
+#pragma unroll
+      for (int i = 7; i >= 0; --i) {
+        const float d = __fsub_rn(k ? b[i] : a[i], z);
+        const float y0 = __fmul_rn(d, r);
+        const float y = fmaf(fmaf(-s, y0, d), r, y0);
+        word[k] = word[k] * 16u +
+                  __float_as_uint(__fadd_rn(fminf(fmaxf(y, 0.f), 15.f), 12582912.f));
+      }
+      word[k] -= 0x3f400000u;  // 0x4b400000 (1 + 16 + 256 + ...) in 32 bits
     }
-    word -= 0x3f400000u;  // 0x4b400000 (1 + 16 + 256 + ...) in 32 bits
   }
-  if (bad) {
-    word = 0;
+  if (zero != zero) {
+    word[0] = word[1] = 0;
     st = from_f32<T>(0.f);
     zt = from_f32<T>(__uint_as_float(0x7fc00000u));
   }
-  reinterpret_cast<uint32_t*>(codes)[4 * w + g] = word;
-  if (w == 0) {
-    T pair[2] = {st, zt};
-    reinterpret_cast<uint32_t*>(meta)[g] = *reinterpret_cast<uint32_t*>(pair);
-  }
+  const T pair[2] = {st, zt};
+  meta = *reinterpret_cast<const uint32_t*>(pair);
 }
 
-// grid (M, ceil(rows per token / (kHalfWarps * rows_per))). Rows of a token: its q
-// heads, its k heads, then (append) its v heads.
-template <typename T, bool kAppend>
-__global__ void __launch_bounds__(kThreads, 8) norm_rope_kernel(const RowArgs a) {
+// Rows of a token: its q heads, its k heads, then (append) its v heads. grid
+// (ceil(M / tokens of a block), row blocks).
+template <typename T, bool kAppend, int kRot>
+__global__ void __launch_bounds__(kThreads) norm_rope_kernel(const RowArgs a) {
   pdl_wait();
   pdl_launch_dependents();
-  const int j = blockIdx.x;
-  const int hw = threadIdx.x >> 4, lane = threadIdx.x & 15;
-  const unsigned mask = 0xffffu << (threadIdx.x & 16);
+  const int quad = threadIdx.x >> 2, q4 = threadIdx.x & 3;
+  const unsigned mask = 0xfu << (threadIdx.x & 28);
+  const int j = blockIdx.x * (kQuads / a.quads) + quad / a.quads;
+  if (j >= a.M) return;
   const int nq = a.q ? a.n_heads : 0;
   const int total = nq + (kAppend ? 2 : 1) * a.n_kv;
   const int c0 = a.counts ? a.counts[0] : a.split_point;
   const int m = j >= c0 ? 1 : 0;
   const int p = a.pos[j];
-  bool ok = p >= 0 && (!a.rc || p < a.rope_len);
+  bool ok = p >= 0 && (kRot == kNone || p < a.rope_len);
   size_t cache_row = 0;  // first (row, head 0, position) index of this token
   int cache_len = 0;
   const Pool pool = m ? a.pool[1] : a.pool[0];
@@ -173,112 +181,161 @@ __global__ void __launch_bounds__(kThreads, 8) norm_rope_kernel(const RowArgs a)
     ok = ok && row >= 0 && row < pool.rows;
     cache_row = ok ? (size_t)row * a.n_kv * cache_len + at : 0;
   }
+  const int first = quad % a.quads + blockIdx.y * a.quads * a.rows_per;
   if (!ok) {
-    if (threadIdx.x == 0 && blockIdx.y == 0) set_status(a.status, PS_ERR_BAD_INDEX);
+    if (first == 0 && q4 == 0) set_status(a.status, PS_ERR_BAD_INDEX);
     return;
   }
-  const int r0 = blockIdx.y * (kHalfWarps * a.rows_per) + hw;
+  const int last = min(total, (int)(blockIdx.y + 1) * a.quads * a.rows_per);
   const T* qj = (const T*)a.q + (size_t)j * a.q_stride;
   const T* kj = (const T*)a.k + (size_t)j * a.k_stride;
   const T* vj = kAppend ? (const T*)a.v + (size_t)j * a.v_stride : nullptr;
-  auto load = [&](int r) {  // this lane's 16 bytes of row r (zeros behind the last)
-    Vec8 x = {{0u, 0u, 0u, 0u}};
-    if (r < total) {
-      const T* src = r < nq ? qj + r * kD
-                            : (r < nq + a.n_kv ? kj + (r - nq) * kD : vj + (r - nq - a.n_kv) * kD);
-      x = reinterpret_cast<const Vec8*>(src)[lane];
-    }
-    return x;
+  auto source = [&](int r) {
+    return reinterpret_cast<const Vec8*>(
+        r < nq ? qj + r * kD : (r < nq + a.n_kv ? kj + (r - nq) * kD : vj + (r - nq - a.n_kv) * kD));
   };
-  Vec8 next = load(r0), after = load(r0 + kHalfWarps);  // two rows ahead
-  // cos / sin of this lane's channels: half layout channel i < rotary/2 pairs
-  // with i + rotary/2; interleaved pairs are (2i, 2i + 1)
-  const int half = a.rotary >> 1;
-  const bool turned = a.rc && 8 * lane < a.rotary;
-  const int pair0 = a.interleaved ? 4 * lane : (8 * lane < half ? 8 * lane : 8 * lane - half);
-  float co[8] = {}, si[8] = {};
-  if (turned) {
-    const float* rc = a.rc + (size_t)p * half + pair0;
-    const float* rs = a.rs + (size_t)p * half + pair0;
-    const int n4 = a.interleaved ? 1 : 2;
+  const int chunk[4] = {2 * q4, 2 * q4 + 1, 2 * q4 + 8, 2 * q4 + 9};
+  Vec8 next[4] = {};
+  if (first < last) {
+    const Vec8* src = source(first);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      if (i < n4) {
-        const float4 c4 = reinterpret_cast<const float4*>(rc)[i];
-        const float4 s4 = reinterpret_cast<const float4*>(rs)[i];
-        co[4 * i] = c4.x, co[4 * i + 1] = c4.y, co[4 * i + 2] = c4.z, co[4 * i + 3] = c4.w;
-        si[4 * i] = s4.x, si[4 * i + 1] = s4.y, si[4 * i + 2] = s4.z, si[4 * i + 3] = s4.w;
-      }
-    }
+    for (int i = 0; i < 4; ++i) next[i] = src[chunk[i]];
   }
-  const bool upper = 8 * lane >= half;  // the second element of its half-layout pairs
-  const int partner = turned ? (upper ? lane - half / 8 : lane + half / 8) : lane;
-  if (!a.interleaved && !upper) {
+  // cos / sin of this lane's 16 pairs: kWhole, channels 16 q4 + 0 .. 15 and the ones 64
+  // above; kInterleaved, 4 of each chunk (cos 1, sin 0 behind the rotary part)
+  float co[16], si[16];
+  const int half = a.rotary >> 1;
+  if (kRot == kWhole || kRot == kInterleaved) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) si[i] = -si[i];
+    for (int i = 0; i < 4; ++i) {
+      const int at = kRot == kWhole ? 16 * q4 + 4 * i : 4 * chunk[i];
+      float4 c4 = make_float4(1.f, 1.f, 1.f, 1.f), s4 = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (at < half) {
+        c4 = *reinterpret_cast<const float4*>(a.rc + (size_t)p * half + at);
+        s4 = *reinterpret_cast<const float4*>(a.rs + (size_t)p * half + at);
+      }
+      co[4 * i] = c4.x, co[4 * i + 1] = c4.y, co[4 * i + 2] = c4.z, co[4 * i + 3] = c4.w;
+      si[4 * i] = s4.x, si[4 * i + 1] = s4.y, si[4 * i + 2] = s4.z, si[4 * i + 3] = s4.w;
+    }
   }
 
 #pragma unroll 1
-  for (int u = 0; u < a.rows_per; ++u) {
-    const int r = r0 + u * kHalfWarps;
-    if (r >= total) break;  // the same for the whole half warp
-    const Vec8 in = next;
-    next = after;
-    if (u + 2 < a.rows_per) after = load(r + 2 * kHalfWarps);
+  for (int r = first; r < last; r += a.quads) {
+    const Vec8* src = source(r);
+    float x[4][8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) unpack8<T>(next[i], x[i]);
+    if (r + a.quads < last) {  // one row ahead
+      const Vec8* ahead = source(r + a.quads);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) next[i] = ahead[chunk[i]];
+    }
     const bool is_q = r < nq, is_v = r >= nq + a.n_kv;
-    float x[8];
-    unpack8<T>(in, x);
     const T* w = (const T*)(is_q ? a.q_w : a.k_w);
+    float rstd = 1.f;
     if (!is_v && w) {
       float ss = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) ss += x[i] * x[i];
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int o = 8; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
-      const float rstd = rsqrtf(ss * (1.f / kD) + a.eps);
-      float g[8];
-      unpack8<T>(reinterpret_cast<const Vec8*>(w + m * kD)[lane], g);
+        for (int c = 0; c < 8; ++c) ss += x[i][c] * x[i][c];
+      ss += __shfl_xor_sync(mask, ss, 1);
+      ss += __shfl_xor_sync(mask, ss, 2);
+      rstd = rsqrtf(ss * (1.f / kD) + a.eps);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = x[i] * rstd * g[i];
-    }
-    if (!is_v && a.rc) {
-      if (a.interleaved) {
-        if (turned) {
+      for (int i = 0; i < 4; ++i) {
+        float g[8];
+        unpack8<T>(reinterpret_cast<const Vec8*>(w + m * kD)[chunk[i]], g);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float e = x[2 * i], o = x[2 * i + 1];
-            x[2 * i] = __fsub_rn(__fmul_rn(e, co[i]), __fmul_rn(o, si[i]));
-            x[2 * i + 1] = __fadd_rn(__fmul_rn(o, co[i]), __fmul_rn(e, si[i]));
-          }
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float y = __shfl_sync(mask, x[i], partner, 16);
-          // si is - sin in the first elements of the pairs; the two products are
-          // rounded each (a packed mul and add would be contracted to one fma)
-          if (turned) x[i] = __fadd_rn(__fmul_rn(x[i], co[i]), __fmul_rn(y, si[i]));
-        }
+        for (int c = 0; c < 8; ++c) x[i][c] = x[i][c] * rstd * g[c];
       }
     }
-    if (is_q) {
-      T* dst = (T*)a.q_out + (size_t)j * a.qo_stride + r * kD;
-      reinterpret_cast<Vec8*>(dst)[lane] = pack8<T>(x);
-    } else if (!kAppend) {
-      T* dst = (T*)a.k_out + (size_t)j * a.ko_stride + (r - nq) * kD;
-      reinterpret_cast<Vec8*>(dst)[lane] = pack8<T>(x);
+    if (kRot != kNone && !is_v) {
+      // products and sums are rounded each
+      if (kRot == kWhole) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            const float e = x[i][c], o = x[i + 2][c], cc = co[8 * i + c], sn = si[8 * i + c];
+            x[i][c] = __fsub_rn(__fmul_rn(e, cc), __fmul_rn(o, sn));
+            x[i + 2][c] = __fadd_rn(__fmul_rn(o, cc), __fmul_rn(e, sn));
+          }
+      } else if (kRot == kInterleaved) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (4 * chunk[i] < half) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const float e = x[i][2 * c], o = x[i][2 * c + 1];
+              const float cc = co[4 * i + c], sn = si[4 * i + c];
+              x[i][2 * c] = __fsub_rn(__fmul_rn(e, cc), __fmul_rn(o, sn));
+              x[i][2 * c + 1] = __fadd_rn(__fmul_rn(o, cc), __fmul_rn(e, sn));
+            }
+          }
+      } else {
+        // pairs (i, i + half) of different lanes: the other channel is read again
+        // (a multiple of 8 away, so a whole chunk), before anything is written
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int ch = 8 * chunk[i];
+          if (ch < 2 * half) {
+            const bool up = ch >= half;
+            const int other = up ? chunk[i] - half / 8 : chunk[i] + half / 8;
+            float y[8];
+            unpack8<T>(src[other], y);
+            if (w) {
+              float g[8];
+              unpack8<T>(reinterpret_cast<const Vec8*>(w + m * kD)[other], g);
+#pragma unroll
+              for (int c = 0; c < 8; ++c) y[c] = y[c] * rstd * g[c];
+            }
+            const float* rc = a.rc + (size_t)p * half + (up ? ch - half : ch);
+            const float* rs = a.rs + (size_t)p * half + (up ? ch - half : ch);
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+              const float b = __fmul_rn(y[c], rs[c]);
+              x[i][c] = __fadd_rn(__fmul_rn(x[i][c], rc[c]), up ? b : -b);
+            }
+          }
+        }
+        __syncwarp(mask);
+      }
+    }
+    if (is_q || !kAppend) {
+      Vec8* dst = reinterpret_cast<Vec8*>(is_q ? (T*)a.q_out + (size_t)j * a.qo_stride + r * kD
+                                               : (T*)a.k_out + (size_t)j * a.ko_stride +
+                                                     (r - nq) * kD);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) dst[chunk[i]] = pack8<T>(x[i]);
     } else {
+      // groups q4 / 2 (chunks 0, 1) and q4 / 2 + 2 (chunks 2, 3): words 2 (q4 & 1)
+      // and the next of each
+      uint32_t lo[2], hi[2], mlo, mhi;
+      quantise_group<T>(x[0], x[1], mask, lo, mlo);
+      quantise_group<T>(x[2], x[3], mask, hi, mhi);
+      // 16 stored bytes hold one word of every group: exchange with the lane of
+      // the two other groups
+      const bool up = q4 >> 1;
+      const uint32_t r0 = __shfl_xor_sync(mask, up ? lo[0] : lo[1], 2);
+      const uint32_t r1 = __shfl_xor_sync(mask, up ? hi[0] : hi[1], 2);
       const int h = is_v ? r - nq - a.n_kv : r - nq;
       const size_t row = cache_row + (size_t)h * cache_len;
-      store_row4<T>(x, lane, mask, (is_v ? pool.v_codes : pool.k_codes) + row * kCodeBytes,
-                    (is_v ? pool.v_meta : pool.k_meta) + row * kMetaBytes);
+      uint8_t* codes = (is_v ? pool.v_codes : pool.k_codes) + row * kCodeBytes;
+      uint8_t* meta = (is_v ? pool.v_meta : pool.k_meta) + row * kMetaBytes;
+      reinterpret_cast<uint4*>(codes)[2 * (q4 & 1) + (up ? 1 : 0)] =
+          up ? make_uint4(r0, lo[1], r1, hi[1]) : make_uint4(lo[0], r0, hi[0], r1);
+      if (!(q4 & 1)) {
+        reinterpret_cast<uint32_t*>(meta)[q4 >> 1] = mlo;
+        reinterpret_cast<uint32_t*>(meta)[(q4 >> 1) + 2] = mhi;
+      }
     }
   }
 }
 
 // Read-back: output row r of sequence i (cu[i] <= r < cu[i+1]) is position
-// seqs[i].first + (r - cu[i]). grid (ceil(total / 32), n_kv), 8 half warps with
-// 4 rows each, whose loads are all issued before the first is used.
+// seqs[i].first + (r - cu[i]). grid (ceil(total / 16), n_kv), 8 half warps with
+// kRows rows each, whose loads are all issued before the first is used.
 struct GatherArgs {
   Pool pool[2];
   const int32_t* seqs;  // [n][3]: model, slot or block-table row, first position
@@ -432,24 +489,31 @@ bool valid_cache(const ps_kv4_cache_t* c) {
   return c->L_cap > 0 && c->L_cap <= (1 << 30);
 }
 
-// Rows of a half warp: what a token's rows come to in as few blocks as hold at
-// most 6 each (its setup, a table row of cos and sin among it, is shared by them);
-// fewer when the tokens alone do not fill the GPU.
-static int rows_per_half_warp(int M, int total, int device) {
-  const int most = M >= 4 * sm_count(device) ? 6 : 2;
-  const int blocks = cdiv(total, kHalfWarps * most);
-  return cdiv(total, kHalfWarps * blocks);
+template <typename T, bool kAppend>
+static cudaError_t launch_rotation(const RowArgs& a, dim3 grid, cudaStream_t st) {
+  if (!a.rc) return launch(norm_rope_kernel<T, kAppend, kNone>, grid, dim3(kThreads), 0, st, a);
+  if (a.interleaved)
+    return launch(norm_rope_kernel<T, kAppend, kInterleaved>, grid, dim3(kThreads), 0, st, a);
+  if (a.rotary == kD)
+    return launch(norm_rope_kernel<T, kAppend, kWhole>, grid, dim3(kThreads), 0, st, a);
+  return launch(norm_rope_kernel<T, kAppend, kPart>, grid, dim3(kThreads), 0, st, a);
 }
 
+// How a token's rows are cut: enough quads that each has at most 12 rows (their
+// setup, cos and sin among it, is shared by them); one row each, over several
+// blocks, when the tokens alone do not fill the GPU.
 template <bool kAppend>
 static int launch_rows(RowArgs& a, int dtype, cudaStream_t st) {
   const int total = (a.q ? a.n_heads : 0) + (kAppend ? 2 : 1) * a.n_kv;
-  a.rows_per = rows_per_half_warp(a.M, total, current_device());
-  const dim3 grid(a.M, cdiv(total, kHalfWarps * a.rows_per));
-  if (dtype == PS_DTYPE_BF16)
-    PS_CUDA_RET(launch(norm_rope_kernel<__nv_bfloat16, kAppend>, grid, dim3(kThreads), 0, st, a));
-  else
-    PS_CUDA_RET(launch(norm_rope_kernel<__half, kAppend>, grid, dim3(kThreads), 0, st, a));
+  const bool many = a.M >= 4 * sm_count(current_device());
+  const int most = many ? 12 : 1;
+  a.quads = 1;
+  while (a.quads < kQuads && a.quads * most < total) a.quads *= 2;
+  const int blocks = cdiv(total, a.quads * most);
+  a.rows_per = cdiv(total, a.quads * blocks);
+  const dim3 grid(cdiv(a.M, kQuads / a.quads), blocks);
+  PS_CUDA_RET((dtype == PS_DTYPE_BF16 ? launch_rotation<__nv_bfloat16, kAppend>(a, grid, st)
+                                      : launch_rotation<__half, kAppend>(a, grid, st)));
   return PS_OK;
 }
 
