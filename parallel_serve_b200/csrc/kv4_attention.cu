@@ -52,6 +52,7 @@ constexpr int kWarpPos = 32;                 // positions of a tile per compute 
 constexpr int kTile = kWarps * kWarpPos;     // 128
 constexpr int kStages = 2;
 constexpr int kCtasPerSm = 3;
+constexpr int kSmallPage = 32;               // positions
 constexpr int kAttnThreads = (kWarps + 1) * 32;
 constexpr int kTileCodes = kTile * kCodeBytes;
 constexpr int kTileMeta = kTile * kMetaBytes;
@@ -121,6 +122,16 @@ PS_DEV float exp2_ftz(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+PS_DEV void cp_async16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src)
+               : "memory");
+}
+// One of the barrier's arrivals, when this thread's copies above have landed.
+PS_DEV void cp_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar))
+               : "memory");
 }
 
 PS_DEV uint32_t transpose8x8(uint32_t v) {
@@ -227,6 +238,12 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm)
   pdl_launch_dependents();
   const int c0 = a.counts ? a.counts[0] : a.split_point;
 
+  // With short pages the (s, z) rows come by 16-byte copies of the producer's lanes:
+  // half as many bulk copies, whose number a tile then waits for (pages of 16: 299 and
+  // 280 us for 96 ragged sequences; pages of 64: 170 with bulk copies, 174 with these;
+  // the codes by 16-byte copies too: 332).
+  const bool small_pages = a.block_table && a.page_size <= kSmallPage;
+
   // Tiles per entry of tokens, then their prefix sums.
   const int entries = (a.M + a.per_entry - 1) / a.per_entry;
   for (int e = tid; e < entries; e += kAttnThreads) {
@@ -241,7 +258,7 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm)
   if (tid == 0) {
     P[0] = 0;
     for (int i = 0; i < kStages; ++i) {
-      mbar_init(full + i, 1);
+      mbar_init(full + i, small_pages ? 33 : 1);
       mbar_init(empty + i, kWarps);
     }
     abort_flag[0] = 0;
@@ -327,7 +344,8 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm)
           if (lane == 0) {
             if (any_bad) set_status(a.status, PS_ERR_BAD_INDEX);
             stage_bad[st] = any_bad ? 1 : 0;
-            mbar_arrive_expect_tx(full + st, (uint32_t)npos * 2 * (kCodeBytes + kMetaBytes));
+            mbar_arrive_expect_tx(full + st, (uint32_t)npos * 2 *
+                                                 (kCodeBytes + (small_pages ? 0 : kMetaBytes)));
           }
           __syncwarp();
           if (lane < nrun) {
@@ -337,12 +355,28 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm)
                                ((pos0 + o) & (a.page_size - 1));
             bulk_load(buf + o * kCodeBytes, pool.k_codes + row * kCodeBytes, n * kCodeBytes,
                       full + st, pol);
-            bulk_load(buf + kTileCodes + o * kMetaBytes, pool.k_meta + row * kMetaBytes,
-                      n * kMetaBytes, full + st, pol);
             bulk_load(buf + kTileCodes + kTileMeta + o * kCodeBytes,
                       pool.v_codes + row * kCodeBytes, n * kCodeBytes, full + st, pol);
-            bulk_load(buf + 2 * kTileCodes + kTileMeta + o * kMetaBytes,
-                      pool.v_meta + row * kMetaBytes, n * kMetaBytes, full + st, pol);
+            if (!small_pages) {
+              bulk_load(buf + kTileCodes + o * kMetaBytes, pool.k_meta + row * kMetaBytes,
+                        n * kMetaBytes, full + st, pol);
+              bulk_load(buf + 2 * kTileCodes + kTileMeta + o * kMetaBytes,
+                        pool.v_meta + row * kMetaBytes, n * kMetaBytes, full + st, pol);
+            }
+          }
+          if (small_pages) {
+#pragma unroll
+            for (int i = 0; i < kTile / 32; ++i) {
+              const int o = lane + 32 * i;
+              const int pg = __shfl_sync(0xffffffffu, page, o >> a.page_shift);
+              if (o < npos) {
+                const size_t at = (((size_t)pg * a.n_kv + pc.kvh) * a.page_size +
+                                   ((pos0 + o) & (a.page_size - 1))) * kMetaBytes;
+                cp_async16(buf + kTileCodes + o * kMetaBytes, pool.k_meta + at);
+                cp_async16(buf + 2 * kTileCodes + kTileMeta + o * kMetaBytes, pool.v_meta + at);
+              }
+            }
+            cp_async_arrive(full + st);
           }
         }
       }
