@@ -6,22 +6,29 @@
 //   over the keys k <= i + (keys - queries) of i's sequence
 //
 // Two matrix products of 4 * 128 flops per visible pair bound it, so the tensor
-// core must never wait. One CTA per SM works on 256 queries of one (sequence,
-// head) as two tiles of 128 that take turns: while one tile's scores are in
-// softmax, the other's products run.
-//   warps 0-3, 4-7  softmax of tile 0 / 1, one thread per query row: S (128 keys) goes
+// core must never wait for long: an SM works on two tiles of 128 queries that take
+// turns, and while one tile's scores are in softmax the other's products run. The
+// two are one CTA's (256 queries of one (sequence, head), long prompts) or two
+// CTAs' (short ones). Warps of a CTA:
+//   4 per tile      softmax, one thread per query row: S (128 keys) goes
 //                   TMEM -> registers in chunks, P goes back in 16 bits over S's
 //                   own columns, in two halves of 64 keys, so that the first half
 //                   is multiplied while the second is still in softmax. P never
 //                   touches shared memory.
-//   warp 8          TMA: Q, then K and V blocks of 128 keys through a 5-slot ring
-//   warp 9          MMA issue, per block and tile: O += P V for both halves, then the
+//   next            TMA: Q, then K and V blocks of 128 keys through a ring
+//   last            MMA issue, per block and tile: O += P V for both halves, then the
 //                   next S = Q K^T over the columns that P leaves. Products of
 //                   one warp run in order, so no barrier says that.
-// TMEM (512 columns): S0 S1 (128 fp32 columns each), O0 O1.
-// Steps of 64 keys with two S buffers per tile were measured too (2.16 ms where this
-// takes SHORTER): a 128 x 64 product reads 6 KB of shared memory in 32 cycles' work
-// and so runs at two thirds of the rate.
+// TMEM: S, 128 fp32 columns a tile, then O, 128 a tile.
+//
+// 16384 tokens, 32 + 8 heads: 1.98 ms, 1.11 PFLOP/s. Of the 3500 cycles of a block
+// of both tiles products take 2050, and at 1 kW the SM clock is at 1.55 GHz, so what
+// shortens the cycles without saving energy gains nothing. Measured and not kept:
+//   P by polynomial on the FMA pipe for a quarter of the keys, scores prefetched
+//   across P's halves: 3380 cycles at 1.52 GHz, 2.00 ms
+//   an issuing warp for each tile of a CTA: the tiles fall into step, 2.30 ms
+//   steps of 64 keys with two S buffers per tile: 2.16 ms, since a 128 x 64 product
+//   reads 6 KB of shared memory in 32 cycles' work
 //
 // P = 2^(s - m) needs no exact maximum, only one reference m for P, the row sum and
 // O that keeps P within 16 bits: m is the row's maximum over its first block and
@@ -47,16 +54,20 @@ namespace pra {
 
 constexpr int kD = 128;
 constexpr int kTile = 128;              // queries of a tile, keys of a block
-constexpr int kTiles = 2;               // tiles of a CTA
-constexpr int kRows = kTile * kTiles;   // queries of a CTA
 constexpr int kTileBytes = kTile * kD * 2;
 constexpr int kHalf = kTileBytes / 2;   // one 64-column TMA box (128 rows x 128 bytes)
 constexpr int kKeys = 64;               // keys of half a block
-constexpr int kSlots = 5;
-constexpr int kThreads = 320;
-constexpr int kSmem = 1024 + kTileBytes * (kTiles + kSlots) + 256;
-constexpr int kTmemCols = 512;
-constexpr int kTmemO = 256;             // S tiles at 0, 128; O tiles at 256, 384
+// What a CTA is made of: kTiles tiles of queries.
+template <int kTiles>
+struct Shape {
+  static constexpr int kRows = kTile * kTiles;           // queries
+  static constexpr int kSlots = kTiles == 2 ? 5 : 2;     // of the K / V ring
+  static constexpr int kThreads = (kTiles * 4 + 2) * 32;
+  static constexpr int kCtas = 3 - kTiles;               // resident on an SM
+  static constexpr int kSmem = 1024 + kTileBytes * (kTiles + kSlots) + 256;
+  static constexpr int kTmemCols = 256 * kTiles;
+  static constexpr int kTmemO = 128 * kTiles;            // S tiles from 0, O tiles from here
+};
 constexpr float kMaxSum = 256.f;        // of 64 P, before the reference moves
 
 struct Args {
@@ -265,14 +276,14 @@ PS_DEV bool finite8(const uint4& u) {
   return fin;
 }
 
-// Sequence i owns CTA slots [cu_q[i] / 256 + i, cu_q[i + 1] / 256 + i + 1): at
+// With R queries to a CTA, sequence i owns slots [cu_q[i] / R + i, cu_q[i + 1] / R + i + 1): at
 // least as many as it has tiles, found by a binary search, no scan of lengths.
 struct Item {
   int q0, k0, lq, lk, row;  // first rows, lengths, first query of this CTA
   bool live;
 };
 
-PS_DEV Item item_at(const Args& a, int slot) {
+PS_DEV Item item_at(const Args& a, int slot, int kRows) {
   int lo = 0, hi = a.n - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
@@ -302,11 +313,13 @@ PS_DEV int blocks_of(const Item& it, int t) {
   return keys > 0 ? (keys + kTile - 1) / kTile : 0;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads, 1)
+template <typename T, int kTiles>
+__global__ void __launch_bounds__(Shape<kTiles>::kThreads, Shape<kTiles>::kCtas)
     prompt_attention_kernel(const __grid_constant__ CUtensorMap tq,
                             const __grid_constant__ CUtensorMap tk,
                             const __grid_constant__ CUtensorMap tv, const Args a) {
+  constexpr int kSlots = Shape<kTiles>::kSlots, kTmemO = Shape<kTiles>::kTmemO;
+  constexpr int kTma = 4 * kTiles, kMma = kTma + 1;  // warps
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t pad = (1024 - (smem_u32(smem_raw) & 1023)) & 1023;
   uint8_t* sQ = smem_raw + pad;             // [2] tiles
@@ -342,8 +355,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     poison[0] = 0x7fffffff;
     fence_mbar_init();
   }
-  if (warp == 9) {
-    tmem_alloc(tmem_slot, kTmemCols);
+  if (warp == kMma) {
+    tmem_alloc(tmem_slot, Shape<kTiles>::kTmemCols);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -354,14 +367,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_launch_dependents();
 
   const int h = blockIdx.x % a.n_heads;
-  const Item it = item_at(a, blockIdx.x / a.n_heads);
+  const Item it = item_at(a, blockIdx.x / a.n_heads, Shape<kTiles>::kRows);
   const int nb0 = (int)uniform(it.live ? blocks_of(it, 0) : 0);
-  const int nb1 = (int)uniform(it.live ? blocks_of(it, 1) : 0);
+  const int nb1 = (int)uniform(it.live && kTiles > 1 ? blocks_of(it, 1) : 0);
   const int nb = max(nb0, nb1);
 
-  if (warp >= 8) {
+  if (warp >= kTma) {
     // ------------------------------------------------------------- producer
-    if (warp == 8 && lane == 0 && nb > 0) {
+    if (warp == kTma && lane == 0 && nb > 0) {
       const uint64_t pol = l2_policy_evict_last();  // a head's K / V serve all its tiles
       for (int t = 0; t < kTiles; ++t) {
         if ((t ? nb1 : nb0) == 0) continue;
@@ -393,7 +406,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     // ------------------------------------------------------------------ MMA
-    if (warp == 9 && nb > 0) {
+    if (warp == kMma && nb > 0) {
       const uint32_t idesc_s = idesc_f16(a.bf16, 0, 0, kTile, kTile);  // Q, K both K-major
       const uint32_t idesc_o = idesc_f16(a.bf16, 0, 1, kTile, kD);     // P K-major, V MN-major
       const uint64_t q_desc = smem_desc_sw128(smem_u32(sQ), 16, 1024);
@@ -442,8 +455,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         mma_commit(kv_empty_a);
       }
       // block j: V in slot vs, and the next block's K in slot ks
-      int vs = 1, ks = 2;
-      uint32_t vph = 0, kph = 0;
+      int vs = 1, ks = 2 % kSlots;
+      uint32_t vph = 0, kph = 2 / kSlots;
 #pragma unroll 1
       for (int j = 0; ok && j < nb; ++j) {
         wait(kv_full_a + 8 * vs, vph);
@@ -480,7 +493,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     // -------------------------------------------------------------- softmax
-    const int t = warp >> 2;
+    const int t = kTiles > 1 ? warp >> 2 : 0;
     const int r = (warp & 3) * 32 + lane;  // TMEM lane = row of the tile
     const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
       const uint32_t o_addr = tmem + kTmemO + t * kD + lane_off;
@@ -613,9 +626,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   tc_fence_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == kMma) {
     tc_fence_after();
-    tmem_dealloc(tmem, kTmemCols);
+    tmem_dealloc(tmem, Shape<kTiles>::kTmemCols);
   }
 }
 
@@ -641,7 +654,15 @@ extern "C" int ps_prompt_attention(const void* q, long long q_stride, const void
                o_stride >= (long long)n_heads * pra::kD && o_stride % 8 == 0);
   PS_CHECK_ARG(Tk == 0 || (k_stride >= (long long)n_kv_heads * pra::kD && k_stride % 8 == 0 &&
                            v_stride >= (long long)n_kv_heads * pra::kD && v_stride % 8 == 0));
-  const long long grid = ((long long)Tq / pra::kRows + n_seqs) * n_heads;
+  // By the mean length, which is what the host knows: two CTAs of one tile on an SM
+  // (128 queries each) waste less of a short sequence and hide each other's start
+  // (64 prompts of 64 to 128 tokens, 32 + 8 heads: 71 us, one CTA of two tiles 118; 8 of
+  // 512 to 1024: 86 and 101); two tiles read each K and V block once for twice the
+  // queries, which wins behind some 4096 (one prompt of 4096: 138 and 140 us, of 8192:
+  // 547 and 515, of 16384: 2084 and 1976).
+  const bool one = Tk < 4096ll * n_seqs;
+  const int rows = pra::kTile * (one ? 1 : 2);
+  const long long grid = ((long long)Tq / rows + n_seqs) * n_heads;
   if (grid > 0x7fffffffll || Tk > (1 << 30) || Tq > (1 << 30)) return PS_ERR_UNSUPPORTED;
   const int device = current_device();
   if (!is_sm100(device)) return PS_ERR_UNSUPPORTED;
@@ -673,14 +694,16 @@ extern "C" int ps_prompt_attention(const void* q, long long q_stride, const void
   a.scale_log2 = scale * 1.4426950408889634f;
   a.status = status;
   cudaStream_t st = (cudaStream_t)stream;
-  if (bf) {
-    PS_CUDA_RET(allow_dynamic_smem(pra::prompt_attention_kernel<__nv_bfloat16>, pra::kSmem));
-    PS_CUDA_RET(launch(pra::prompt_attention_kernel<__nv_bfloat16>, dim3((unsigned)grid),
-                       dim3(pra::kThreads), pra::kSmem, st, tq, tk, tv, a));
-  } else {
-    PS_CUDA_RET(allow_dynamic_smem(pra::prompt_attention_kernel<__half>, pra::kSmem));
-    PS_CUDA_RET(launch(pra::prompt_attention_kernel<__half>, dim3((unsigned)grid),
-                       dim3(pra::kThreads), pra::kSmem, st, tq, tk, tv, a));
-  }
-  return PS_OK;
+  auto run = [&](auto kernel, int threads, int smem) -> int {
+    PS_CUDA_RET(allow_dynamic_smem(kernel, smem));
+    PS_CUDA_RET(launch(kernel, dim3((unsigned)grid), dim3(threads), smem, st, tq, tk, tv, a));
+    return PS_OK;
+  };
+  using One = pra::Shape<1>;
+  using Two = pra::Shape<2>;
+  if (one)
+    return bf ? run(pra::prompt_attention_kernel<__nv_bfloat16, 1>, One::kThreads, One::kSmem)
+              : run(pra::prompt_attention_kernel<__half, 1>, One::kThreads, One::kSmem);
+  return bf ? run(pra::prompt_attention_kernel<__nv_bfloat16, 2>, Two::kThreads, Two::kSmem)
+            : run(pra::prompt_attention_kernel<__half, 2>, Two::kThreads, Two::kSmem);
 }

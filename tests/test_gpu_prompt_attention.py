@@ -168,3 +168,50 @@ def test_non_finite_values_reach_their_queries_only(dt):
         assert torch.equal(out[:key], want[:key]), key
         assert not torch.isfinite(out.view(400, nh, 128)[key:, :, 77]).any()
     assert _status() == 0
+
+
+# Long mean lengths (4096 keys and more) take CTAs of two tiles.
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_long_histories(dt):
+    lens = [5, 130, 1, 300]
+    _run(lens, [n + h for n, h in zip(lens, [5000, 4100, 3900, 4096])], 4, 2, dt, 71, heads=[0, 3])
+    _run([257, 0], [4099, 4200], 2, 1, dt, 73, scale=1.0)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("lens,klens", [([1], [1]), ([128], [128]), ([129], [129]), ([256], [256]),
+                                        ([300, 0, 513], [300, 0, 513]), ([300, 20, 7], [10, 20, 0]),
+                                        ([40, 300, 100], [40, 290, 229])])
+def test_two_tiles_of_short_sequences(dt, lens, klens):
+    """Rows of NaN behind the last key make the mean length long."""
+    from parallel_serve_b200 import ops
+    nh, nkv, T = 2, 1, 4096 * len(lens) + 64
+    q = cpu_randn((sum(lens), nh, 128), 81, 1.0, dt)
+    k, v = (torch.full((T, nkv, 128), float("nan"), dtype=dt) for _ in range(2))
+    k[:sum(klens)] = cpu_randn((sum(klens), nkv, 128), 82, 1.0, dt)
+    v[:sum(klens)] = cpu_randn((sum(klens), nkv, 128), 83, 1.0, dt)
+    out = ops.prompt_attention(q.to(DEV), k.to(DEV), v.to(DEV), _cu(lens), _cu(klens))
+    assert _status() == 0
+    _check(out, q, k[:sum(klens)], v[:sum(klens)], lens, klens, dt)
+
+
+def test_two_tiles_and_non_finite_values():
+    from parallel_serve_b200 import ops
+    dt, nh, nkv, n = torch.float16, 2, 1, 400
+    q, k, v = (cpu_randn((m, h, 128), 91 + i, 1.0, dt).to(DEV)
+               for i, (m, h) in enumerate(((n, nh), (4200, nkv), (4200, nkv))))
+    cu = _cu([n])
+    want = ops.prompt_attention(q, k, v, cu, cu)
+    for key in (0, 127, 128, 200, 256, 399):
+        bad = v.clone()
+        bad[key, 0, 77] = float("nan") if key & 1 else float("inf")
+        out = ops.prompt_attention(q, k, bad, cu, cu)
+        assert torch.equal(out[:key], want[:key]), key
+        assert not torch.isfinite(out.view(n, nh, 128)[key:, :, 77]).any()
+        bad = k.clone()
+        bad[key, 0, 5] = float("nan")
+        out = ops.prompt_attention(q, bad, v, cu, cu)
+        assert torch.equal(out[:key], want[:key]), key
+        assert torch.isnan(out[key:]).all()
+    assert _status() == 0
