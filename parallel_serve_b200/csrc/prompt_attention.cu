@@ -277,17 +277,22 @@ PS_DEV bool finite8(const uint4& u) {
 }
 
 // With R queries to a CTA, sequence i owns slots [cu_q[i] / R + i, cu_q[i + 1] / R + i + 1): at
-// least as many as it has tiles, found by a binary search, no scan of lengths.
+// least as many as it has tiles, found by a search, no scan of lengths (every lane of a warp
+// calls it).
 struct Item {
   int q0, k0, lq, lk, row;  // first rows, lengths, first query of this CTA
   bool live;
 };
 
 PS_DEV Item item_at(const Args& a, int slot, int kRows) {
-  int lo = 0, hi = a.n - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (a.cu_q[mid] / kRows + mid <= slot) lo = mid; else hi = mid - 1;
+  const int lane = threadIdx.x & 31;
+  int lo = 0, count = a.n;  // the last i of [lo, lo + count) whose slots begin by `slot`
+  while (count > 1) {       // 32 of them looked at together: the loads are what takes time
+    const int step = (count + 31) / 32, i = lo + lane * step;
+    const bool le = lane == 0 || (lane * step < count && a.cu_q[i] / kRows + i <= slot);
+    const int last = 31 - __clz((int)__ballot_sync(0xffffffffu, le));
+    lo += last * step;
+    count = min(step, count - last * step);
   }
   Item it;
   it.q0 = a.cu_q[lo];
@@ -338,7 +343,12 @@ __global__ void __launch_bounds__(Shape<kTiles>::kThreads, Shape<kTiles>::kCtas)
   int* poison = reinterpret_cast<int*>(tmem_slot + 2);  // first cleared key that was not finite
 
   const int warp = (int)uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (threadIdx.x == 0) {
+  const bool producer = warp == kTma && lane == 0;
+  if (warp == kMma) {
+    tmem_alloc(tmem_slot, Shape<kTiles>::kTmemCols);
+    tmem_relinquish();
+  }
+  if (producer) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(q_full + i, 1);
       mbar_init(s_full + i, 1);
@@ -355,14 +365,7 @@ __global__ void __launch_bounds__(Shape<kTiles>::kThreads, Shape<kTiles>::kCtas)
     poison[0] = 0x7fffffff;
     fence_mbar_init();
   }
-  if (warp == kMma) {
-    tmem_alloc(tmem_slot, Shape<kTiles>::kTmemCols);
-    tmem_relinquish();
-  }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = uniform(*tmem_slot);
+  __syncwarp();
   pdl_wait();
   pdl_launch_dependents();
 
@@ -372,31 +375,44 @@ __global__ void __launch_bounds__(Shape<kTiles>::kThreads, Shape<kTiles>::kCtas)
   const int nb1 = (int)uniform(it.live && kTiles > 1 ? blocks_of(it, 1) : 0);
   const int nb = max(nb0, nb1);
 
+  // Key or value block of ring item i: K0 V0 K1 V1 ...
+  const uint64_t pol = l2_policy_evict_last();  // a head's K / V serve all its tiles
+  auto load_kv = [&](int i) {
+    const int st = i % kSlots, c = (h / a.group) * kD;
+    const CUtensorMap* tm = i & 1 ? &tv : &tk;
+    const int r = it.k0 + (i >> 1) * kTile;
+    uint8_t* dst = sKV + st * kTileBytes;
+    mbar_arrive_expect_tx(kv_full + st, kTileBytes);
+    tma_load_2d(dst, tm, kv_full + st, c, r, pol);
+    tma_load_2d(dst + kHalf, tm, kv_full + st, c + 64, r, pol);
+  };
+  // What the first products need is on its way before the warps meet and TMEM is known
+  if (producer && nb > 0) {
+    load_kv(0);
+    for (int t = 0; t < kTiles; ++t) {
+      if ((t ? nb1 : nb0) == 0) continue;
+      mbar_arrive_expect_tx(q_full + t, kTileBytes);
+      const int r = it.q0 + it.row + t * kTile;
+      tma_load_2d(sQ + t * kTileBytes, &tq, q_full + t, h * kD, r, pol);
+      tma_load_2d(sQ + t * kTileBytes + kHalf, &tq, q_full + t, h * kD + 64, r, pol);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = uniform(*tmem_slot);
+
   if (warp >= kTma) {
     // ------------------------------------------------------------- producer
-    if (warp == kTma && lane == 0 && nb > 0) {
-      const uint64_t pol = l2_policy_evict_last();  // a head's K / V serve all its tiles
-      for (int t = 0; t < kTiles; ++t) {
-        if ((t ? nb1 : nb0) == 0) continue;
-        mbar_arrive_expect_tx(q_full + t, kTileBytes);
-        const int r = it.q0 + it.row + t * kTile;
-        tma_load_2d(sQ + t * kTileBytes, &tq, q_full + t, h * kD, r, pol);
-        tma_load_2d(sQ + t * kTileBytes + kHalf, &tq, q_full + t, h * kD + 64, r, pol);
-      }
-      const int kc = (h / a.group) * kD;
-      int i = 0;
+    if (producer && nb > 0) {
+      int i = 1;
       for (; i < 2 * nb; ++i) {
-        const int st = i % kSlots;
-        if (abort_flag[0] || !mbar_wait(kv_empty + st, ((i / kSlots) & 1) ^ 1, a.status)) {
+        if (abort_flag[0] ||
+            !mbar_wait(kv_empty + i % kSlots, ((i / kSlots) & 1) ^ 1, a.status)) {
           abort_flag[0] = 1;
           break;
         }
-        const CUtensorMap* tm = i & 1 ? &tv : &tk;
-        const int r = it.k0 + (i >> 1) * kTile;
-        uint8_t* dst = sKV + st * kTileBytes;
-        mbar_arrive_expect_tx(kv_full + st, kTileBytes);
-        tma_load_2d(dst, tm, kv_full + st, kc, r, pol);
-        tma_load_2d(dst + kHalf, tm, kv_full + st, kc + 64, r, pol);
+        load_kv(i);
       }
       if (abort_flag[0]) {  // let every issued copy land before the CTA exits
         if (nb0) mbar_wait(q_full, 0, a.status);
