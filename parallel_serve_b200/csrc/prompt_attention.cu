@@ -367,7 +367,6 @@ __global__ void __launch_bounds__(Shape<kTiles>::kThreads, Shape<kTiles>::kCtas)
   }
   __syncwarp();
   pdl_wait();
-  pdl_launch_dependents();
 
   const int h = blockIdx.x % a.n_heads;
   const Item it = item_at(a, blockIdx.x / a.n_heads, Shape<kTiles>::kRows);
@@ -401,6 +400,9 @@ __global__ void __launch_bounds__(Shape<kTiles>::kThreads, Shape<kTiles>::kCtas)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = uniform(*tmem_slot);
+  // Not before every CTA has its TMEM: the next kernel's CTAs allocate theirs before they
+  // wait for this grid.
+  pdl_launch_dependents();
 
   if (warp >= kTma) {
     // ------------------------------------------------------------- producer
@@ -672,8 +674,8 @@ extern "C" int ps_prompt_attention(const void* q, long long q_stride, const void
                            v_stride >= (long long)n_kv_heads * pra::kD && v_stride % 8 == 0));
   // By the mean length, which is what the host knows: two CTAs of one tile on an SM
   // (128 queries each) waste less of a short sequence and hide each other's start
-  // (64 prompts of 64 to 128 tokens, 32 + 8 heads: 71 us, one CTA of two tiles 118; 8 of
-  // 512 to 1024: 86 and 101); two tiles read each K and V block once for twice the
+  // (64 prompts of 64 to 128 tokens, 32 + 8 heads: 68 us, one CTA of two tiles 118; 8 of
+  // 512 to 1024: 87 and 101); two tiles read each K and V block once for twice the
   // queries, which wins behind some 4096 (one prompt of 4096: 138 and 140 us, of 8192:
   // 547 and 515, of 16384: 2084 and 1976).
   const bool one = Tk < 4096ll * n_seqs;
