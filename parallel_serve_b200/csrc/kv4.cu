@@ -28,8 +28,6 @@ namespace kv4 {
 
 constexpr int kThreads = 128;
 constexpr int kQuads = kThreads / 4;
-constexpr int kHalfWarps = kThreads / 16;  // the read-back
-constexpr int kRows = 2;                   // rows of one half warp there
 
 struct RowArgs {
   const void* q;  // [M, n_heads, 128], token stride q_stride (elements); nullable
@@ -334,8 +332,11 @@ __global__ void __launch_bounds__(kThreads) norm_rope_kernel(const RowArgs a) {
 }
 
 // Read-back: output row r of sequence i (cu[i] <= r < cu[i+1]) is position
-// seqs[i].first + (r - cu[i]). grid (ceil(total / 16), n_kv), 8 half warps with
-// kRows rows each, whose loads are all issued before the first is used.
+// seqs[i].first + (r - cu[i]). grid (ceil(total / 32), n_kv). Four lanes to a
+// row: lane w reads 16 bytes, word w of every group, for K and for V, and writes the
+// 4 x 8 channels of each that they stand for. (One word a lane, 16 lanes to a row,
+// takes 4 bytes an instruction and its index arithmetic four times over: ALU at 70%,
+// write + read of 16 prompts 382 us; this way 368.)
 struct GatherArgs {
   Pool pool[2];
   const int32_t* seqs;  // [n][3]: model, slot or block-table row, first position
@@ -388,72 +389,46 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads) kv4_gather_kernel(const GatherArgs a) {
   pdl_wait();
   pdl_launch_dependents();
-  const int hw = threadIdx.x >> 4, lane = threadIdx.x & 15;
-  const int h = blockIdx.y;
-  const int base = blockIdx.x * kHalfWarps * kRows + hw;
-  if (base >= a.total) return;
-  int lo = 0, hi = a.n;  // the last i with cu[i] <= base, or n
+  const int w = threadIdx.x & 3, h = blockIdx.y;
+  const int r = blockIdx.x * kQuads + (threadIdx.x >> 2);
+  if (r >= a.total) return;
+  int lo = 0, hi = a.n;  // the last i with cu[i] <= r, or n
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (a.cu[mid] <= base) lo = mid; else hi = mid - 1;
+    if (a.cu[mid] <= r) lo = mid; else hi = mid - 1;
   }
-  const int g = lane >> 2, w = lane & 3;
-  // of the current sequence: its rows [begin, end), home, first position, pool
-  int i = lo - 1, begin = 0, end = base, home = 0, first = 0;
-  bool known = false, good = false;
-  Pool pool{};
-  size_t src = 0;  // cache row of this lane's row (contiguous: moves with it)
-  uint32_t kw[kRows], vw[kRows], km[kRows], vm[kRows];
-  unsigned live = 0;
-#pragma unroll
-  for (int u = 0; u < kRows; ++u) {
-    const int r = base + u * kHalfWarps;
-    src += kHalfWarps;
-    while (end <= r && i + 1 < a.n) {
-      ++i;
-      begin = a.cu[i];
-      end = a.cu[i + 1];
-      known = false;
-    }
-    if (r >= a.total || i < 0 || r < begin || r >= end) continue;  // no sequence's row
-    if (!known) {
-      const int m = a.seqs[3 * i];
-      home = a.seqs[3 * i + 1];
-      first = a.seqs[3 * i + 2];
-      pool = m == 1 ? a.pool[1] : a.pool[0];
-      good = (m == 0 || m == 1) && home >= 0 && first >= 0 &&
-             home < (a.block_table ? a.table_rows : pool.rows);
-      if (!a.block_table)
-        src = ((size_t)home * a.n_kv + h) * a.L_cap + (size_t)((long long)first + r - begin);
-      known = true;
-    }
-    const long long p = (long long)first + r - begin;
-    bool ok = good;
-    if (a.block_table) {
-      const long long page = p >> a.page_shift;
-      ok = ok && page < a.max_pages;
-      const int row = ok ? a.block_table[(size_t)home * a.max_pages + page] : -1;
-      ok = ok && row >= 0 && row < pool.rows;
-      src = ((size_t)row * a.n_kv + h) * a.page_size + ((int)p & (a.page_size - 1));
-    } else {
-      ok = ok && p < a.L_cap;
-    }
-    if (!ok) {
-      if (lane == 0 && h == 0) set_status(a.status, PS_ERR_BAD_INDEX);
-      continue;
-    }
-    live |= 1u << u;
-    kw[u] = reinterpret_cast<const uint32_t*>(pool.k_codes + src * kCodeBytes)[4 * w + g];
-    vw[u] = reinterpret_cast<const uint32_t*>(pool.v_codes + src * kCodeBytes)[4 * w + g];
-    km[u] = reinterpret_cast<const uint32_t*>(pool.k_meta + src * kMetaBytes)[g];
-    vm[u] = reinterpret_cast<const uint32_t*>(pool.v_meta + src * kMetaBytes)[g];
+  if (lo == a.n || r < a.cu[lo]) return;  // no sequence's row
+  const int m = a.seqs[3 * lo], home = a.seqs[3 * lo + 1], first = a.seqs[3 * lo + 2];
+  const Pool pool = m == 1 ? a.pool[1] : a.pool[0];
+  bool ok = (m == 0 || m == 1) && home >= 0 && first >= 0 &&
+            home < (a.block_table ? a.table_rows : pool.rows);
+  const long long p = (long long)first + r - a.cu[lo];
+  size_t src = 0;  // cache row
+  if (a.block_table) {
+    const long long page = p >> a.page_shift;
+    ok = ok && page < a.max_pages;
+    const int row = ok ? a.block_table[(size_t)home * a.max_pages + page] : -1;
+    ok = ok && row >= 0 && row < pool.rows;
+    src = ((size_t)row * a.n_kv + h) * a.page_size + ((int)p & (a.page_size - 1));
+  } else {
+    ok = ok && p < a.L_cap;
+    src = ((size_t)home * a.n_kv + h) * a.L_cap + p;
   }
+  if (!ok) {
+    if (w == 0 && h == 0) set_status(a.status, PS_ERR_BAD_INDEX);
+    return;
+  }
+  const Vec8 kw = reinterpret_cast<const Vec8*>(pool.k_codes + src * kCodeBytes)[w];
+  const Vec8 vw = reinterpret_cast<const Vec8*>(pool.v_codes + src * kCodeBytes)[w];
+  const Vec8 km = *reinterpret_cast<const Vec8*>(pool.k_meta + src * kMetaBytes);
+  const Vec8 vm = *reinterpret_cast<const Vec8*>(pool.v_meta + src * kMetaBytes);
+  const size_t dst = ((size_t)r * a.n_kv + h) * kD;
+  Vec8* k = reinterpret_cast<Vec8*>((T*)a.k_out + dst);
+  Vec8* v = reinterpret_cast<Vec8*>((T*)a.v_out + dst);
 #pragma unroll
-  for (int u = 0; u < kRows; ++u) {
-    if (!(live >> u & 1)) continue;
-    const size_t dst = ((size_t)(base + u * kHalfWarps) * a.n_kv + h) * kD;
-    reinterpret_cast<Vec8*>((T*)a.k_out + dst)[lane] = values8<T>(kw[u], km[u]);
-    reinterpret_cast<Vec8*>((T*)a.v_out + dst)[lane] = values8<T>(vw[u], vm[u]);
+  for (int g = 0; g < 4; ++g) {
+    k[4 * g + w] = values8<T>(kw.u[g], km.u[g]);
+    v[4 * g + w] = values8<T>(vw.u[g], vm.u[g]);
   }
 }
 
@@ -643,7 +618,7 @@ extern "C" int ps_kv4_gather(const ps_kv4_cache_t* cache, const int32_t* seqs, c
   while (cache->block_table && (1 << a.page_shift) < cache->page_size) ++a.page_shift;
   a.max_pages = cache->max_pages;
   a.table_rows = cache->table_rows;
-  const dim3 grid(cdiv(total, kv4::kHalfWarps * kv4::kRows), cache->n_kv_heads);
+  const dim3 grid(cdiv(total, kv4::kQuads), cache->n_kv_heads);
   cudaStream_t st = (cudaStream_t)stream;
   if (dtype == PS_DTYPE_BF16)
     PS_CUDA_RET(launch(kv4::kv4_gather_kernel<__nv_bfloat16>, grid, dim3(kv4::kThreads), 0, st, a));
