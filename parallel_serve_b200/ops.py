@@ -390,6 +390,9 @@ def positions_routed(seq_len: torch.Tensor, perm: torch.Tensor | None, out: torc
 
 _HD = 128
 _CACHE = struct.Struct("=4Qi4x4Qi4xQ5i4x")       # ps_kv4_cache_t
+_POOL_SHAPE = ("a 4-bit pool is codes [rows, n_kv_heads, length, 64] and meta [rows, n_kv_heads, "
+               "length, 4, 2], for K and for V")
+_U8, _DENSE = torch.uint8, torch.contiguous_format
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _current_device = torch._C._cuda_getDevice
 
@@ -501,25 +504,31 @@ def _kv4_cache(pools, block_table: torch.Tensor | None, idx: int,
     n_kv = length = 0
     desc = []
     for p in pools:
-        if p is None or p[0].shape[0] == 0:
+        if p is None:
             desc += (0, 0, 0, 0, 0)
             continue
         kc, km, vc, vm = p
-        sh, ms = kc.shape, km.shape
-        if len(sh) != 4 or sh[3] != 64 or vc.shape != sh or len(ms) != 5 or \
-                ms[:3] != sh[:3] or ms[3:] != (4, 2) or vm.shape != ms:
-            raise ValueError("a 4-bit pool is codes [rows, n_kv_heads, length, 64] and meta "
-                             "[rows, n_kv_heads, length, 4, 2], for K and for V")
-        if kc.dtype != torch.uint8 or vc.dtype != torch.uint8 or km.dtype != dtype or \
-                vm.dtype != dtype:
+        sh = kc.shape
+        if len(sh) != 4:
+            raise ValueError(_POOL_SHAPE)
+        rows, heads, n, code_bytes = sh
+        if rows == 0:
+            desc += (0, 0, 0, 0, 0)
+            continue
+        ms = (rows, heads, n, 4, 2)
+        if code_bytes != 64 or vc.shape != sh or km.shape != ms or vm.shape != ms:
+            raise ValueError(_POOL_SHAPE)
+        if kc.dtype is not _U8 or vc.dtype is not _U8 or km.dtype is not dtype or \
+                vm.dtype is not dtype:
             raise TypeError(f"a 4-bit pool holds uint8 codes and {dtype} meta here")
-        for t in p:
-            if t.get_device() != idx or not t.is_contiguous():
-                raise ValueError(f"4-bit pools must be contiguous tensors on cuda:{idx}")
-        if n_kv and (n_kv, length) != (sh[1], sh[2]):
+        if not (kc.get_device() == km.get_device() == vc.get_device() == vm.get_device() == idx
+                and kc.is_contiguous() and km.is_contiguous() and vc.is_contiguous()
+                and vm.is_contiguous()):
+            raise ValueError(f"4-bit pools must be contiguous tensors on cuda:{idx}")
+        if n_kv and (n_kv != heads or length != n):
             raise ValueError("both models' pools must have the same heads and length")
-        n_kv, length = sh[1], sh[2]
-        desc += (kc.data_ptr(), km.data_ptr(), vc.data_ptr(), vm.data_ptr(), sh[0])
+        n_kv, length = heads, n
+        desc += (kc.data_ptr(), km.data_ptr(), vc.data_ptr(), vm.data_ptr(), rows)
     if not n_kv or not length:
         raise ValueError("at least one model needs a 4-bit pool")
     if block_table is None:
@@ -567,14 +576,14 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, pos: torch.Tensor, *,
     if Mk != M:
         raise ValueError("q and k must have the same tokens")
     if q_out is None:
-        q_out, qos = q.new_empty(q.shape), nh * _HD
+        q_out, qos = torch.empty_like(q, memory_format=_DENSE), nh * _HD
     else:
         _on(q_out, "q_out", idx, dt)
         n, h, qos = _heads(q_out, "q_out")
         if (n, h) != (M, nh):
             raise ValueError("q_out must have the shape of q")
     if k_out is None:
-        k_out, kos = k.new_empty(k.shape), nkv * _HD
+        k_out, kos = torch.empty_like(k, memory_format=_DENSE), nkv * _HD
     else:
         _on(k_out, "k_out", idx, dt)
         n, h, kos = _heads(k_out, "k_out")
@@ -625,7 +634,7 @@ def kv4_append(k: torch.Tensor, v: torch.Tensor, pools: tuple, pos: torch.Tensor
         if Mq != M:
             raise ValueError("q must have one row per token of k")
         if q_out is None:
-            q_out, qos = q.new_empty(q.shape), nh * _HD
+            q_out, qos = torch.empty_like(q, memory_format=_DENSE), nh * _HD
         else:
             _on(q_out, "q_out", idx, dt)
             n, h, qos = _heads(q_out, "q_out")
@@ -668,7 +677,7 @@ def kv4_gather(pools: tuple, seqs: torch.Tensor, cu: torch.Tensor, total: int, *
     if total < 0:
         raise ValueError("total must be >= 0")
     if out is None:
-        k, v = meta.new_empty((total, nkv, _HD)), meta.new_empty((total, nkv, _HD))
+        k, v = meta.new_empty((2, total, nkv, _HD)).unbind()  # one allocation
     else:
         k, v = out
         for t in out:
