@@ -677,7 +677,7 @@ def kv4_gather(pools: tuple, seqs: torch.Tensor, cu: torch.Tensor, total: int, *
     if total < 0:
         raise ValueError("total must be >= 0")
     if out is None:
-        k, v = meta.new_empty((2, total, nkv, _HD)).unbind()  # one allocation
+        k, v = meta.new_empty((total, nkv, _HD)), meta.new_empty((total, nkv, _HD))
     else:
         k, v = out
         for t in out:
