@@ -74,6 +74,18 @@ PS_DEV Vec8 pack8(const float* f) {
 // interleaved pairs, and half-layout pairs of a part of the head.
 enum Rotation { kNone, kWhole, kInterleaved, kPart };
 
+// The smallest and largest of three values, NaN when one of them is.
+PS_DEV float min3(float a, float b, float c) {
+  float d;
+  asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+PS_DEV float max3(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 // Quantise a group: 16 channels of this lane, 16 of the lane beside it. Words of 8
 // codes and the group's (s, z).
 //
@@ -86,16 +98,16 @@ enum Rotation { kNone, kWhole, kInterleaved, kPart };
 template <typename T>
 PS_DEV void quantise_group(const float (&a)[8], const float (&b)[8], unsigned mask,
                            uint32_t (&word)[2], uint32_t& meta) {
-  float lo = fminf(a[0], b[0]), hi = fmaxf(a[0], b[0]), zero = 0.f;  // NaN when not all finite
+  float lo = a[0], hi = a[0];  // NaN when one is
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    lo = fminf(lo, fminf(a[i], b[i]));
-    hi = fmaxf(hi, fmaxf(a[i], b[i]));
-    zero = fmaf(a[i], 0.f, fmaf(b[i], 0.f, zero));
+    lo = min3(lo, a[i], b[i]);
+    hi = max3(hi, a[i], b[i]);
   }
-  lo = fminf(lo, __shfl_xor_sync(mask, lo, 1));
-  hi = fmaxf(hi, __shfl_xor_sync(mask, hi, 1));
-  zero += __shfl_xor_sync(mask, zero, 1);
+  const float lo1 = __shfl_xor_sync(mask, lo, 1), hi1 = __shfl_xor_sync(mask, hi, 1);
+  lo = min3(lo, lo1, lo1);
+  hi = max3(hi, hi1, hi1);
+  const bool finite = fabsf(lo) <= 3.402823466e38f && fabsf(hi) <= 3.402823466e38f;
   T zt = saturate<T>(lo);
   const float z = to_f32<T>(zt);
   const float span = __fsub_rn(hi, z);
@@ -134,7 +146,7 @@ PS_DEV void quantise_group(const float (&a)[8], const float (&b)[8], unsigned ma
       word[k] -= 0x3f400000u;  // 0x4b400000 (1 + 16 + 256 + ...) in 32 bits
     }
   }
-  if (zero != zero) {
+  if (!finite) {
     word[0] = word[1] = 0;
     st = from_f32<T>(0.f);
     zt = from_f32<T>(__uint_as_float(0x7fc00000u));
