@@ -758,7 +758,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     the same rows) of ``k``, ``v`` [keys, n_kv_heads, 128]; the last query sees every
     key, so keys that precede the queries are their history. A query that sees
     no key gets 0. q, k, v may be views of one qkv row. ``cu_q``, ``cu_k`` are int32
-    on the device. Returns [tokens, n_heads * 128].
+    on the device. Rows outside every sequence are left as ``out`` had them.
+    Returns [tokens, n_heads * 128].
     """
     idx, code = _first(q)
     dt = q.dtype

@@ -222,6 +222,63 @@ def test_append_with_norm_and_rotation(dt, page):
     assert _status() == 0
 
 
+ROTATIONS = [(128, False), (128, True), (64, False), (96, False), (48, True), (0, False)]
+
+
+@pytest.mark.parametrize("rotary,inter", ROTATIONS)
+@pytest.mark.parametrize("nh,nkv", [(1, 1), (40, 8), (13, 13), (96, 32)])
+def test_many_tokens_are_as_few(rotary, inter, nh, nkv):
+    """Rows do not depend on how many tokens a call has, nor on being done in place."""
+    from parallel_serve_b200 import ops
+    dt, M, c0 = torch.float16, 701, 300
+    x = cpu_randn((M, nh + nkv, 128), nh + rotary, 1.0, dt).to(DEV)
+    pos = torch.randint(0, 900, (M,), generator=torch.Generator().manual_seed(9)).int().to(DEV)
+    kw = dict(q_weight=_weights(6, dt).to(DEV), k_weight=_weights(7, dt).to(DEV), interleaved=inter)
+    if rotary:
+        kw["rope_cos"], kw["rope_sin"] = _tables(900, rotary)
+    q, k = ops.qk_norm_rope(x[:, :nh], x[:, nh:], pos, split_point=c0, **kw)
+    for a in range(0, M, 67):
+        b = min(M, a + 67)
+        qs, ks = ops.qk_norm_rope(x[a:b, :nh], x[a:b, nh:], pos[a:b],
+                                  split_point=min(max(c0 - a, 0), b - a), **kw)
+        assert torch.equal(qs, q[a:b]) and torch.equal(ks, k[a:b])
+    ops.qk_norm_rope(x[:, :nh], x[:, nh:], pos, split_point=c0, q_out=x[:, :nh], k_out=x[:, nh:], **kw)
+    assert torch.equal(x[:, :nh], q) and torch.equal(x[:, nh:], k) and _status() == 0
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("page", [0, 8])
+@pytest.mark.parametrize("nh,nkv,rotary,inter", [(0, 1, 0, False), (5, 5, 96, False), (40, 8, 128, False),
+                                                 (32, 32, 64, True)])
+def test_a_long_append_is_as_short_ones(dt, page, nh, nkv, rotary, inter):
+    from parallel_serve_b200 import ops
+    lens, n0, cap = [400, 300, 29], 2, 400
+    T = sum(lens)
+    x = cpu_randn((T, nh + 2 * nkv, 128), T + nh, 1.0, dt).to(DEV)
+    pos = torch.cat([torch.arange(n) for n in lens]).int().to(DEV)
+    home = torch.cat([torch.full((n,), i if page or i < n0 else i - n0)
+                      for i, n in enumerate(lens)]).int().to(DEV)
+    kw = dict(k_weight=_weights(8, dt).to(DEV), interleaved=inter)
+    if rotary:
+        kw["rope_cos"], kw["rope_sin"] = _tables(cap, rotary)
+    split = sum(lens[:n0])
+    got = []
+    for step in (T, 41):
+        pools, table = _pools(lens[:n0], lens[n0:], nkv, dt, page, cap)
+        qs = []
+        for a in range(0, T, step):
+            b = min(T, a + step)
+            qs.append(ops.kv4_append(x[a:b, nh:nh + nkv], x[a:b, nh + nkv:], pools, pos[a:b],
+                                     q=x[a:b, :nh] if nh else None, rows=home[a:b], block_table=table,
+                                     split_point=min(max(split - a, 0), b - a), **kw))
+        got.append((pools, torch.cat(qs) if nh else None))
+    for one, many in zip(*(g[0] for g in got)):
+        for a, b in zip(one, many):
+            assert torch.equal(a, b)
+    assert nh == 0 or torch.equal(got[0][1], got[1][1])
+    assert _status() == 0
+
+
 def test_gather_windows_and_untouched_rows():
     from parallel_serve_b200 import ops
     dt, lens, n0, nkv = torch.float16, [30, 12, 50], 2, 2
