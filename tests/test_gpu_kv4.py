@@ -533,6 +533,44 @@ def test_step_in_a_graph_and_on_another_stream():
     assert _status() == 0
 
 
+def test_two_streams_and_two_graphs_at_once():
+    """Calls that overlap have workspaces of their own: long sequences, whose pieces
+    several CTAs join, on two streams and in two graphs replayed side by side."""
+    from parallel_serve_b200 import ops
+    dt, nkv, nh, cap = torch.float16, 2, 8, 8192
+    sides, todo = [torch.cuda.Stream() for _ in range(2)], []
+    for i, (lens, page) in enumerate((([8000, 3, 5000], 16), ([7000], 0))):
+        pools, table, _, _, _, _ = _filled(lens, 1, nkv, dt, page, cap, 51 + i)
+        pos = torch.tensor([n - 1 for n in lens], dtype=torch.int32, device=DEV)
+        q = cpu_randn((len(lens), nh, 128), 61 + i, 1.0, dt).to(DEV)
+
+        def call(q=q, pools=pools, pos=pos, table=table):
+            return ops.kv4_decode_attention(q, pools, pos, max_len=cap, block_table=table,
+                                            split_point=1)
+        todo.append((call, call()))
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(sides):
+            with torch.cuda.stream(s):
+                outs[i].append(todo[i][0]())
+    torch.cuda.synchronize()
+    graphs = []
+    for call, _ in todo:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = call()
+        graphs.append((g, out))
+    for _ in range(20):
+        for (g, _), s in zip(graphs, sides):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for i, (_, want) in enumerate(todo):
+        assert all(torch.equal(o, want) for o in outs[i]) and torch.equal(graphs[i][1], want)
+    assert _status() == 0
+
+
 def test_registered_operators_run_together():
     """norm + rotation, cache write, decode and prompt attention through torch.ops: what
     a prompt and the step after it do."""
