@@ -76,6 +76,7 @@ struct Args {
   const int32_t* cu_q;  // [n + 1]
   const int32_t* cu_k;
   int n, Tq, Tk, n_heads, group, bf16;
+  int wide;  // out's rows are 32-byte aligned
   float scale_log2;
   int32_t* status;
 };
@@ -184,6 +185,15 @@ PS_DEV void st32(uint32_t taddr, const uint32_t* r) {
       "%24,%25,%26,%27,%28,%29,%30,%31};" ::PS_IN32(r),
       "r"(taddr)
       : "memory");
+}
+
+// 32 bytes, a whole sector, in one store: a warp's 32 rows are 32 sectors of different
+// lines, and with 16-byte stores each is touched twice (8 prompts of 512 to 1024
+// tokens: 87 and 82 us; one of 16384: 2.00 and 1.99 ms).
+PS_DEV void st_32bytes(void* p, const uint32_t (&w)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]),
+               "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
 }
 
 PS_DEV float exp2_ftz(float x) {
@@ -626,16 +636,20 @@ __global__ void __launch_bounds__(Shape<kTiles>::kThreads, Shape<kTiles>::kCtas)
         }
         if (live) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 8) {
-            uint4 w = make_uint4(0u, 0u, 0u, 0u);
+          for (int i = 0; i < 32; i += 16) {
+            uint32_t w[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
             if (my_nb > 0 && inv != 0.f) {
-              float f[8];
 #pragma unroll
-              for (int k = 0; k < 8; ++k) f[k] = __uint_as_float(o[i + k]) * inv;
-              w = make_uint4(pack16<T>(f[0], f[1]), pack16<T>(f[2], f[3]), pack16<T>(f[4], f[5]),
-                             pack16<T>(f[6], f[7]));
+              for (int k = 0; k < 8; ++k)
+                w[k] = pack16<T>(__uint_as_float(o[i + 2 * k]) * inv,
+                                 __uint_as_float(o[i + 2 * k + 1]) * inv);
             }
-            *reinterpret_cast<uint4*>(orow + c + i) = w;
+            if (a.wide) {
+              st_32bytes(orow + c + i, w);
+            } else {
+              reinterpret_cast<uint4*>(orow + c + i)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+              reinterpret_cast<uint4*>(orow + c + i)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+            }
           }
         }
       }
@@ -674,8 +688,8 @@ extern "C" int ps_prompt_attention(const void* q, long long q_stride, const void
                            v_stride >= (long long)n_kv_heads * pra::kD && v_stride % 8 == 0));
   // By the mean length, which is what the host knows: two CTAs of one tile on an SM
   // (128 queries each) waste less of a short sequence and hide each other's start
-  // (64 prompts of 64 to 128 tokens, 32 + 8 heads: 68 us, one CTA of two tiles 118; 8 of
-  // 512 to 1024: 87 and 101); two tiles read each K and V block once for twice the
+  // (64 prompts of 64 to 128 tokens, 32 + 8 heads: 65 us, one CTA of two tiles 118; 8 of
+  // 512 to 1024: 82 and 101); two tiles read each K and V block once for twice the
   // queries, which wins behind some 4096 (one prompt of 4096: 138 and 140 us, of 8192:
   // 547 and 515, of 16384: 2084 and 1976).
   const bool one = Tk < 4096ll * n_seqs;
@@ -709,6 +723,7 @@ extern "C" int ps_prompt_attention(const void* q, long long q_stride, const void
   a.n_heads = n_heads;
   a.group = n_heads / n_kv_heads;
   a.bf16 = bf ? 1 : 0;
+  a.wide = (reinterpret_cast<uintptr_t>(out) % 32 == 0 && o_stride % 16 == 0) ? 1 : 0;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.status = status;
   cudaStream_t st = (cudaStream_t)stream;

@@ -215,3 +215,22 @@ def test_two_tiles_and_non_finite_values():
         assert torch.equal(out[:key], want[:key]), key
         assert torch.isnan(out[key:]).all()
     assert _status() == 0
+
+
+@pytest.mark.parametrize("keys", [600, 4200])
+@pytest.mark.parametrize("shift,extra", [(0, 8), (8, 0), (8, 8), (16, 16)])
+def test_output_rows_of_any_alignment(shift, extra, keys):
+    """Rows at 16-byte and at 32-byte boundaries give the same, and nothing beside them is written."""
+    from parallel_serve_b200 import ops
+    dt, nh, nkv, n = torch.bfloat16, 2, 1, 300
+    q, k, v = (cpu_randn((m, h, 128), 111 + i, 1.0, dt).to(DEV)
+               for i, (m, h) in enumerate(((n, nh), (keys, nkv), (keys, nkv))))
+    cu_q, cu_k = _cu([n]), _cu([keys])
+    want = ops.prompt_attention(q, k, v, cu_q, cu_k)
+    stride = nh * 128 + extra
+    buf = torch.full((shift + n * stride + 64,), 9.0, dtype=dt, device=DEV)
+    out = buf[shift:].as_strided((n, nh * 128), (stride, 1), shift)
+    ops.prompt_attention(q, k, v, cu_q, cu_k, out=out)
+    assert torch.equal(out, want) and _status() == 0
+    out.fill_(9.0)
+    assert (buf == 9).all()
