@@ -15,7 +15,7 @@
 // keeps the token's cos / sin in registers.
 // What it reaches now is 5.1 TB/s (append) to 5.4 (norm and rotation alone). Measured and
 // not kept: rows three ahead through a shared-memory ring (382 us, write + read 372
-// otherwise), 32-byte loads and stores (370), cos / sin read again for each row (61 us
+// otherwise), 32-byte loads (no change; 32-byte stores: 63 and 61 us), cos / sin read again for each row (61 us
 // for norm and rotation alone, ragged write + read 74 instead of 72), fewer registers
 // for more warps (386 and more).
 //
@@ -52,6 +52,7 @@ struct RowArgs {
   Pool pool[2];
   int32_t* status;
   int M, n_heads, n_kv, split_point, rotary, interleaved, rope_len;
+  int wide;      // q_out and k_out rows are 32-byte aligned
   int quads;     // of a token in a block: a power of two up to kQuads
   int rows_per;  // rows of a quad
   int L_cap, page_size, page_shift, max_pages, table_rows;  // append
@@ -322,7 +323,17 @@ __global__ void __launch_bounds__(kThreads) norm_rope_kernel(const RowArgs a) {
                                                : (T*)a.k_out + (size_t)j * a.ko_stride +
                                                      (r - nq) * kD);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) dst[chunk[i]] = pack8<T>(x[i]);
+      for (int i = 0; i < 4; i += 2) {  // chunks 2 q4 and 2 q4 + 1: 32 bytes
+        const Vec8 lo = pack8<T>(x[i]), hi = pack8<T>(x[i + 1]);
+        if (a.wide) {
+          const uint32_t w[8] = {lo.u[0], lo.u[1], lo.u[2], lo.u[3],
+                                 hi.u[0], hi.u[1], hi.u[2], hi.u[3]};
+          st_32bytes(dst + chunk[i], w);
+        } else {
+          dst[chunk[i]] = lo;
+          dst[chunk[i + 1]] = hi;
+        }
+      }
     } else {
       // groups q4 / 2 (chunks 0, 1) and q4 / 2 + 2 (chunks 2, 3): words 2 (q4 & 1)
       // and the next of each
@@ -496,6 +507,10 @@ static cudaError_t launch_rotation(const RowArgs& a, dim3 grid, cudaStream_t st)
 // blocks, when the tokens alone do not fill the GPU.
 template <bool kAppend>
 static int launch_rows(RowArgs& a, int dtype, cudaStream_t st) {
+  auto aligned32 = [](const void* p, long long stride) {
+    return reinterpret_cast<uintptr_t>(p) % 32 == 0 && stride % 16 == 0;
+  };
+  a.wide = aligned32(a.q_out, a.qo_stride) && (kAppend || aligned32(a.k_out, a.ko_stride));
   const int total = (a.q ? a.n_heads : 0) + (kAppend ? 2 : 1) * a.n_kv;
   const bool many = a.M >= 4 * sm_count(current_device());
   const int most = many ? 12 : 1;

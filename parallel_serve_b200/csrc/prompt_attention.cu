@@ -187,15 +187,6 @@ PS_DEV void st32(uint32_t taddr, const uint32_t* r) {
       : "memory");
 }
 
-// 32 bytes, a whole sector, in one store: a warp's 32 rows are 32 sectors of different
-// lines, and with 16-byte stores each is touched twice (8 prompts of 512 to 1024
-// tokens: 87 and 82 us; one of 16384: 2.00 and 1.99 ms).
-PS_DEV void st_32bytes(void* p, const uint32_t (&w)[8]) {
-  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]),
-               "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
-               : "memory");
-}
-
 PS_DEV float exp2_ftz(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -644,6 +635,9 @@ __global__ void __launch_bounds__(Shape<kTiles>::kThreads, Shape<kTiles>::kCtas)
                 w[k] = pack16<T>(__uint_as_float(o[i + 2 * k]) * inv,
                                  __uint_as_float(o[i + 2 * k + 1]) * inv);
             }
+            // a warp's 32 rows are 32 sectors of different lines; with 16-byte stores each is
+            // touched twice (8 prompts of 512 to 1024 tokens: 87 and 82 us; one of 16384:
+            // 2.00 and 1.99 ms)
             if (a.wide) {
               st_32bytes(orow + c + i, w);
             } else {

@@ -386,6 +386,13 @@ PS_DEV uint64_t f32x2_mul(uint64_t a, uint64_t b) {
   return d;
 }
 
+// 32 bytes, a whole sector, in one store; p is 32-byte aligned.
+PS_DEV void st_32bytes(void* p, const uint32_t (&w)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]),
+               "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
+
 // Generic named barrier over `nthreads` threads (multiple of 32).
 PS_DEV void named_bar_sync(int id, int nthreads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(nthreads) : "memory");

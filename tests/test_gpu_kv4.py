@@ -246,6 +246,30 @@ def test_many_tokens_are_as_few(rotary, inter, nh, nkv):
     assert torch.equal(x[:, :nh], q) and torch.equal(x[:, nh:], k) and _status() == 0
 
 
+@pytest.mark.parametrize("M", [5, 700])
+@pytest.mark.parametrize("shift,extra", [(8, 0), (0, 8), (8, 8), (16, 16)])
+def test_output_rows_of_any_alignment(M, shift, extra):
+    """Rows at 16-byte and at 32-byte boundaries give the same, and nothing beside them is written."""
+    from parallel_serve_b200 import ops
+    dt, nh, nkv = torch.bfloat16, 6, 3
+    x = cpu_randn((M, nh + nkv, 128), 77, 1.0, dt).to(DEV)
+    pos = torch.arange(M, dtype=torch.int32, device=DEV)
+    cos, sin = _tables(M, 128)
+    want = ops.qk_norm_rope(x[:, :nh], x[:, nh:], pos, rope_cos=cos, rope_sin=sin)
+    bufs, outs = [], []
+    for h in (nh, nkv):
+        stride = h * 128 + extra
+        bufs.append(torch.full((shift + M * stride + 64,), 9.0, dtype=dt, device=DEV))
+        outs.append(bufs[-1].as_strided((M, h, 128), (stride, 128, 1), shift))
+    ops.qk_norm_rope(x[:, :nh], x[:, nh:], pos, rope_cos=cos, rope_sin=sin, q_out=outs[0],
+                     k_out=outs[1])
+    for buf, out, w in zip(bufs, outs, want):
+        assert torch.equal(out, w)
+        out.fill_(9.0)
+        assert (buf == 9).all()
+    assert _status() == 0
+
+
 @pytest.mark.parametrize("dt", DTYPES)
 @pytest.mark.parametrize("page", [0, 8])
 @pytest.mark.parametrize("nh,nkv,rotary,inter", [(0, 1, 0, False), (5, 5, 96, False), (40, 8, 128, False),
