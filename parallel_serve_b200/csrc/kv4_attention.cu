@@ -252,8 +252,9 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm)
 
   // With short pages the (s, z) rows come by 16-byte copies of the producer's lanes:
   // half as many bulk copies, whose number a tile then waits for (pages of 16: 299 and
-  // 280 us for 96 ragged sequences; pages of 64: 170 with bulk copies, 174 with these;
-  // the codes by 16-byte copies too: 332).
+  // 280 us for 96 ragged sequences, 267 since the producer's addresses are made once a
+  // piece: its instructions are taken from the compute warps'; pages of 64: 170 with
+  // bulk copies, 174 with these; the codes by 16-byte copies too: 332).
   const bool small_pages = a.block_table && a.page_size <= kSmallPage;
 
   // Tiles per entry of tokens, then their prefix sums.
@@ -315,6 +316,13 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm)
       const int m = pc.j >= c0 ? 1 : 0;
       const Pool pool = m ? a.pool[1] : a.pool[0];
       const int home = a.rows ? a.rows[pc.j] : (a.block_table ? pc.j : pc.j - (m ? c0 : 0));
+      // paged: the token's table row, the log of a run's positions, row 0 of this head in
+      // a page, and rows from one page to the next
+      const int32_t* table = a.block_table + (a.block_table ? (size_t)home * a.max_pages : 0);
+      const int run_shift = min(a.page_shift, 7);
+      const size_t head_row = (size_t)pc.kvh * a.page_size;
+      const size_t page_rows = (size_t)a.n_kv * a.page_size;
+      const size_t meta_at = (head_row + (lane & (a.page_size - 1))) * kMetaBytes;  // short pages
       for (int t = pc.t0; t < pc.t1; ++t, ++gs) {
         const int st = gs % kStages;
         const int pos0 = t * kTile;
@@ -322,11 +330,9 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm)
         // one run per page (128 % page_size == 0 or page_size % 128 == 0, so runs
         // start at multiples of page_size or fill the tile): lane l takes run l (at
         // most 16 of them), and looks its page up while the stage is still in use
-        const int run = min(a.page_size, kTile);
-        const int nrun = a.block_table ? (npos + run - 1) / run : 0;
+        const int o = lane << run_shift;  // the run's first position in the tile
         int page = 0;
-        if (lane < nrun)
-          page = a.block_table[(size_t)home * a.max_pages + ((pos0 + lane * run) >> a.page_shift)];
+        if (a.block_table && o < npos) page = table[(pos0 + o) >> a.page_shift];
         if (!mbar_wait(empty + st, ((gs / kStages) & 1) ^ 1, a.status)) abort_flag[0] = 1;
         dead = __any_sync(0xffffffffu, abort_flag[0] != 0);
         if (dead) break;
@@ -360,11 +366,9 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm)
                                                  (kCodeBytes + (small_pages ? 0 : kMetaBytes)));
           }
           __syncwarp();
-          if (lane < nrun) {
-            const int o = lane * run;
-            const int n = min(run, npos - o);
-            const size_t row = ((size_t)page * a.n_kv + pc.kvh) * a.page_size +
-                               ((pos0 + o) & (a.page_size - 1));
+          if (o < npos) {
+            const int n = min(1 << run_shift, npos - o);
+            const size_t row = page * page_rows + head_row + ((pos0 + o) & (a.page_size - 1));
             bulk_load(buf + o * kCodeBytes, pool.k_codes + row * kCodeBytes, n * kCodeBytes,
                       full + st, pol);
             bulk_load(buf + kTileCodes + kTileMeta + o * kCodeBytes,
@@ -379,13 +383,12 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm)
           if (small_pages) {
 #pragma unroll
             for (int i = 0; i < kTile / 32; ++i) {
-              const int o = lane + 32 * i;
-              const int pg = __shfl_sync(0xffffffffu, page, o >> a.page_shift);
-              if (o < npos) {
-                const size_t at = (((size_t)pg * a.n_kv + pc.kvh) * a.page_size +
-                                   ((pos0 + o) & (a.page_size - 1))) * kMetaBytes;
-                cp_async16(buf + kTileCodes + o * kMetaBytes, pool.k_meta + at);
-                cp_async16(buf + 2 * kTileCodes + kTileMeta + o * kMetaBytes, pool.v_meta + at);
+              const int r = lane + 32 * i;
+              const int pg = __shfl_sync(0xffffffffu, page, r >> a.page_shift);
+              if (r < npos) {
+                const size_t at = meta_at + pg * (page_rows * kMetaBytes);
+                cp_async16(buf + kTileCodes + r * kMetaBytes, pool.k_meta + at);
+                cp_async16(buf + 2 * kTileCodes + kTileMeta + r * kMetaBytes, pool.v_meta + at);
               }
             }
             cp_async_arrive(full + st);
