@@ -479,7 +479,6 @@ __global__ void __launch_bounds__(Shape<kTiles>::kThreads, Shape<kTiles>::kCtas)
 #pragma unroll 1
       for (int j = 0; ok && j < nb; ++j) {
         wait(kv_full_a + 8 * vs, vph);
-        if (j + 1 < nb) wait(kv_full_a + 8 * ks, kph);
 #pragma unroll
         for (int t = 0; t < kTiles; ++t) {
           const int n = t ? nb1 : nb0;
@@ -488,6 +487,9 @@ __global__ void __launch_bounds__(Shape<kTiles>::kThreads, Shape<kTiles>::kCtas)
             tc_fence_after();
             values(t, 0, vs, j == 0);
             mma_commit(pv_done_a + 8 * t);
+            // The next block's K is waited for where P's second half is not there yet
+            // (at the loop's top it delayed P V: 8 heads of 4096 tokens 66 and 62 us)
+            if (j + 1 < nb && t == (j < nb0 ? 0 : 1)) wait(kv_full_a + 8 * ks, kph);
             wait(p_full_a + 16 * t + 8, j & 1);
             tc_fence_after();
             values(t, 1, vs, false);
@@ -683,10 +685,10 @@ extern "C" int ps_prompt_attention(const void* q, long long q_stride, const void
   // By the mean length, which is what the host knows: two CTAs of one tile on an SM
   // (128 queries each) waste less of a short sequence and hide each other's start
   // (64 prompts of 64 to 128 tokens, 32 + 8 heads: 65 us, one CTA of two tiles 118; 8 of
-  // 512 to 1024: 82 and 101); two tiles read each K and V block once for twice the
+  // 512 to 1024: 81 and 101); two tiles read each K and V block once for twice the
   // queries, which wins behind some 4096 (one prompt of 4096: 138 and 140 us, of 8192:
   // 547 and 515, of 16384: 2084 and 1976).
-  const bool one = Tk < 4096ll * n_seqs;
+  const bool one = Tk <= 4096ll * n_seqs;
   const int rows = pra::kTile * (one ? 1 : 2);
   const long long grid = ((long long)Tq / rows + n_seqs) * n_heads;
   if (grid > 0x7fffffffll || Tk > (1 << 30) || Tq > (1 << 30)) return PS_ERR_UNSUPPORTED;
