@@ -40,8 +40,9 @@
 //
 // A masked key's P is 0, but 0 * NaN is not: in the blocks that need a mask (the
 // diagonal and a sequence's end) the V rows behind the end are cleared in shared
-// memory, and a row that holds a NaN or an infinity is cleared too, its key
-// remembered: the queries that see it get NaN, the others what they should.
+// memory, and so is a single value that is not finite. The first key with +inf, -inf
+// and NaN is kept for each channel, and the queries that see it get it added to
+// that channel of their output, as the product does in a block without a mask.
 #include <cuda_runtime.h>
 
 #include <type_traits>
@@ -57,6 +58,8 @@ constexpr int kTile = 128;              // queries of a tile, keys of a block
 constexpr int kTileBytes = kTile * kD * 2;
 constexpr int kHalf = kTileBytes / 2;   // one 64-column TMA box (128 rows x 128 bytes)
 constexpr int kKeys = 64;               // keys of half a block
+constexpr int kBadBytes = 3 * kD * 4;   // first key with +inf, -inf, NaN in each channel
+constexpr int kNoKey = 0x7fffffff;
 // What a CTA is made of: kTiles tiles of queries.
 template <int kTiles>
 struct Shape {
@@ -64,7 +67,7 @@ struct Shape {
   static constexpr int kSlots = kTiles == 2 ? 5 : 2;     // of the K / V ring
   static constexpr int kThreads = (kTiles * 4 + 2) * 32;
   static constexpr int kCtas = 3 - kTiles;               // resident on an SM
-  static constexpr int kSmem = 1024 + kTileBytes * (kTiles + kSlots) + 256;
+  static constexpr int kSmem = 1024 + kTileBytes * (kTiles + kSlots) + 256 + kBadBytes;
   static constexpr int kTmemCols = 256 * kTiles;
   static constexpr int kTmemO = 128 * kTiles;            // S tiles from 0, O tiles from here
 };
@@ -277,6 +280,22 @@ PS_DEV bool finite8(const uint4& u) {
   return fin;
 }
 
+// Clear the values of one row's 64 channels (128 swizzled bytes of key `key`) that are not
+// finite, noting their keys by kind and channel. Rare, so small rather than fast.
+template <typename T>
+PS_DEV void clear_bad(uint8_t* row, int key, int ch0, int* bad) {
+#pragma unroll 1
+  for (int c = 0; c < 64; ++c) {
+    T* p = reinterpret_cast<T*>(row + ((((c >> 3) ^ key) & 7) << 4)) + (c & 7);
+    const float x = to_f32<T>(*p);
+    if (fabsf(x) <= 3.402823466e38f) continue;
+    const int kind = x != x ? 2 : (x > 0.f ? 0 : 1);
+    atomicMin(bad + kind * kD + ch0 + c, key);
+    __threadfence_block();  // whoever finds it cleared finds its key
+    *p = from_f32<T>(0.f);
+  }
+}
+
 // With R queries to a CTA, sequence i owns slots [cu_q[i] / R + i, cu_q[i + 1] / R + i + 1): at
 // least as many as it has tiles, found by a search, no scan of lengths (every lane of a warp
 // calls it).
@@ -341,7 +360,8 @@ __global__ void __launch_bounds__(Shape<kTiles>::kThreads, Shape<kTiles>::kCtas)
   uint64_t* drain = o_done + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  int* poison = reinterpret_cast<int*>(tmem_slot + 2);  // first cleared key that was not finite
+  int* poison = reinterpret_cast<int*>(tmem_slot + 2);  // first key with a value cleared
+  int* bad = reinterpret_cast<int*>(bars + 32);         // [3 kinds][128 channels]: the same of each
 
   const int warp = (int)uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const bool producer = warp == kTma && lane == 0;
@@ -363,9 +383,10 @@ __global__ void __launch_bounds__(Shape<kTiles>::kThreads, Shape<kTiles>::kCtas)
     }
     mbar_init(drain, 1);
     abort_flag[0] = 0;
-    poison[0] = 0x7fffffff;
+    poison[0] = kNoKey;
     fence_mbar_init();
   }
+  for (int i = threadIdx.x; i < 3 * kD; i += Shape<kTiles>::kThreads) bad[i] = kNoKey;
   __syncwarp();
   pdl_wait();
 
@@ -583,18 +604,16 @@ __global__ void __launch_bounds__(Shape<kTiles>::kThreads, Shape<kTiles>::kCtas)
           if (mbar_wait(kv_full + i % kSlots, (i / kSlots) & 1, a.status)) {
             uint8_t* v = sKV + (i % kSlots) * kTileBytes + (r >> 6) * kHalf +
                          (key & (kTile - 1)) * 128;
-            bool clear = key >= it.lk;
-            if (!clear) {
+            if (key < it.lk) {
               bool fin = true;
 #pragma unroll
               for (int c = 0; c < 8; ++c)  // 16-byte chunks, rotated by row: no bank conflicts
                 fin &= finite8<T>(*reinterpret_cast<const uint4*>(v + (((c + r) & 7) << 4)));
               if (!fin) {
-                clear = true;
                 atomicMin(poison, key);
+                clear_bad<T>(v, key, (r >> 6) * 64, bad);
               }
-            }
-            if (clear) {
+            } else {
 #pragma unroll
               for (int c = 0; c < 8; ++c)
                 *reinterpret_cast<uint4*>(v + (((c + r) & 7) << 4)) = make_uint4(0u, 0u, 0u, 0u);
@@ -616,8 +635,7 @@ __global__ void __launch_bounds__(Shape<kTiles>::kThreads, Shape<kTiles>::kCtas)
     if (!fin) abort_flag[0] = 1;
     if (fin && it.live) {
       tc_fence_after();
-      float inv = l > 0.f || l != l ? 1.f / l : 0.f;  // a row that sees no key: 0
-      if (seen > *reinterpret_cast<volatile int*>(poison)) inv = __uint_as_float(0x7fc00000u);
+      const float inv = l > 0.f || l != l ? 1.f / l : 0.f;  // a row that sees no key: 0
       T* orow = reinterpret_cast<T*>(a.out) + (size_t)(it.q0 + row) * a.o_stride + h * kD;
 #pragma unroll 1
       for (int c = 0; c < kD; c += 32) {
@@ -647,6 +665,17 @@ __global__ void __launch_bounds__(Shape<kTiles>::kThreads, Shape<kTiles>::kCtas)
               reinterpret_cast<uint4*>(orow + c + i)[1] = make_uint4(w[4], w[5], w[6], w[7]);
             }
           }
+        }
+      }
+      if (live && seen > *reinterpret_cast<volatile int*>(poison)) {
+        const volatile int* key = bad;
+#pragma unroll 1
+        for (int c = 0; c < kD; ++c) {
+          float x = 0.f;
+          if (seen > key[c]) x += __uint_as_float(0x7f800000u);
+          if (seen > key[kD + c]) x -= __uint_as_float(0x7f800000u);
+          if (seen > key[2 * kD + c]) x = __uint_as_float(0x7fc00000u);
+          if (x != 0.f) orow[c] = from_f32<T>(to_f32<T>(orow[c]) + x);
         }
       }
     }
