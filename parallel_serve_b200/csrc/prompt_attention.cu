@@ -31,8 +31,8 @@
 //   reads 6 KB of shared memory in 32 cycles' work
 //
 // P = 2^(s - m) needs no exact maximum, only one reference m for P, the row sum and
-// O that keeps P within 16 bits: m is the row's maximum over its first block and
-// moves only when the sum of 64 P exceeds 2^8 (so no P does otherwise). Then the
+// O that keeps P within 16 bits: m is the row's maximum over its first block (that
+// has a score above -inf) and moves only when the sum of 64 P exceeds 2^8 (so no P does otherwise). Then the
 // half is looked at again, O and the sum are rescaled (a read and write of 128
 // columns) and its P recomputed: rare after the first block, and until then no
 // maximum is taken at all. Sums and maxima are fp32;
@@ -556,16 +556,19 @@ __global__ void __launch_bounds__(Shape<kTiles>::kThreads, Shape<kTiles>::kCtas)
       tc_fence_after();
       const bool masked = j * kTile + kTile > all_seen;  // the diagonal, or the end
       const int lim = seen - j * kTile;                  // this row's keys of the block
-      if (j == 0) {  // nothing to go by yet: the row's maximum (0 for a row of -inf)
-        m = row_max<kTile>(s_addr, masked, lim) * a.scale_log2;
-        if (m == -INFINITY) m = 0.f;
+      // Rows with nothing to go by yet take their maximum: all of them in the first block, and
+      // later those whose every score so far was -inf (their P, sum and O are still 0).
+      if (__any_sync(0xffffffffu, m == -INFINITY)) {
+        const float mx = row_max<kTile>(s_addr, masked, lim) * a.scale_log2;
+        if (m == -INFINITY) m = mx;
       }
 #pragma unroll 1
       for (int half = 0; half < 2; ++half) {
         const uint32_t h_addr = s_addr + half * kKeys;
         const int hlim = lim - half * kKeys;
         uint32_t p[32];
-        float lsum = softmax_half<T>(h_addr, masked, hlim, a.scale_log2, -m, p);
+        const float neg = m == -INFINITY ? 0.f : -m;
+        float lsum = softmax_half<T>(h_addr, masked, hlim, a.scale_log2, neg, p);
         if (__any_sync(0xffffffffu, lsum > kMaxSum)) {
           // tcgen05 loads and stores are warp-collective: rows that stay scale by 1
           const float mx = row_max<kKeys>(h_addr, masked, hlim) * a.scale_log2;
@@ -594,7 +597,7 @@ __global__ void __launch_bounds__(Shape<kTiles>::kThreads, Shape<kTiles>::kCtas)
               st32(o_addr + c, o);
             }
           }
-          lsum = softmax_half<T>(h_addr, masked, hlim, a.scale_log2, -m, p);
+          lsum = softmax_half<T>(h_addr, masked, hlim, a.scale_log2, moved ? -mx : neg, p);
         }
         st32(h_addr, p);
         l += lsum;

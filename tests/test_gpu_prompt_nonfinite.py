@@ -89,3 +89,33 @@ def test_many_values_and_a_history(dt, rows):
     assert torch.equal(out.isnan(), expect.isnan())
     assert torch.equal(out[~finite & ~expect.isnan()], expect[~finite & ~expect.isnan()])
     assert _status() == 0
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("n,pad", [(300, 0), (300, 4200)])
+@pytest.mark.parametrize("hidden", [40, 128, 130, 200])
+def test_scores_of_minus_infinity(dt, n, pad, hidden):
+    """Keys whose score is -inf weigh nothing, and the weights of the others do not
+    depend on how far below 0 their scores are: the first `hidden` keys are -inf, the rest lie
+    at -120 (2^-173 of what a score of 0 would weigh). A query that sees only keys at -inf
+    has no softmax (0 / 0): it is not looked at."""
+    import oracle
+    from parallel_serve_b200 import ops
+    q = cpu_randn((n, 1, 128), 221, 0.1, torch.float32)
+    k = cpu_randn((n + pad, 1, 128), 222, 0.1, torch.float32)
+    v = cpu_randn((n + pad, 1, 128), 223, 1.0, dt)
+    q[..., 0], k[..., 0] = 32.0, -3.75                # -120 of every score, scale 1
+    q, k = q.to(dt), k.to(dt)
+    k[:hidden, 0, 0] = -INF
+    cu = _cu([n])
+    out = to_np(ops.prompt_attention(q.to(DEV), k.to(DEV), v.to(DEV), cu, cu, scale=1.0))
+    kf = k.clone()
+    kf[:hidden, 0, 0] = -60.0                         # -1920: weighs 0 in 64 bits, too
+    want, size = oracle.grouped_attention(to_np(q), to_np(kf[:n]), to_np(v[:n]), scale=1.0)
+    # the output's and P's rounding; scores near 120 in fp32: 173 of log2 p at 2^-24, a few
+    # operations, and the reference is a product rounded at the same size: 2^-13 of each term
+    eps = torch.finfo(dt).eps
+    tol = eps / 2 * np.abs(want) + (eps / 2 + 2.0 ** -13) * size
+    rows = slice(hidden, n)
+    assert np.all(np.abs(out.reshape(want.shape) - want)[rows] <= tol[rows])
+    assert _status() == 0
