@@ -444,40 +444,43 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm)
 #pragma unroll
       for (int gi = 0; gi < 4; ++gi) {
         const uint32_t u[4] = {raw[gi].x, raw[gi].y, raw[gi].z, raw[gi].w};
-        sum[gi] = 0.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           float x, y;
           unpack2<T>(u[i], x, y);
           mx = fmaxf(mx, fmaxf(fabsf(x), fabsf(y)));
-          sum[gi] += x + y;
         }
       }
 #pragma unroll
-      for (int o = 1; o <= 2; o <<= 1) {
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-#pragma unroll
-        for (int gi = 0; gi < 4; ++gi) sum[gi] += __shfl_xor_sync(0xffffffffu, sum[gi], o);
-      }
-      int e = (int)(__float_as_uint(mx) >> 23) - 127;  // max |q| in [2^e, 2^(e+1))
-      e = max(-100, min(100, e));
+      for (int o = 1; o <= 2; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      // max |q| in [2^e, 2^(e+1)), as far as 2^e and 2^-e are normal numbers (at 2^127 q
+      // comes to less than 4 and at bf16's subnormals to less than 1)
+      const int e = max(-126, min(126, (int)(__float_as_uint(mx) >> 23) - 127));
       const float down = __uint_as_float((uint32_t)(127 - e) << 23);
 #pragma unroll
       for (int gi = 0; gi < 4; ++gi) {
         const uint32_t u[4] = {raw[gi].x, raw[gi].y, raw[gi].z, raw[gi].w};
         float f[8];
+        sum[gi] = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) unpack2<T>(u[i], f[2 * i], f[2 * i + 1]);
-        const float low = 16.f * down;  // low nibbles: even channels
-        qb[gi * 32] = make_uint4(half2_bits(f[0] * low, f[4] * low),
-                                 half2_bits(f[1] * down, f[5] * down),
-                                 half2_bits(f[2] * low, f[6] * low),
-                                 half2_bits(f[3] * down, f[7] * down));
+        for (int i = 0; i < 4; ++i) {
+          unpack2<T>(u[i], f[2 * i], f[2 * i + 1]);
+          f[2 * i] *= down;
+          f[2 * i + 1] *= down;
+          sum[gi] += f[2 * i] + f[2 * i + 1];
+        }
+        // low nibbles: even channels
+        qb[gi * 32] = make_uint4(half2_bits(f[0] * 16.f, f[4] * 16.f), half2_bits(f[1], f[5]),
+                                 half2_bits(f[2] * 16.f, f[6] * 16.f), half2_bits(f[3], f[7]));
       }
+#pragma unroll
+      for (int o = 1; o <= 2; o <<= 1)
+#pragma unroll
+        for (int gi = 0; gi < 4; ++gi) sum[gi] += __shfl_xor_sync(0xffffffffu, sum[gi], o);
       // B operand of the z term: rows k = 4 part + group hold the parts of the
       // group sums, each part what the ones before leave of it in 16 bits
       // (fp16: 11 bits each, bf16: 8; three parts make fp32's 24)
-      float r0 = (t4 & 1 ? sum[2] : sum[0]) * down, r1 = (t4 & 1 ? sum[3] : sum[1]) * down;
+      float r0 = t4 & 1 ? sum[2] : sum[0], r1 = t4 & 1 ? sum[3] : sum[1];
       uint32_t part[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
