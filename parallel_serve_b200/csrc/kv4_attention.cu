@@ -501,7 +501,7 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm)
     float o[8][4];   // [2 g + half][channel pair x head]: see the store below
     float zs[4][2];  // sum over positions of P z_g (this lane's rows)
     float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
-    float ref = __uint_as_float(27u << 23);  // 2^-100
+    float ref = __uint_as_float(1u << 23);  // 2^-126
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
@@ -679,7 +679,6 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm)
         for (int gi = 0; gi < 4; ++gi)
           zs[gi][x] += __shfl_xor_sync(0xffffffffu, zs[gi][x], off);
       }
-    const float lo24 = ref * 16777216.f, hi20 = ref * 1048576.f;
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
       const int head = 2 * t4 + x;
@@ -691,10 +690,11 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm)
       for (int gi = 0; gi < 4; ++gi) {
         const float z = zs[gi][x];
         float4 f;
-        f.x = o[2 * gi][x] * lo24 + z;
-        f.y = o[2 * gi][2 + x] * hi20 + z;
-        f.z = o[2 * gi + 1][x] * lo24 + z;
-        f.w = o[2 * gi + 1][2 + x] * hi20 + z;
+        // 2^24 and 2^20 first: times ref they may be beyond fp32
+        f.x = o[2 * gi][x] * 16777216.f * ref + z;
+        f.y = o[2 * gi][2 + x] * 1048576.f * ref + z;
+        f.z = o[2 * gi + 1][x] * 16777216.f * ref + z;
+        f.w = o[2 * gi + 1][2 + x] * 1048576.f * ref + z;
         *reinterpret_cast<float4*>(so + (warp * kHB + head) * kD + gi * kGroup + 4 * gr) = f;
       }
     }

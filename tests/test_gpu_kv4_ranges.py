@@ -31,3 +31,26 @@ def test_queries_of_every_exponent(e, nh):
     tol = torch.finfo(dt).eps / 2 * np.abs(want) + 2.0 ** -10 * (size + np.abs(vs).max())
     assert np.all(np.abs(to_np(out).reshape(want.shape) - want) <= tol)
     assert _status() == 0
+
+
+@pytest.mark.parametrize("e", [-117, -105, -70, 70, 104, 112])
+@pytest.mark.parametrize("n", [150, 3000])            # one CTA, and several joined
+def test_values_of_every_exponent(e, n):
+    """V times 2^e: the output is 2^e of what it was (the sums, at most 2^8 x n of the
+    values, stay below fp32's 2^128)."""
+    import oracle
+    from parallel_serve_b200 import KV4Pool, ops
+    dt = torch.bfloat16
+    k = cpu_randn((n, 1, 128), 91, 1.0, dt)
+    v = (cpu_randn((n, 1, 128), 92, 1.0, torch.float32).double() * 2.0 ** e).to(dt)
+    pools = (KV4Pool.zeros(1, 1, n, dt, DEV), None)
+    ops.kv4_append(k.to(DEV), v.to(DEV), pools, torch.arange(n, dtype=torch.int32, device=DEV),
+                   rows=torch.zeros(n, dtype=torch.int32, device=DEV))
+    q = cpu_randn((1, 4, 128), 93, 1.0, dt)
+    out = ops.kv4_decode_attention(q.to(DEV), pools, torch.tensor([n - 1], dtype=torch.int32, device=DEV),
+                                   max_len=n)
+    ks, vs = (_stored(pools, None, [n], 1, 0, part)[0] for part in "kv")
+    want, size = oracle.grouped_attention(to_np(q), ks, vs)
+    tol = torch.finfo(dt).eps / 2 * np.abs(want) + 2.0 ** -10 * (size + np.abs(vs).max())
+    assert np.all(np.abs(to_np(out).reshape(want.shape) - want) <= tol)
+    assert _status() == 0
