@@ -15,15 +15,16 @@
 // by q (low-nibble channels times 16) and, for V, by the output channel. Scale
 // and zero stay outside the products, in fp32:
 //   S = sum_g s_g * (sum_{ch in g} q c) + z_g * (sum_{ch in g} q)
-//   O = sum_pos (P s_g) (c - 8)  (P s_g / ref rounded to fp16)
+//   O = sum_pos (P s_g) (c - 8)  (P s_g inv_g rounded to fp16)
 //       + sum_pos P (z_g + 8 s_g)  (fp32)
-// with ref a running power of two >= every s seen, rescaled like the softmax's
-// running maximum, so bf16 scales of any exponent fit. The - 8 (one packed
+// with inv_g a power of two for each group that keeps every s_g inv_g seen at 2^7 or
+// less, rescaled like the softmax's running maximum, so bf16 scales of any exponent
+// fit and no group's depend on another's. The - 8 (one packed
 // subtraction of subnormals, exact) keeps the summands of O as small as the values
 // themselves: around c alone, the rounding of P s_g weighs about twice as much and a
 // long sum loses the digits that z then cancels.
-// A weight P s_g / ref below 2^-14 is an fp16 subnormal: off by at most 2^-25 of the
-// head's largest scale, whatever the group.
+// P is at most 2^8, so P s_g inv_g fits fp16; one below 2^-14 is a subnormal, off by at
+// most 2^-25 of its own 1 / inv_g, which is 2^-31 of the group's largest scale.
 // The z term of S is a product too: the sums of q, cut into 16-bit parts that
 // together carry fp32's digits, against the stored zeros. q is scaled per head by a
 // power of two into fp16's range (exact down to 2^-24 of the head's largest).
@@ -240,6 +241,8 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm)
   volatile int* last_flag = abort_flag + 1;
   volatile int* stage_bad = last_flag + 1;                         // [kStages]
   int* wsum = const_cast<int*>(stage_bad) + kStages;               // [8]
+  // [warp][4 groups]: inv, the scales' power of two (in registers it would spill)
+  float4* sinv = reinterpret_cast<float4*>(smem + kStages * kStageBytes + kMergeBytes + 128);
   uint4* sq = reinterpret_cast<uint4*>(smem + kStages * kStageBytes + kMergeBytes + 256);
   int32_t* P =
       reinterpret_cast<int32_t*>(smem + kStages * kStageBytes + kMergeBytes + 256 + kQBytes);
@@ -501,7 +504,11 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm)
     float o[8][4];   // [2 g + half][channel pair x head]: see the store below
     float zs[4][2];  // sum over positions of P z_g (this lane's rows)
     float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
-    float ref = __uint_as_float(1u << 23);  // 2^-126
+    if (lane == 0) {
+      const float most = __uint_as_float(253u << 23);  // 2^126
+      sinv[warp] = make_float4(most, most, most, most);
+    }
+    __syncwarp();
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
@@ -575,7 +582,7 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm)
           }
         }
         // V's meta of this lane's rows, and their largest scale (low halves)
-        uint32_t ve[2][2][4], top2 = 0;
+        uint32_t ve[2][2][4], top2[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
@@ -584,28 +591,28 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm)
                 *reinterpret_cast<const uint4*>(vm + (mt * 16 + k * 8 + sig) * kMetaBytes);
             ve[mt][k][0] = e.x, ve[mt][k][1] = e.y, ve[mt][k][2] = e.z, ve[mt][k][3] = e.w;
 #pragma unroll
-            for (int gi = 0; gi < 4; ++gi) top2 = max16x2<T>(top2, ve[mt][k][gi]);
+            for (int gi = 0; gi < 4; ++gi) top2[gi] = max16x2<T>(top2[gi], ve[mt][k][gi]);
           }
-        float smax, unused;
-        unpack2<T>(top2 & 0xffffu, smax, unused);
+        float4 inv4 = sinv[warp];
+        float smax[4], over = 0.f;
+#pragma unroll
+        for (int gi = 0; gi < 4; ++gi) {
+          float unused;
+          unpack2<T>(top2[gi] & 0xffffu, smax[gi], unused);
+          over = fmaxf(over, smax[gi] * (&inv4.x)[gi]);
+        }
         float mx[2] = {fmaxf(fmaxf(s[0][0], s[0][2]), fmaxf(s[1][0], s[1][2])),
                        fmaxf(fmaxf(s[0][1], s[0][3]), fmaxf(s[1][1], s[1][3]))};
         // The references move only when a score is 2^8 above its head's, or a
-        // scale above ref: P (at most 2^8) stays within fp16 and sums keep their
+        // scale above its group's: P (at most 2^8) stays within fp16 and sums keep their
         // precision, and most tiles need no exchange between lanes at all.
         if (__any_sync(0xffffffffu, mx[0] > m_run[0] + 8.f || mx[1] > m_run[1] + 8.f ||
-                                        smax > ref)) {
+                                        over > 128.f)) {
 #pragma unroll
           for (int x = 0; x < 2; ++x)
 #pragma unroll
             for (int off = 4; off <= 16; off <<= 1)
               mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], off));
-          // the next power of two above the largest scale of the warp's rows
-          const uint32_t top =
-              __reduce_max_sync(0xffffffffu, __float_as_uint(smax)) & 0x7f800000u;
-          const float ref_new = fmaxf(ref, __uint_as_float(min(top + 0x00800000u, 0x7f000000u)));
-          const float shrink = ref / ref_new;
-          ref = ref_new;
           float al[2];
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
@@ -614,23 +621,31 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm)
             m_run[x] = mn;
             l_run[x] *= al[x];
           }
-          const float f0 = al[0] * shrink, f1 = al[1] * shrink;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) o[i][0] *= f0, o[i][1] *= f1, o[i][2] *= f0, o[i][3] *= f1;
+          for (int gi = 0; gi < 4; ++gi) {
+            // 2^7 / the next power of two above the largest scale of the warp's rows,
+            // within normal numbers
+            const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(smax[gi])) >> 23;
+            const float was = (&inv4.x)[gi];
+            const float now = fminf(was, __uint_as_float(min(253u, 260u - top) << 23));
+            const float shrink = now * __uint_as_float(0x7f000000u - __float_as_uint(was));
+            const float f0 = al[0] * shrink, f1 = al[1] * shrink;
 #pragma unroll
-          for (int gi = 0; gi < 4; ++gi) zs[gi][0] *= al[0], zs[gi][1] *= al[1];
+            for (int i = 2 * gi; i < 2 * gi + 2; ++i)
+              o[i][0] *= f0, o[i][1] *= f1, o[i][2] *= f0, o[i][3] *= f1;
+            zs[gi][0] *= al[0], zs[gi][1] *= al[1];
+            (&inv4.x)[gi] = now;
+          }
+          __syncwarp();
+          if (lane == 0) sinv[warp] = inv4;
         }
-        const float inv = __uint_as_float(0x7f000000u - __float_as_uint(ref));  // 1 / 2^k
         const float mu[2] = {m_run[0] == -INFINITY ? 0.f : m_run[0],
                              m_run[1] == -INFINITY ? 0.f : m_run[1]};
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt) {
-          float p[4], pn[4];
+          float p[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            p[k] = exp2_ftz(s[mt][k] - mu[k & 1]);
-            pn[k] = p[k] * inv;
-          }
+          for (int k = 0; k < 4; ++k) p[k] = exp2_ftz(s[mt][k] - mu[k & 1]);
           l_run[0] += p[0] + p[2];
           l_run[1] += p[1] + p[3];
           // V codes of rows 2 t4, 2 t4 + 1 and 2 t4 + 8, 2 t4 + 9
@@ -646,8 +661,9 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm)
             float s0, z0, s1, z1;
             unpack2<T>(ve[mt][0][gi], s0, z0);
             unpack2<T>(ve[mt][1][gi], s1, z1);
-            const uint32_t b0 = transpose8x8(half2_bits(pn[0] * s0, pn[1] * s0));
-            const uint32_t b1 = transpose8x8(half2_bits(pn[2] * s1, pn[3] * s1));
+            const float w0 = s0 * (&inv4.x)[gi], w1 = s1 * (&inv4.x)[gi];
+            const uint32_t b0 = transpose8x8(half2_bits(p[0] * w0, p[1] * w0));
+            const uint32_t b1 = transpose8x8(half2_bits(p[2] * w1, p[3] * w1));
             z0 += 8.f * s0;
             z1 += 8.f * s1;
             zs[gi][0] += p[0] * z0 + p[2] * z1;
@@ -679,6 +695,8 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm)
         for (int gi = 0; gi < 4; ++gi)
           zs[gi][x] += __shfl_xor_sync(0xffffffffu, zs[gi][x], off);
       }
+    __syncwarp();
+    const float4 inv4 = sinv[warp];
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
       const int head = 2 * t4 + x;
@@ -689,8 +707,9 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm)
 #pragma unroll
       for (int gi = 0; gi < 4; ++gi) {
         const float z = zs[gi][x];
+        // 2^24 and 2^20 first: divided by inv they may be beyond fp32
+        const float ref = __uint_as_float(0x7f000000u - __float_as_uint((&inv4.x)[gi]));
         float4 f;
-        // 2^24 and 2^20 first: times ref they may be beyond fp32
         f.x = o[2 * gi][x] * 16777216.f * ref + z;
         f.y = o[2 * gi][2 + x] * 1048576.f * ref + z;
         f.z = o[2 * gi + 1][x] * 16777216.f * ref + z;
