@@ -14,14 +14,18 @@ __all__ = ["kv4_quantize", "kv4_pack", "kv4_unpack", "norm_rope", "grouped_atten
 def kv4_quantize(x: np.ndarray, kind: str):
     """x [..., 128] (any finite float32 values) -> codes uint8 [..., 4, 32], scale and
     zero [..., 4] (values of the 16-bit type ``kind``, as float32). The steps round
-    as the format says: differences and quotients in fp32, (s, z) to 16 bits."""
+    as the format says: differences and quotients in fp32, (s, z) to 16 bits. A
+    difference beyond fp32 is taken of halves, which rounds the same."""
     g = np.asarray(x, np.float32).reshape(*x.shape[:-1], 4, 32)
     top = np.float32(65504.0 if kind == "f16" else 3.3895313892515355e38)
     z = round16(np.clip(g.min(-1), -top, top), kind).astype(np.float32)
-    s = round16(np.clip((g.max(-1) - z) / np.float32(15), -top, top), kind).astype(np.float32)
-    step = np.where(s == 0, np.float32(1), s)
-    c = np.clip(np.rint((g - z[..., None]) / step[..., None]), 0, 15).astype(np.uint8)
-    return c, s, z
+    with np.errstate(over="ignore"):
+        half = np.where(np.isinf(g.max(-1) - z), np.float32(0.5), np.float32(1))
+    s = (g.max(-1) * half - z * half) / np.float32(15) / half
+    s = round16(np.clip(s, -top, top), kind).astype(np.float32)
+    step, half = np.where(s == 0, np.float32(1), s)[..., None], half[..., None]
+    y = (g * half - z[..., None] * half) / (step * half)
+    return np.clip(np.rint(y), 0, 15).astype(np.uint8), s, z
 
 
 def kv4_pack(codes: np.ndarray) -> np.ndarray:

@@ -119,18 +119,21 @@ PS_DEV void quantise_group(const float (&a)[8], const float (&b)[8], unsigned ma
   const float span = __fsub_rn(hi, z);
   float range = span * (1.f / 15.f);
   range = fmaf(fmaf(-15.f, range, span), 1.f / 15.f, range);
-  if (isinf(span)) range = hi / 15.f - z / 15.f;  // max - min beyond fp32
+  // max - min beyond fp32: differences of halves, whose rounding is the same
+  const bool wide = isinf(span);
+  const float half = wide ? 0.5f : 1.f;
+  if (wide) range = 2.f * __fdiv_rn(__fsub_rn(0.5f * hi, 0.5f * z), 15.f);
   T st = saturate<T>(range);
   float s = to_f32<T>(st);
   if (s == 0.f) s = 1.f;  // a constant group: every code 0
-  if (s < 1.1754944e-38f || isinf(span)) {
+  if (s < 1.1754944e-38f || wide) {
     // 1 / s or a difference may not exist in fp32: divide
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       word[k] = 0;
 #pragma unroll
       for (int i = 7; i >= 0; --i) {
-        const float y = __fdiv_rn(__fsub_rn(k ? b[i] : a[i], z), s);
+        const float y = __fdiv_rn(__fsub_rn(half * (k ? b[i] : a[i]), half * z), half * s);
         word[k] = word[k] * 16u + (uint32_t)rintf(fminf(fmaxf(y, 0.f), 15.f));
       }
     }

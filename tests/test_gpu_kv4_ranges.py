@@ -94,3 +94,63 @@ def test_groups_of_different_scales(dt, ratio, top):
     err = np.abs(to_np(out).reshape(M, nh, 128) - want)
     assert np.all(err <= tol), float((err / tol).max())
     assert _status() == 0
+
+
+def _codes(x, dt):
+    """Codes, scale and zero of a row [128] as kv4_append stores them."""
+    import oracle
+    from parallel_serve_b200 import KV4Pool, ops
+    pool = KV4Pool.zeros(1, 1, 8, dt, DEV)
+    x = x.to(dt).view(1, 1, 128).to(DEV)
+    ops.kv4_append(x, x, (pool, None), torch.zeros(1, dtype=torch.int32, device=DEV))
+    meta = to_np(pool.k_meta)[0, 0, 0]
+    ident = np.stack([np.ones(4), np.zeros(4)], -1)                   # s = 1, z = 0: the codes
+    c = oracle.kv4_unpack(pool.k_codes.cpu().numpy()[0, 0, 0], ident).reshape(4, 32)
+    assert torch.equal(pool.k_codes, pool.v_codes) and torch.equal(pool.k_meta, pool.v_meta)
+    return c, meta[:, 0], meta[:, 1]
+
+
+def _exact(x, dt):
+    """The format's definition in 64 bits (the inputs here leave no quotient within 2^-20
+    of a half, which the test checks)."""
+    g = to_np(x.to(dt)).reshape(4, 32)
+    z = to_np(torch.from_numpy(g.min(-1)).to(dt))
+    s = to_np(torch.from_numpy((g.max(-1) - z) / 15).to(dt))
+    y = (g - z[:, None]) / np.where(s == 0, 1, s)[:, None]
+    return np.clip(np.rint(y), 0, 15), s, z, np.abs(y - np.floor(y) - 0.5).min()
+
+
+def test_groups_wider_than_fp32():
+    """bf16 groups whose largest and smallest value are more than fp32's range apart."""
+    dt, top = torch.bfloat16, torch.finfo(torch.bfloat16).max
+    x = torch.linspace(-1, 1, 32).double().repeat(4, 1) * top
+    x[1] *= 0.8
+    x[2] = x[2].flip(0) * 0.6
+    x[3, 1:] *= 0.01                                   # one value far below the others
+    c, s, z = _codes(x, dt)
+    want, ws, wz, margin = _exact(x.flatten(), dt)
+    assert margin > 2.0 ** -20
+    assert np.array_equal(z, wz) and np.array_equal(s, ws) and np.array_equal(c, want)
+    assert _status() == 0
+
+
+@pytest.mark.parametrize("e", [-130, -126, -124, -122, -115, -101, -90])
+def test_groups_of_tiny_values(e):
+    """bf16 groups whose step is near fp32's smallest normal number: the codes of a
+    division, ties included (fp32 holds these quotients' operands exactly)."""
+    import oracle
+    dt = torch.bfloat16
+    g = torch.Generator().manual_seed(3)
+    for _ in range(8):
+        x = (torch.randn(128, generator=g).to(dt).double() * 2.0 ** e).to(dt)
+        c, s, z = _codes(x, dt)
+        wc, ws, wz = oracle.kv4_quantize(to_np(x).astype(np.float32), KIND[dt])
+        assert np.array_equal(s, ws) and np.array_equal(z, wz) and np.array_equal(c, wc)
+        # halves of the step on purpose: 15 steps, then odd multiples of half a step
+        step = 2.0 ** e
+        y = torch.arange(32).double().repeat(4) * step / 2
+        y[31::32] = 15 * step
+        c, s, z = _codes(y, dt)
+        wc, ws, wz = oracle.kv4_quantize(to_np(y.to(dt)).astype(np.float32), KIND[dt])
+        assert np.array_equal(s, ws) and np.array_equal(z, wz) and np.array_equal(c, wc)
+    assert _status() == 0
