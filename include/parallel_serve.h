@@ -477,7 +477,7 @@ int ps_kv4_gather(const ps_kv4_cache_t* cache, const int32_t* seqs, const int32_
  * n_kv_heads; query head h reads KV head h / (n_heads / n_kv_heads)):
  * out[j, h] = softmax(q[j, h] . K[0..pos[j]] * scale) V[0..pos[j]]. q
  * [M, n_heads, 128] with a token stride, out [M, n_heads * 128]; rows as in
- * ps_kv4_append; max_len bounds pos[j] + 1. A token whose position, row or page
+ * ps_kv4_append; max_len bounds pos[j] + 1; |scale| < 2e38. A token whose position, row or page
  * is out of range sets PS_ERR_BAD_INDEX and its output stays unwritten.
  * The workspace starts with 4096 bytes of counters: zero them once before the
  * first use, calls leave them zero, so calls of any shapes may follow one
@@ -497,7 +497,7 @@ int ps_kv4_decode_attention(const void* q, long long q_stride, const ps_kv4_cach
  * 0 .. r + (lk - lq), where keys that precede the queries are a history. out
  * [Tq, n_heads, 128]; a query that sees no key gets 0, rows outside every
  * sequence stay as they were. Token strides in elements (multiples of 8, heads
- * contiguous); scale > 0. cu_q and cu_k are device arrays, nondecreasing; a
+ * contiguous); 0 < scale < 2e38. cu_q and cu_k are device arrays, nondecreasing; a
  * sequence whose range leaves [0, Tq] or [0, Tk] sets PS_ERR_BAD_INDEX and is
  * skipped. */
 int ps_prompt_attention(const void* q, long long q_stride, const void* k, long long k_stride,

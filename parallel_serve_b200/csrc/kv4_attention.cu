@@ -831,6 +831,7 @@ extern "C" int ps_kv4_decode_attention(const void* q, long long q_stride,
   PS_CHECK_ARG(M >= 0 && n_heads > 0 && n_heads % n_kv == 0 && max_len > 0);
   PS_CHECK_ARG(max_len <= (cache->block_table ? cache->max_pages * cache->page_size : cache->L_cap));
   PS_CHECK_ARG(dtype == PS_DTYPE_F16 || dtype == PS_DTYPE_BF16);
+  PS_CHECK_ARG(scale > -kMaxScale && scale < kMaxScale);  // NaN fails both
   if (!counts) PS_CHECK_ARG(split_point >= 0 && split_point <= M);
   if (M == 0) return PS_OK;
   PS_CHECK_ARG(q && out && pos && aligned16(q) && q_stride >= (long long)n_heads * kv4::kD &&

@@ -706,7 +706,7 @@ extern "C" int ps_prompt_attention(const void* q, long long q_stride, const void
   PS_CHECK_ARG(n_seqs >= 0 && Tq >= 0 && Tk >= 0 && n_heads > 0 && n_kv_heads > 0 &&
                n_heads % n_kv_heads == 0);
   PS_CHECK_ARG(dtype == PS_DTYPE_F16 || dtype == PS_DTYPE_BF16);
-  PS_CHECK_ARG(scale > 0.f && scale < 3.0e38f);
+  PS_CHECK_ARG(scale > 0.f && scale < kMaxScale);
   if (n_seqs == 0 || Tq == 0) return PS_OK;
   PS_CHECK_ARG(q && out && cu_q && cu_k && aligned16(q) && aligned16(out));
   PS_CHECK_ARG(Tk == 0 || (k && v && aligned16(k) && aligned16(v)));

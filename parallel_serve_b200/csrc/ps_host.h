@@ -19,6 +19,9 @@ namespace ps {
 constexpr size_t kCounterRegionBytes = 256 * 1024;
 constexpr int kMaxCounters = (int)(kCounterRegionBytes / 4);
 
+// Softmax scales are taken below this: times log2 e they are still finite in fp32.
+constexpr float kMaxScale = 2.0e38f;
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 inline int round_up(int v, int m) { return (v + m - 1) / m * m; }

@@ -724,6 +724,10 @@ def kv4_decode_attention(q: torch.Tensor, pools: tuple, pos: torch.Tensor, *, ma
         raise ValueError(f"{nh} query heads do not divide over {nkv} KV heads")
     if not 0 < max_len <= cap:
         raise ValueError(f"max_len must be in [1, {cap}]")
+    if scale is None:
+        scale = 0.08838834764831845
+    elif not -2e38 < scale < 2e38:
+        raise ValueError("scale must be finite, its magnitude below 2e38")
     if out is None:
         out = q.new_empty((M, nh * _HD))
     else:
@@ -743,8 +747,7 @@ def kv4_decode_attention(q: torch.Tensor, pools: tuple, pos: torch.Tensor, *, ma
         raise ValueError(f"workspace must be a contiguous tensor on cuda:{idx}")
     _call(lib.ps_kv4_decode_attention, "ps_kv4_decode_attention", idx, q.data_ptr(), qs, cache,
           out.data_ptr(), pp, home, cnt, split, M, nh, max_len,
-          0.08838834764831845 if scale is None else scale, code, workspace.data_ptr(),
-          workspace.nbytes)
+          scale, code, workspace.data_ptr(), workspace.nbytes)
     return out
 
 
@@ -783,8 +786,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
         raise ValueError("cu_q and cu_k must have the same length")
     if scale is None:
         scale = 0.08838834764831845
-    elif not 0.0 < scale < 3e38:
-        raise ValueError("scale must be positive and finite")
+    elif not 0.0 < scale < 2e38:
+        raise ValueError("scale must be positive and below 2e38")
     if out is None:
         out, os_ = q.new_empty((Tq, nh * _HD)), nh * _HD
     else:

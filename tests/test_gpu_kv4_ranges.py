@@ -154,3 +154,25 @@ def test_groups_of_tiny_values(e):
         wc, ws, wz = oracle.kv4_quantize(to_np(y.to(dt)).astype(np.float32), KIND[dt])
         assert np.array_equal(s, ws) and np.array_equal(z, wz) and np.array_equal(c, wc)
     assert _status() == 0
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("scale", [-0.1, 0.0, 3.0])
+def test_scales_of_either_sign(dt, scale):
+    """Scores reach some 100 at scale 3: |log2 p| <= 256 at 2^-24, 2^-13 of each term in place
+    of the 2^-14 of scores around 1."""
+    import oracle
+    from parallel_serve_b200 import ops
+    lens = [300]
+    pools, table, *_ = _filled(lens, 1, 1, dt, 0, 300, 85)
+    q = cpu_randn((1, 4, 128), 86, 1.0, dt)
+    pos = torch.tensor([299], dtype=torch.int32, device=DEV)
+    out = ops.kv4_decode_attention(q.to(DEV), pools, pos, max_len=300, scale=scale)
+    ks, vs = (_stored(pools, table, lens, 1, 0, part)[0] for part in "kv")
+    want, size = oracle.grouped_attention(to_np(q), ks, vs, scale=scale)
+    tol = torch.finfo(dt).eps / 2 * np.abs(want) + (2.0 ** -10 + 2.0 ** -13) * (size + np.abs(vs).max())
+    assert np.all(np.abs(to_np(out).reshape(want.shape) - want) <= tol)
+    for bad in (float("nan"), float("inf"), -2.5e38):
+        with pytest.raises(ValueError):
+            ops.kv4_decode_attention(q.to(DEV), pools, pos, max_len=300, scale=bad)
+    assert _status() == 0
