@@ -692,8 +692,11 @@ def kv4_gather(pools: tuple, seqs: torch.Tensor, cu: torch.Tensor, total: int, *
 def _counter_workspace(like: torch.Tensor, idx: int, nbytes: int, tag: str,
                        counter_bytes: int) -> torch.Tensor:
     """Workspace whose first ``counter_bytes`` are zero at rest. Under graph capture
-    a workspace of the graph's own (two captured graphs may run at the same
-    time), else the stream's."""
+    (of device idx's current stream, whichever device is current) a workspace of
+    the graph's own (two captured graphs may run at the same time), else the stream's."""
+    if _current_device() != idx:
+        with torch.cuda.device(idx):
+            return _counter_workspace(like, idx, nbytes, tag, counter_bytes)
     if torch.cuda.is_current_stream_capturing():
         ws = like.new_empty(nbytes, dtype=torch.uint8)
         ws[:counter_bytes].zero_()

@@ -22,3 +22,28 @@ def test_scales_of_a_decode_call():
     for scale in (0.1, 0.0, -3.0, 1e38):
         assert _lib.lib.ps_kv4_decode_attention(P, 1024, cache(), P, P, None, None, 0, 0, 8, 64, scale,
                                                 0, None, 0, None, None) == 0
+
+
+def test_a_captured_stream_of_another_device_gets_its_own_workspace(monkeypatch):
+    """Whether a call is captured is asked of its tensors' device, not of the current one."""
+    now = [0]
+
+    class Device:
+        def __init__(self, idx):
+            self.idx = idx
+
+        def __enter__(self):
+            self.was, now[0] = now[0], self.idx
+
+        def __exit__(self, *a):
+            now[0] = self.was
+    shared = torch.zeros(1)
+    monkeypatch.setattr(ops, "_current_device", lambda: now[0])
+    monkeypatch.setattr(ops, "_raw_stream", lambda idx: 7)
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: now[0] == 1)
+    monkeypatch.setattr(_lib, "stream_workspace", lambda idx, stream, nbytes, tag: shared)
+    like = torch.zeros(1)
+    assert ops._counter_workspace(like, 0, 5000, "x", 4096) is shared
+    ws = ops._counter_workspace(like, 1, 5000, "x", 4096)
+    assert ws is not shared and ws.numel() == 5000 and bool((ws[:4096] == 0).all()) and now == [0]
