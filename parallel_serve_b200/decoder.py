@@ -449,6 +449,9 @@ class TwoModelDecoder:
         L = k.shape[2]
         if self.kv_bits == 4:
             n, (seqs, _) = k.shape[0], self._kv4_sequences(model, L)
+            if n != self.counts_host[model] or v.shape != k.shape:
+                raise ValueError(f"model {model} has {self.counts_host[model]} sequences; k and v have "
+                                 "the same shape")
             if L == 0 or n == 0:
                 return
             pos = torch.arange(L, dtype=torch.int32, device=self.device).repeat(n)
@@ -502,6 +505,12 @@ class TwoModelDecoder:
         """(seqs, cu) of positions [0, L) of every sequence of one model, as kv4_gather takes them."""
         n = self.counts_host[model]
         base = 0 if model == 0 or self.block_table is None else self.counts_host[0]
+        if L > self.L_cap:
+            raise ValueError(f"{L} positions, a sequence has at most {self.L_cap}")
+        if self.block_table is not None:
+            if any(len(self.block_table.pages_of(base + s)) * self.page_size < L for s in range(n)):
+                raise ValueError("reserve pages for the history first")
+            self.block_table.sync()
         seqs = torch.tensor([[model, base + s, 0] for s in range(n)], dtype=torch.int32,
                             device=self.device).view(n, 3)
         return seqs, torch.arange(n + 1, dtype=torch.int32, device=self.device) * L

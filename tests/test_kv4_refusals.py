@@ -47,3 +47,41 @@ def test_a_captured_stream_of_another_device_gets_its_own_workspace(monkeypatch)
     assert ops._counter_workspace(like, 0, 5000, "x", 4096) is shared
     ws = ops._counter_workspace(like, 1, 5000, "x", 4096)
     assert ws is not shared and ws.numel() == 5000 and bool((ws[:4096] == 0).all()) and now == [0]
+
+
+def _decoder(page_size=None):
+    """A decoder's bookkeeping alone: 2 sequences of model 0 and 1 of model 1, 64 positions."""
+    from parallel_serve_b200.decoder import TwoModelDecoder
+    from parallel_serve_b200.paged_kv import BlockTable, PageAllocator
+    dec = TwoModelDecoder.__new__(TwoModelDecoder)
+    dec.device, dec.dt, dec.nh, dec.kv_bits = torch.device("cpu"), torch.float16, 2, 4
+    dec.counts_host, dec.L_cap, dec.page_size, dec.block_table = (2, 1), 64, page_size, None
+    if page_size:
+        dec.block_table = BlockTable([0, 0, 1], (PageAllocator(8), PageAllocator(4)), 64 // page_size,
+                                     page_size)
+    return dec
+
+
+def test_a_history_needs_its_room():
+    """Positions beyond the capacity, pages that are not reserved and sequences that the model does
+    not have were left out of the cache in silence."""
+    dec, kv = _decoder(), lambda n, L: (torch.zeros(n, 2, L, 128),) * 2
+    for n, L in ((2, 65), (1, 4), (3, 4)):
+        with pytest.raises(ValueError):
+            dec.write_kv(0, 0, *kv(n, L))
+    with pytest.raises(ValueError):
+        dec.write_kv(0, 0, kv(2, 4)[0], kv(2, 5)[0])
+    with pytest.raises(ValueError):
+        dec.read_kv(0, 1, 65)
+    dec = _decoder(16)
+    with pytest.raises(ValueError):
+        dec.write_kv(0, 0, *kv(2, 4))
+    with pytest.raises(ValueError):
+        dec.read_kv(0, 1, 4)
+    dec.block_table.ensure(range(3), 20)             # reserved on the host, not yet on the device
+    seqs, cu = dec._kv4_sequences(0, 32)
+    assert seqs.tolist() == [[0, 0, 0], [0, 1, 0]] and cu.tolist() == [0, 32, 64]
+    assert torch.equal(dec.block_table.device, torch.from_numpy(dec.block_table.host))
+    with pytest.raises(ValueError):
+        dec._kv4_sequences(1, 33)
+    dec.write_kv(0, 0, *kv(2, 0))                    # no positions: nothing to do
