@@ -222,6 +222,10 @@ class TwoModelDecoder:
             raise ValueError(f"kv_bits must be 4 or 16, got {kv_bits}")
         if kv_bits == 4 and chain:
             raise ValueError("the projection chain appends to 16-bit pools: kv_bits=4 runs without it")
+        if kv_bits == 4 and page_size is not None and \
+                (not 8 <= page_size <= 4096 or page_size & (page_size - 1)):
+            raise ValueError("kv_bits=4 takes pages of a power of two in [8, 4096] positions, "
+                             f"got {page_size}")
         self.kv_bits = kv_bits
         dev, dt = self.device, self.dt
         H, FF, V = cfg.hidden, cfg.ffn, cfg.vocab

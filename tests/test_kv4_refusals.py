@@ -85,3 +85,12 @@ def test_a_history_needs_its_room():
     with pytest.raises(ValueError):
         dec._kv4_sequences(1, 33)
     dec.write_kv(0, 0, *kv(2, 0))                    # no positions: nothing to do
+
+
+@pytest.mark.parametrize("page_size", [4, 12, 8192])
+def test_page_sizes_of_a_4_bit_decoder(page_size):
+    """Refused where it is made, not at the first step, and before anything is allocated."""
+    from parallel_serve_b200.decoder import DecoderConfig, TwoModelDecoder
+    cfg = DecoderConfig(n_layers=1, hidden=256, n_heads=2, ffn=256, vocab=256)
+    with pytest.raises(ValueError, match="power of two"):
+        TwoModelDecoder(cfg, [0, 1], 64, kv_bits=4, page_size=page_size)
