@@ -663,6 +663,8 @@ def kv4_gather(pools: tuple, seqs: torch.Tensor, cu: torch.Tensor, total: int, *
     position) fills rows ``cu[i]`` to ``cu[i + 1]`` (``cu`` int32 [n + 1] on the
     device). Rows behind the last sequence are left as ``out`` had them.
     """
+    if len(pools) != 2:
+        raise ValueError("pools are (model 0's, model 1's), either may be None")
     p = pools[0] if pools[0] is not None and pools[0][0].shape[0] else pools[1]
     if p is None:
         raise ValueError("at least one model needs a 4-bit pool")

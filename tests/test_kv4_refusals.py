@@ -94,3 +94,13 @@ def test_page_sizes_of_a_4_bit_decoder(page_size):
     cfg = DecoderConfig(n_layers=1, hidden=256, n_heads=2, ffn=256, vocab=256)
     with pytest.raises(ValueError, match="power of two"):
         TwoModelDecoder(cfg, [0, 1], 64, kv_bits=4, page_size=page_size)
+
+
+def test_gather_takes_two_pools():
+    from parallel_serve_b200 import KV4Pool
+    pool = KV4Pool.zeros(2, 1, 8, device="cpu")
+    none = KV4Pool.zeros(0, 1, 8, device="cpu")
+    seqs, cu = torch.zeros(1, 3, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    for pools in ((), (None,), (none,), (pool,), (pool, None, None), (None, None)):
+        with pytest.raises(ValueError):
+            ops.kv4_gather(pools, seqs, cu, 0)
