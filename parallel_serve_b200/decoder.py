@@ -185,7 +185,8 @@ class TwoModelDecoder:
     160 bytes per position and head instead of 512. The QKV projection then
     writes a plain qkv row, ``ops.kv4_append`` rotates and quantises it, and
     attention reads the quantised history, in the prefill too (read back and
-    packed per chunk), so chunk boundaries do not change the result.
+    packed per chunk), so a prompt's result does not depend on its chunks beyond
+    rounding (their products have other shapes, and a code may move by one).
     """
 
     def __init__(self, cfg: DecoderConfig, model_id, L_cap: int, *, device="cuda",
