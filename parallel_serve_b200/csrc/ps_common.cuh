@@ -380,11 +380,6 @@ PS_DEV uint64_t f32x2_add(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
-PS_DEV uint64_t f32x2_mul(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
 
 // 32 bytes, a whole sector, in one store; p is 32-byte aligned.
 PS_DEV void st_32bytes(void* p, const uint32_t (&w)[8]) {

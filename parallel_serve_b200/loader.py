@@ -34,7 +34,7 @@ def decoder_config_from_hf(hf: Mapping | object, dtype: torch.dtype = torch.floa
     nkv = int(get("num_key_value_heads") or nh)
     if nkv != nh:
         raise ValueError(f"grouped-query attention ({nkv} KV heads for {nh} query heads) "
-                         "is not supported by the decode kernels")
+                         "is not supported by TwoModelDecoder")
     theta = get("rope_theta")
     if theta is None:
         rp = get("rope_parameters") or get("rope_scaling") or {}
@@ -50,7 +50,7 @@ def _layer(sd: Mapping[str, torch.Tensor], i: int) -> dict:
     q, k, v, o = (sd[p + f"self_attn.{n}_proj.weight"] for n in "qkvo")
     gate, up, down = (sd[p + f"mlp.{n}_proj.weight"] for n in ("gate", "up", "down"))
     if k.shape != q.shape or v.shape != q.shape:
-        raise ValueError("grouped-query attention is not supported by the decode kernels")
+        raise ValueError("grouped-query attention is not supported by TwoModelDecoder")
     return dict(W_qkv=torch.cat([q, k, v], dim=0).t(), W_o=o.t(),
                 W_gu=torch.cat([gate, up], dim=0).t(), W_d=down.t(),
                 ln1=sd[p + "input_layernorm.weight"], ln2=sd[p + "post_attention_layernorm.weight"])
