@@ -409,7 +409,8 @@ int ps_prefill_attention(const void* q, const void* k_pool0, const void* v_pool0
  * (nullable); rope tables [rope_len][rotary_dim / 2] fp32 (nullable: no
  * rotation); rotary_dim a multiple of 16. Pairs are (i, i + rotary_dim / 2), or
  * (2i, 2i + 1) when interleaved. fp32 arithmetic, one rounding at the end. A row
- * may be written in place (q_out == q, k_out == k). q may be NULL with q_out. A
+ * may be written in place (q_out == q with its stride, k_out == k with its); outputs
+ * overlap inputs in no other way. q may be NULL with q_out. A
  * position outside [0, rope_len) (negative, without tables) sets
  * PS_ERR_BAD_INDEX and leaves the token's rows unwritten.
  * ------------------------------------------------------------------------- */
@@ -477,8 +478,10 @@ int ps_kv4_gather(const ps_kv4_cache_t* cache, const int32_t* seqs, const int32_
  * n_kv_heads; query head h reads KV head h / (n_heads / n_kv_heads)):
  * out[j, h] = softmax(q[j, h] . K[0..pos[j]] * scale) V[0..pos[j]]. q
  * [M, n_heads, 128] with a token stride, out [M, n_heads * 128]; rows as in
- * ps_kv4_append; max_len bounds pos[j] + 1; |scale| < 2e38. A token whose position, row or page
- * is out of range sets PS_ERR_BAD_INDEX and its output stays unwritten.
+ * ps_kv4_append; max_len bounds pos[j] + 1; |scale| < 2e38. A token whose position,
+ * row or page is out of range sets PS_ERR_BAD_INDEX and its output stays unwritten.
+ * Sums are fp32; a weight times its group's scale is rounded to fp16 (2^-11 of it) before
+ * it meets the codes. Sums of weight x value, weights up to 2^8, have to fit fp32.
  * The workspace starts with 4096 bytes of counters: zero them once before the
  * first use, calls leave them zero, so calls of any shapes may follow one
  * another on it. Calls that may overlap need workspaces of their own. */
@@ -497,9 +500,11 @@ int ps_kv4_decode_attention(const void* q, long long q_stride, const ps_kv4_cach
  * 0 .. r + (lk - lq), where keys that precede the queries are a history. out
  * [Tq, n_heads, 128]; a query that sees no key gets 0, rows outside every
  * sequence stay as they were. Token strides in elements (multiples of 8, heads
- * contiguous); 0 < scale < 2e38. cu_q and cu_k are device arrays, nondecreasing; a
- * sequence whose range leaves [0, Tq] or [0, Tk] sets PS_ERR_BAD_INDEX and is
- * skipped. */
+ * contiguous); 0 < scale < 2e38; out overlaps no input. cu_q and cu_k are device
+ * arrays, nondecreasing; a sequence whose range leaves [0, Tq] or [0, Tk] sets
+ * PS_ERR_BAD_INDEX and is skipped. Sums are fp32, the weights are rounded to the 16-bit
+ * type for their product with v. A value of v that is not finite makes its channel so
+ * (an infinity, or NaN where its weight rounds to 0) for the queries that see its key. */
 int ps_prompt_attention(const void* q, long long q_stride, const void* k, long long k_stride,
                         const void* v, long long v_stride, void* out, long long o_stride,
                         const int32_t* cu_q, const int32_t* cu_k, int n_seqs, int Tq, int Tk,

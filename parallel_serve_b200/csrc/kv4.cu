@@ -1,7 +1,8 @@
 // Head norms + position rotation in one pass, the 4-bit cache's write and its
 // read-back (format: kv4.cuh). Elementwise work on 128-channel rows: what bounds
 // all three is memory traffic, so every row is read once and written once, 16
-// bytes a lane.
+// bytes a lane. (One exception: half-layout pairs of a part of the head lie in different
+// lanes, and the other channel's chunk is read a second time, out of L1.)
 //
 // Norm, rotation and write: four lanes own a row. Lane q has the 16-byte chunks 2q,
 // 2q + 1, 2q + 8 and 2q + 9, so both channels of a pair (i, i + 64) of the whole-head
@@ -9,11 +10,12 @@
 // lanes: what a group takes beside its channels (its zero, scale and reciprocal)
 // is done by two lanes, not by four with four times the calls. Instructions bounded
 // the write with 16 lanes to a row: writing and reading back 16 prompts of up to 2048
-// tokens with 32 + 32 heads took 575 us, with four lanes 382 (the bytes alone 299);
+// tokens with 32 + 32 heads took 575 us, with four lanes for the write 382, with four for
+// the read-back, too, 368 (367 to 390 on different GPUs; the bytes alone 299);
 // norm and rotation of 16384 tokens with 32 + 8 heads 74 and 63 (52). A block takes a
 // few tokens; each quad takes every Q-th of its token's rows, loads one ahead, and
 // keeps the token's cos / sin in registers.
-// What it reaches now is 5.1 TB/s (append) to 5.4 (norm and rotation alone). Measured and
+// What it reaches now is 5.1 TB/s (append) to 5.5 (norm and rotation alone). Measured and
 // not kept: rows three ahead through a shared-memory ring (382 us, write + read 372
 // otherwise), 32-byte loads (no change; 32-byte stores: 63 and 61 us), cos / sin read again for each row (61 us
 // for norm and rotation alone, ragged write + read 74 instead of 72), fewer registers

@@ -40,11 +40,13 @@
 // last CTA to finish a piece of an item merges the pieces in order, so results
 // do not depend on timing.
 //
-// 64 sequences of 2048 positions, 32 heads: 161 us, 4.2 TB/s (the bytes alone 102 us
-// at the measured copy rate; loads without arithmetic take 109, with the K side 117).
+// 64 sequences of 2048 positions, 32 heads: 164 to 168 us on different GPUs, 4.0 to 4.1 TB/s
+// (the bytes alone 102 us at the measured copy rate; loads without arithmetic take
+// 109, with the K side 117). One power of two for all groups' scales saves 3 us of it (161
+// and 164), and loses the unlikely keys of a group whose scales are far below another's.
 // Instructions bound it, and their costs add up: per SM sub-partition a product takes
 // 8 cycles and an AND or shift 2, so that unpacking costs as much as multiplying.
-// Measured and not kept: two CTAs of one SM with the same stages (161 us), a ring per
+// Measured and not kept (beside 161 us, with one power of two): two CTAs of one SM with the same stages (161 us), a ring per
 // warp without a producer (193; with four CTAs 252), q in registers (no gain), the - 8
 // as a second product with a constant operand (177), tcgen05 products over tiles
 // unpacked into shared memory (192 with two CTAs, 211 with three: unpacked, a tile
@@ -226,7 +228,7 @@ PS_DEV Piece piece_at(const AttnArgs& a, const int32_t* first, int entries, int 
   return p;
 }
 
-// Merged softmax state of up to 8 heads x 128 channels, one thread a channel.
+// One CTA: its range of tiles, piece by piece. Warps 0 to 3 compute, warp 4 loads.
 template <typename T>
 __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm)
     kv4_decode_attention_kernel(const AttnArgs a) {

@@ -21,7 +21,7 @@
 //                   one warp run in order, so no barrier says that.
 // TMEM: S, 128 fp32 columns a tile, then O, 128 a tile.
 //
-// 16384 tokens, 32 + 8 heads: 1.98 ms, 1.11 PFLOP/s. Of the 3500 cycles of a block
+// 16384 tokens, 32 + 8 heads: 1.99 to 2.06 ms on different GPUs, 1.07 to 1.10 PFLOP/s. Of the 3500 cycles of a block
 // of both tiles products take 2050, and at 1 kW the SM clock is at 1.55 GHz, so what
 // shortens the cycles without saving energy gains nothing. Measured and not kept:
 //   P by polynomial on the FMA pipe for a quarter of the keys, scores prefetched
@@ -84,16 +84,16 @@ struct Args {
   int32_t* status;
 };
 
-// The MMA warp runs as one: every lane computes the same operands and waits on
-// the same barriers, and the instructions themselves are predicated to one lane.
-// Inside a single-lane branch each operand would have to be moved to a uniform
-// register first, which made issuing a product take longer than the product
-// (155 instead of 64 cycles).
 // A value that all lanes share, known as such to the compiler (a warp reduction
 // ends in a uniform register): loops over it and addresses made from it stay in
 // the uniform data path, which the product instructions take their operands from.
 PS_DEV uint32_t uniform(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
 
+// The MMA warp runs as one: every lane computes the same operands and waits on
+// the same barriers, and the instructions themselves are predicated to one lane.
+// Inside a single-lane branch each operand would have to be moved to a uniform
+// register first, which made issuing a product take longer than the product
+// (155 instead of 64 cycles).
 // D[tmem] (+)= A[smem desc] * B[smem desc], kind::f16.
 PS_DEV void mma_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
                    uint32_t accumulate) {
@@ -538,7 +538,7 @@ __global__ void __launch_bounds__(Shape<kTiles>::kThreads, Shape<kTiles>::kCtas)
     const int t = kTiles > 1 ? warp >> 2 : 0;
     const int r = (warp & 3) * 32 + lane;  // TMEM lane = row of the tile
     const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
-      const uint32_t o_addr = tmem + kTmemO + t * kD + lane_off;
+    const uint32_t o_addr = tmem + kTmemO + t * kD + lane_off;
     const int first = it.row + t * kTile;
     const int row = first + r;
     const int my_nb = t ? nb1 : nb0;
@@ -719,7 +719,11 @@ extern "C" int ps_prompt_attention(const void* q, long long q_stride, const void
   // (64 prompts of 64 to 128 tokens, 32 + 8 heads: 65 us, one CTA of two tiles 118; 8 of
   // 512 to 1024: 81 and 101); two tiles read each K and V block once for twice the
   // queries, which wins behind some 4096 (one prompt of 4096: 138 and 140 us, of 8192:
-  // 547 and 515, of 16384: 2084 and 1976).
+  // 547 and 515, of 16384: 2084 and 1976; with 32 + 32 heads of 4096: 158 and 172, of
+  // 8192: 524 and 508, of 16384: 2157 and 1948). The rule looks at keys alone: with few
+  // queries behind them one tile stays ahead by 1 to 6% (256 queries behind 8192 keys: 130 and
+  // 138 us, behind 16384: 245 and 255, behind 65536: 915 and 946), and a long prompt among
+  // many short ones gets one (one of 16384 and 31 of 64: 2082 and 2014).
   const bool one = Tk <= 4096ll * n_seqs;
   const int rows = pra::kTile * (one ? 1 : 2);
   const long long grid = ((long long)Tq / rows + n_seqs) * n_heads;

@@ -565,8 +565,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, pos: torch.Tensor, *,
     rotary_dim channels, as pairs (i, i + rotary_dim / 2), or (2i, 2i + 1) when
     ``interleaved``. Tokens are in routed order: the first ``split_point`` (or
     counts[0], read on the device; default: all) belong to model 0.
-    ``q_out`` / ``k_out`` may be the inputs themselves. A position outside the
-    tables raises PS_ERR_BAD_INDEX in the status word and leaves its rows unwritten.
+    ``q_out`` may be ``q`` itself and ``k_out`` ``k``; they overlap the inputs in no other
+    way. A position outside the tables raises PS_ERR_BAD_INDEX in the status word and leaves its rows unwritten.
     """
     idx, code = _first(q)
     dt = q.dtype
@@ -613,8 +613,8 @@ def kv4_append(k: torch.Tensor, v: torch.Tensor, pools: tuple, pos: torch.Tensor
     ``block_table`` [rows, max_pages] to the pages of table row ``rows[j]``
     (default: j). Norms and rotation as in ``qk_norm_rope`` (all optional) happen
     in the same pass: k is quantised from their fp32 result, ``q`` (optional)
-    returns in 16 bits. Two tokens of a call must not share a position of a
-    sequence. Returns q_out, or None without ``q``.
+    returns in 16 bits (``q_out`` may be ``q`` itself). Two tokens of a call must not
+    share a position of a sequence. Returns q_out, or None without ``q``.
     """
     idx, code = _first(k)
     dt = k.dtype
@@ -661,7 +661,8 @@ def kv4_gather(pools: tuple, seqs: torch.Tensor, cu: torch.Tensor, total: int, *
 
     Sequence i (``seqs`` int32 [n, 3]: model, slot or block-table row, first
     position) fills rows ``cu[i]`` to ``cu[i + 1]`` (``cu`` int32 [n + 1] on the
-    device). Rows behind the last sequence are left as ``out`` had them.
+    device). Rows of no sequence are left as ``out`` had them; without ``out`` they hold
+    whatever the memory did.
     """
     if len(pools) != 2:
         raise ValueError("pools are (model 0's, model 1's), either may be None")
@@ -719,7 +720,9 @@ def kv4_decode_attention(q: torch.Tensor, pools: tuple, pos: torch.Tensor, *, ma
     ``split_point`` and ``counts`` as in ``kv4_append``; ``max_len`` bounds
     pos[j] + 1. ``workspace`` (default: the stream's own) has
     ps_kv4_decode_attention_workspace_bytes bytes, the first 4096 zero before its
-    first use. Returns [M, n_heads * 128].
+    first use; without one, a call that is captured into a graph zeroes its own (one
+    launch more a replay). ``scale`` is any finite number below 2e38 in magnitude
+    (default: 128^-1/2). Returns [M, n_heads * 128].
     """
     idx, code = _first(q)
     dt = q.dtype
@@ -766,8 +769,9 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     the same rows) of ``k``, ``v`` [keys, n_kv_heads, 128]; the last query sees every
     key, so keys that precede the queries are their history. A query that sees
     no key gets 0. q, k, v may be views of one qkv row. ``cu_q``, ``cu_k`` are int32
-    on the device. Rows outside every sequence are left as ``out`` had them.
-    Returns [tokens, n_heads * 128].
+    on the device. Rows outside every sequence are left as ``out`` had them (without
+    ``out`` they hold whatever the memory did); ``out`` overlaps no input. ``scale`` is
+    positive and below 2e38 (default: 128^-1/2). Returns [tokens, n_heads * 128].
     """
     idx, code = _first(q)
     dt = q.dtype

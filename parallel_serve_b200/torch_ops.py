@@ -25,6 +25,8 @@ implementation, so they appear as single operators to the profiler, to
   parallel_serve::prompt_attention(Tensor q, Tensor k, Tensor v, Tensor cu_q, Tensor cu_k) -> Tensor
 
 A 4-bit pool is the four tensors of ``KV4Pool`` as a list, empty for a model without sequences.
+These forms have the calls' defaults only: ``ops.kv4_append`` also takes q, norms and the rotation,
+the attentions a scale, and ``ops.kv4_gather`` reads rows back.
 
 Every CUDA implementation is the same ctypes call into libparallel_serve.so
 that the Python API makes (one kernel launch on the current stream, no host
